@@ -52,9 +52,13 @@ from .ops import (  # noqa: E402
 from .quant import (dequantize_int4_group_wise, dequantize_linear_per_channel,  # noqa: E402
                     quantize_int4_group_wise, quantize_int4_per_channel,
                     quantize_linear_per_channel)
+from .kv8 import (KV8Cache, KV8Plan, kv8_append, kv8_attention, kv8_plan, kv8_read,  # noqa: E402
+                  qk_norm_rope, rope_table)
 from .nn import W4A16Linear, W8A16Embedding, W8A16Linear  # noqa: E402
 
 __all__ = [
+    "KV8Cache",
+    "KV8Plan",
     "LAYOUT_ROWMAJOR",
     "LAYOUT_TILE16X64",
     "KERNEL_AUTO",
@@ -66,6 +70,10 @@ __all__ = [
     "W8A16Linear",
     "dequantize_int4_group_wise",
     "dequantize_linear_per_channel",
+    "kv8_append",
+    "kv8_attention",
+    "kv8_plan",
+    "kv8_read",
     "linear",
     "linear_argmax",
     "linear_into",
@@ -76,9 +84,11 @@ __all__ = [
     "pack_weight_int4",
     "packed_shape",
     "packed_shape_int4",
+    "qk_norm_rope",
     "quantize_int4_group_wise",
     "quantize_int4_per_channel",
     "quantize_linear_per_channel",
+    "rope_table",
     "select_kernel",
     "unpack_weight",
     "unpack_weight_int4",

@@ -1,7 +1,7 @@
 """Build the native pieces in-tree (no JIT cache, no pip install).
 
 * ``lib/librf_w8a16.so``       -- gfx950 HIP kernels + the C ABI (hipcc)
-* ``lib/librf_w8a16_torch.so`` -- the thin torch-library op (g++ against
+* ``lib/librf_w8a16_torch.so`` -- the thin torch-library ops (g++ against
   the installed PyTorch-ROCm headers), linked to the C-ABI library
 * ``lib/librf_bench.so``       -- bench.py's streaming-read reference kernel
   (a measurement helper, not part of the C ABI)
@@ -25,7 +25,9 @@ CSRC = PKG / "csrc"
 LIBDIR = PKG / "lib"
 INCLUDE = ROOT / "include"
 
-CAPI_SOURCES = ["w8a16_capi.hip", "w8a16_gemv.hip", "w8a16_gemm.hip", "w8a16_quant.hip"]
+CAPI_SOURCES = ["w8a16_capi.hip", "w8a16_gemv.hip", "w8a16_gemm.hip", "w8a16_quant.hip",
+                "kv8_capi.hip", "kv8_cache.hip", "kv8_attn.hip"]
+TORCH_SOURCES = ["w8a16_torch.cpp", "kv8_torch.cpp"]
 CAPI_LIB = LIBDIR / "librf_w8a16.so"
 TORCH_LIB = LIBDIR / "librf_w8a16_torch.so"
 BENCH_LIB = LIBDIR / "librf_bench.so"
@@ -97,7 +99,7 @@ def build_torch_op(verbose: bool = False) -> Path:
            "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
            "-DTORCH_EXTENSION_NAME=rf_w8a16_torch",
            *[f"-I{p}" for p in inc], "-I/opt/rocm/include", f"-I{INCLUDE}",
-           str(CSRC / "w8a16_torch.cpp"),
+           *[str(CSRC / s) for s in TORCH_SOURCES],
            f"-L{libdir}", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip", "-ltorch_hip",
            f"-L{LIBDIR}", "-lrf_w8a16", "-Wl,-rpath,$ORIGIN",
            "-Wl,-soname,librf_w8a16_torch.so",

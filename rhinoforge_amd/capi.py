@@ -1,4 +1,4 @@
-"""ctypes binding of the C ABI in include/w8a16.h.
+"""ctypes binding of the C ABI in include/w8a16.h and include/kv8.h.
 
 This is the binding a Python host (such as the reference's runtime) would add
 to call the library without the torch op.  It loads ``lib/librf_w8a16.so``;
@@ -128,6 +128,61 @@ SIGNATURES = {
                                    _c.c_void_p, _c.c_size_t, _c.c_void_p]),
 }
 
+class KV8Cache(ctypes.Structure):
+    """struct rf_kv8_cache (include/kv8.h)."""
+    _fields_ = [("k", _c.c_void_p), ("v", _c.c_void_p), ("k_scale", _c.c_void_p),
+                ("v_scale", _c.c_void_p), ("num_blocks", _c.c_int64), ("kv_heads", _c.c_int32),
+                ("head_dim", _c.c_int32), ("block_size", _c.c_int32)]
+
+
+class KV8Heads(ctypes.Structure):
+    """struct rf_kv8_heads."""
+    _fields_ = [("data", _c.c_void_p), ("token_stride", _c.c_int64), ("head_stride", _c.c_int64),
+                ("heads", _c.c_int32)]
+
+
+class KV8RopeArgs(ctypes.Structure):
+    """struct rf_kv8_rope_args."""
+    _fields_ = [("q", KV8Heads), ("k", KV8Heads), ("q_out", _c.c_void_p), ("k_out", _c.c_void_p),
+                ("q_weight", _c.c_void_p), ("k_weight", _c.c_void_p), ("cos", _c.c_void_p),
+                ("sin", _c.c_void_p), ("positions", _c.c_void_p), ("tokens", _c.c_int64),
+                ("table_rows", _c.c_int64), ("head_dim", _c.c_int32), ("rot", _c.c_int32),
+                ("dtype", _c.c_int32), ("positions64", _c.c_int32), ("interleaved", _c.c_int32),
+                ("eps", _c.c_float)]
+
+
+class KV8PlanArgs(ctypes.Structure):
+    """struct rf_kv8_plan_args."""
+    _fields_ = [(n, _c.c_void_p) for n in ("block_table", "cached", "fresh", "free_blocks",
+                                           "free_start", "slots", "positions", "cu", "kv_lens",
+                                           "free_next")] + \
+               [(n, _c.c_int64) for n in ("requests", "width", "table_stride", "num_free",
+                                          "tokens")] + [("block_size", _c.c_int32)]
+
+
+class KV8AttentionArgs(ctypes.Structure):
+    """struct rf_kv8_attention_args."""
+    _fields_ = [("cache", KV8Cache), ("q", KV8Heads), ("cu_q", _c.c_void_p),
+                ("kv_lens", _c.c_void_p), ("block_table", _c.c_void_p), ("out", _c.c_void_p),
+                ("lse", _c.c_void_p), ("workspace", _c.c_void_p), ("workspace_bytes", _c.c_size_t),
+                ("tokens", _c.c_int64), ("requests", _c.c_int64), ("width", _c.c_int64),
+                ("table_stride", _c.c_int64), ("max_q_len", _c.c_int64), ("max_kv_len", _c.c_int64),
+                ("dtype", _c.c_int32), ("causal", _c.c_int32), ("window", _c.c_int64),
+                ("scale", _c.c_float)]
+
+
+# name -> (restype, argtypes): every entry point declared in include/kv8.h
+KV8_SIGNATURES = {
+    "rf_kv8_qk_norm_rope": (_c.c_int, [_c.POINTER(KV8RopeArgs), _c.c_void_p]),
+    "rf_kv8_plan": (_c.c_int, [_c.POINTER(KV8PlanArgs), _c.c_void_p]),
+    "rf_kv8_append": (_c.c_int, [_c.POINTER(KV8Cache), _c.POINTER(KV8Heads), _c.POINTER(KV8Heads),
+                                 _c.c_int32, _c.c_void_p, _c.c_int64, _c.c_void_p]),
+    "rf_kv8_read": (_c.c_int, [_c.POINTER(KV8Cache), _c.c_void_p, _c.c_int64, _c.c_int32,
+                               _c.c_void_p, _c.c_void_p, _c.c_void_p]),
+    "rf_kv8_attention_workspace": (_c.c_size_t, [_c.POINTER(KV8AttentionArgs)]),
+    "rf_kv8_attention": (_c.c_int, [_c.POINTER(KV8AttentionArgs), _c.c_void_p]),
+}
+
 _lib = None
 
 
@@ -138,7 +193,7 @@ def load() -> ctypes.CDLL:
         if not LIB_PATH.is_file():
             raise OSError(f"{LIB_PATH} not built; run `python rhinoforge_amd/_build.py`")
         lib = ctypes.CDLL(str(LIB_PATH))
-        for name, (res, args) in SIGNATURES.items():
+        for name, (res, args) in {**SIGNATURES, **KV8_SIGNATURES}.items():
             fn = getattr(lib, name)
             fn.restype = res
             fn.argtypes = args
