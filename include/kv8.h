@@ -162,11 +162,14 @@ int rf_kv8_read(const rf_kv8_cache* cache, const int32_t* slots, int64_t n, int3
  *         lse -inf.  A block id outside the cache gives NaN.
  *   out   contiguous, q's type; lse (may be NULL) fp32 [tokens][heads], natural log
  *   scale > 0 and finite
+ *   tokens * heads < 2^31 and width * block_size <= 2^30.
  *   max_q_len, max_kv_len  the largest of each, as far as the caller knows (0:
  *         not known).  They choose the launch; results are right without them.
- *   workspace  rf_kv8_attention_workspace(args) bytes, 16-byte aligned
- *         (0: none); its contents are lost.  Calls that run at the same time
- *         need one each. */
+ *   scratch  for calls whose tokens are split over workgroups: counters as
+ *         every split launch has them (zero between calls, rf_w8a16_scratch),
+ *         and rf_kv8_attention_workspace(args) bytes of partials (0: scratch
+ *         may be NULL).  Missing or too small: RF_W8A16_EWORKSPACE, before any
+ *         launch.  Calls that run at the same time need one each. */
 typedef struct rf_kv8_attention_args {
   rf_kv8_cache cache;
   rf_kv8_heads q;
@@ -175,8 +178,7 @@ typedef struct rf_kv8_attention_args {
   const int32_t* block_table;
   void* out;
   float* lse;
-  void* workspace;
-  size_t workspace_bytes;
+  const rf_w8a16_scratch* scratch;
   int64_t tokens;
   int64_t requests;
   int64_t width;        /* entries of a block_table row */

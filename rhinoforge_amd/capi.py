@@ -164,7 +164,7 @@ class KV8AttentionArgs(ctypes.Structure):
     """struct rf_kv8_attention_args."""
     _fields_ = [("cache", KV8Cache), ("q", KV8Heads), ("cu_q", _c.c_void_p),
                 ("kv_lens", _c.c_void_p), ("block_table", _c.c_void_p), ("out", _c.c_void_p),
-                ("lse", _c.c_void_p), ("workspace", _c.c_void_p), ("workspace_bytes", _c.c_size_t),
+                ("lse", _c.c_void_p), ("scratch", _c.POINTER(Scratch)),
                 ("tokens", _c.c_int64), ("requests", _c.c_int64), ("width", _c.c_int64),
                 ("table_stride", _c.c_int64), ("max_q_len", _c.c_int64), ("max_kv_len", _c.c_int64),
                 ("dtype", _c.c_int32), ("causal", _c.c_int32), ("window", _c.c_int64),

@@ -37,85 +37,139 @@ struct AttnArgs {
   const int32_t *cu, *lens, *table;
   uint8_t* out;
   float* lse;
-  float* part;         // [tokens * heads][splits][D] fp32, unnormalized
-  floatx4* stat;       // [tokens * heads][splits] (m, l): see Stat
-  int64_t tokens, table_stride, num_blocks;
-  int requests, width, hq, hk, group, shift;
+  uint32_t* counters;  // one per tile and key head, zero between launches
+  float* part;         // [tokens * heads][splits][D], unnormalized
+  uint64_t* stat;      // [tokens * heads][splits]: m, l
+  int64_t table_stride;
+  int num_blocks;
+  int tokens, requests, width, hq, hk, group, shift;
   int per_request;     // cu == nullptr: queries of a request
-  int splits, tiles;
-  int causal;
-  int64_t window;      // 0: none
+  int splits, least, tiles;
+  bool merge;          // partial results are added by kv8_merge_kernel, else by join()
+  int causal, window;  // window 0: none
   float scale_log2e;
 };
 
-// Where a workgroup works: request, its queries, this tile's first row.
+// Where a workgroup works.  Rows (query * group + head of the group), tokens
+// and positions fit 32 bits (checked on the host).
 struct Tile {
-  int64_t first_token;  // of the request
-  int64_t queries;
-  int64_t row0;         // first row (query * group + head of the group) of the tile
-  int64_t kv_len;
+  int first_token, queries;  // of the request
+  int row0;                  // first row of the tile
+  int kv_len;
   const int32_t* table;
-  bool pad;             // the tokens past the batch: nothing is seen
 };
 
-__device__ __forceinline__ int64_t cu_at(const AttnArgs& a, int b) {
+// A value that is the same in all lanes, in a scalar register: the compiler
+// does not see it through the loads and searches below, and would carry every
+// bound, id and branch of the loops per lane (the builtin it folds away where
+// it knows the value uniform but has it in a vector register).  The wait states
+// are the ones the compiler keeps around its own instruction but cannot know
+// of here: the vector register may be written by the instruction before it,
+// and the scalar one be a load's address in the one after.
+__device__ __forceinline__ int uniform(int v) {
+  int r;
+  asm("s_nop 1\n\tv_readfirstlane_b32 %0, %1\n\ts_nop 4" : "=s"(r) : "v"(v));
+  return r;
+}
+// The same for a value that is in one: not to be merged with per-lane counters.
+__device__ __forceinline__ int opaque(int v) {
+  asm("" : "+s"(v));
+  return v;
+}
+// Ids, lengths and scales are read only, at uniform addresses: scalar loads,
+// which do not queue behind the cache's bytes.
+template <typename T>
+__device__ __forceinline__ T read_scalar(const T* p, int64_t i) {
+  return reinterpret_cast<const __attribute__((address_space(4))) T*>(reinterpret_cast<uintptr_t>(p))[i];
+}
+
+__device__ __forceinline__ int cu_at(const AttnArgs& a, int b) {
   if (b <= 0) return 0;
   if (b > a.requests) return a.tokens;
-  const int64_t c = a.cu[b];
-  return c < 0 ? 0 : c > a.tokens ? a.tokens : c;
+  return min(max(a.cu[b], 0), a.tokens);
 }
 
 // Tile x of the launch: request b's tiles begin at floor(cu[b] group / R) + b,
-// which leaves room for all of them.  Every lane looks at one boundary at a
-// time: two rounds for up to 4096 requests.
+// which leaves room for all of them.  Each lane looks at one boundary (and up
+// to 62 requests at their lengths too: one memory round trip); more requests
+// take a round per factor of 64.
 template <int R>
-__device__ bool find_tile(const AttnArgs& a, int64_t x, Tile* t) {
-  int b;
+__device__ __forceinline__ bool find_tile(const AttnArgs& a, int x, Tile* t) {
+  int b, len;
   if (a.cu == nullptr) {
-    const int64_t rows = (int64_t)a.per_request * a.group, per = (rows + R - 1) / R;
-    b = (int)(x / per);
+    const int per = (a.per_request * a.group + R - 1) / R;
+    b = (int)((unsigned)x / (unsigned)per);
     if (b >= a.requests) return false;
-    t->first_token = (int64_t)b * a.per_request;
+    t->first_token = b * a.per_request;
     t->queries = a.per_request;
-    t->row0 = (x - (int64_t)b * per) * R;
+    t->row0 = (x - b * per) * R;
+    len = a.lens[b];
   } else {
     const int lane = threadIdx.x % kWave;
-    const int last = a.requests;  // the tokens past the batch
-    int lo = 0, n = last + 1;     // the answer is in [lo, lo + n)
-    while (n > 1) {
-      const int step = (n + kWave - 1) / kWave;
-      const int at = lo + lane * step;
-      const bool below = at < lo + n && cu_at(a, at) * a.group / R + at <= x;
-      const int hits = __popcll(__ballot(below));
-      const int base = lo + (hits > 0 ? hits - 1 : 0) * step;
-      n = min(step, lo + n - base);
-      lo = base;
+    const auto begin = [&](int c, int i) { return (int)((int64_t)c * a.group / R) + i; };
+    int first, next;
+    if (a.requests < kWave - 1) {
+      const int c = cu_at(a, lane);
+      const int n = lane < a.requests ? a.lens[lane] : 0;
+      const int hits = __popcll(__ballot(lane <= a.requests && begin(c, lane) <= x));
+      b = hits - 1;
+      first = __builtin_amdgcn_readlane(c, b);
+      next = __builtin_amdgcn_readlane(c, b + 1);
+      len = __builtin_amdgcn_readlane(n, b);
+    } else {
+      int lo = 0, n = a.requests + 1;  // the answer is in [lo, lo + n)
+      while (n > 1) {
+        const int step = (n + kWave - 1) / kWave, at = lo + lane * step;
+        const bool below = at < lo + n && begin(cu_at(a, at), at) <= x;
+        const int hits = __popcll(__ballot(below));
+        const int base = lo + (hits > 0 ? hits - 1 : 0) * step;
+        n = min(step, lo + n - base);
+        lo = base;
+      }
+      b = __builtin_amdgcn_readfirstlane(lo);
+      first = cu_at(a, b);
+      next = cu_at(a, b + 1);
+      len = b < a.requests ? a.lens[b] : 0;
     }
-    b = __builtin_amdgcn_readfirstlane(lo);
-    t->first_token = cu_at(a, b);
-    const int64_t next = cu_at(a, b + 1);
-    t->queries = next > t->first_token ? next - t->first_token : 0;
-    t->row0 = (x - (t->first_token * a.group / R + b)) * R;
+    t->first_token = first;
+    t->queries = max(next - first, 0);
+    t->row0 = (x - begin(first, b)) * R;
   }
   if (t->row0 < 0 || t->row0 >= t->queries * a.group) return false;
-  t->pad = b >= a.requests;
-  const int64_t most = (int64_t)a.width << a.shift;
-  const int64_t len = t->pad ? 0 : a.lens[b];
-  t->kv_len = len < 0 ? 0 : len > most ? most : len;
-  t->table = a.table + (t->pad ? 0 : (int64_t)b * a.table_stride);
+  // (b == requests: the tokens past the batch, which see nothing)
+  b = uniform(b);
+  t->first_token = uniform(t->first_token);
+  t->queries = uniform(t->queries);
+  t->row0 = uniform(t->row0);
+  t->kv_len = uniform(min(max(len, 0), a.width << a.shift));
+  t->table = a.table + (b < a.requests ? b * a.table_stride : 0);
   return true;
 }
 
 // Tokens [lo, hi) that row `row` of a request sees.
-__device__ __forceinline__ void seen(const AttnArgs& a, const Tile& t, int64_t row, int64_t* lo,
-                                     int64_t* hi) {
+__device__ __forceinline__ void seen(const AttnArgs& a, const Tile& t, int row, int* lo, int* hi) {
   *lo = 0;
   *hi = t.kv_len;
   if (a.causal) {
-    const int64_t pos = t.kv_len - t.queries + row / a.group;
-    *hi = pos < 0 ? 0 : pos + 1 < t.kv_len ? pos + 1 : t.kv_len;
-    if (a.window > 0 && pos - a.window + 1 > 0) *lo = pos - a.window + 1;
+    const int pos = t.kv_len - t.queries + (int)((unsigned)row / (unsigned)a.group);
+    *hi = max(pos + 1, 0);
+    if (a.window > 0) *lo = max(pos - a.window + 1, 0);
   }
+}
+
+// The 32-token groups [begin, end) of one split of a tile, and how many splits
+// the tile has: the launch's, or fewer of at least `least` groups.
+struct Share {
+  int begin, end, splits;
+};
+__device__ __forceinline__ Share share_of(const AttnArgs& a, int g_lo, int g_hi, int split) {
+  const int n = max(g_hi - g_lo, 0);
+  const int per = max((n + a.splits - 1) / a.splits, a.least);
+  Share r;
+  r.begin = g_lo + min(split * per, n);
+  r.end = min(r.begin + per, g_lo + n);
+  r.splits = max((n + per - 1) / per, 1);
+  return r;
 }
 
 // One 32-token group of a head: where its bytes are and its scales.  A block id
@@ -128,12 +182,21 @@ struct Group {
 __device__ __forceinline__ Group group_of(const AttnArgs& a, const Tile& t, int h, int g) {
   Group r;
   const int per = a.shift - 5;
-  const int64_t id = t.table[g >> per];
-  r.ok = id >= 0 && id < a.num_blocks;
-  r.at = (r.ok ? id : 0) * a.hk + h;
+  const int id = read_scalar(t.table, g >> per);
+  const bool ok = (unsigned)id < (unsigned)a.num_blocks;
+  r.at = (int64_t)(ok ? id : 0) * a.hk + h;
   r.sub = g & ((1 << per) - 1);
+  r.ok = ok;
   return r;
 }
+// A scale's bits (kept as an integer: compares and branches on it are scalar).
+// Scales are not negative, so their order is that of the bits.
+constexpr uint32_t kInfBits = 0x7f800000u;
+__device__ __forceinline__ uint32_t scale_bits(const float* p, const Group& g) {
+  const uint32_t v = read_scalar(reinterpret_cast<const uint32_t*>(p), g.at);
+  return g.ok ? v : kInfBits;
+}
+__device__ __forceinline__ float as_float(uint32_t bits) { return __builtin_bit_cast(float, bits); }
 
 // Eight query values as fp16 times 2^-e.
 template <typename T>
@@ -163,18 +226,144 @@ struct Running {
 __device__ __forceinline__ float safe(float m) { return m == -__builtin_inff() ? 0.0f : m; }
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-__device__ __forceinline__ bool larger(float vs, float top) {
-  return vs > top && vs < __builtin_inff();
+// The largest value scale so far, and log2 of it.
+struct Top {
+  uint32_t bits = 0;
+  float log = -__builtin_inff();
+};
+__device__ __forceinline__ float log2_fast(float x) { return __builtin_amdgcn_logf(x); }
+
+// log2(vs / top) for the exponent, not below -60: a block of zeros (whatever
+// its p are, they add nothing) or one that adds far less than one rounding of
+// the result.
+__device__ __forceinline__ float ratio_log2(uint32_t vs, const Top& t) {
+  return fmaxf(log2_fast(as_float(vs)) - t.log, -60.0f);
 }
 
-// log2(vs / top) for the exponent.  A block of zeros counts as if its scale
-// were the largest; one 2^60 below it as 2^-60 (what it adds is far below one
-// rounding of the result).  A scale that is not finite gives NaN.
-__device__ __forceinline__ float ratio_log2(float vs, float top) {
-  if (!(vs < __builtin_inff())) return __builtin_nanf("");
-  if (vs == 0.0f || vs == top) return 0.0f;
-  const float r = vs / top;
-  return r < 0x1p-60f ? -60.0f : __builtin_amdgcn_logf(r);
+// A group with a scale that is not finite (or negative): its scores become NaN
+// (those of tokens that a row does not see are overwritten after that) and the
+// scales harmless.
+__device__ __forceinline__ bool not_finite(uint32_t ks, uint32_t vs) {
+  return (ks > vs ? ks : vs) >= kInfBits;
+}
+constexpr uint32_t kOneBits = 0x3f800000u;
+// Inside a branch on a uniform condition: keeps the compiler from turning it
+// into a select per value that every group would pay for.
+__device__ __forceinline__ void keep_branch() { asm volatile(""); }
+
+// ---------------------------------------------------------------------------
+// Splits of one tile.  Each workgroup stores its rows' sums and (m, l), waits
+// for its stores and counts itself; the last one adds all of them in split
+// order, so the order of arrival does not show.  Stores and loads go past the
+// XCD's own L2 (device scope).  One workgroup adds at what its own loads in
+// flight allow: where a tile has many rows a second kernel does it (4 requests
+// of 50 queries, 8 heads of 256, 8 splits: 87 us with join(), 36 with it).
+// ---------------------------------------------------------------------------
+constexpr int kThreads = 256;
+
+__device__ __forceinline__ void store2(void* p, float a, float b) {
+  const uint64_t v = (uint64_t)__builtin_bit_cast(uint32_t, b) << 32 | __builtin_bit_cast(uint32_t, a);
+  __hip_atomic_store((uint64_t*)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void load2(const void* p, float* a, float* b) {
+  const uint64_t v = __hip_atomic_load((uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  *a = __builtin_bit_cast(float, (uint32_t)v);
+  *b = __builtin_bit_cast(float, (uint32_t)(v >> 32));
+}
+
+// Output row of tile row rc: token * heads + head.
+__device__ __forceinline__ int64_t out_row(const AttnArgs& a, const Tile& t, int h, int rc) {
+  const int row = t.row0 + rc, qi = (int)((unsigned)row / (unsigned)a.group);
+  return (int64_t)(t.first_token + qi) * a.hq + h * a.group + (row - qi * a.group);
+}
+
+template <typename T>
+__device__ __forceinline__ void finish(const AttnArgs& a, int64_t to, int D, int d, floatx8 o, float m,
+                                       float l) {
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  if (l == 0.0f) o = 0.0f;
+  Eight<T>::store(a.out + (to * D + d) * 2, o * inv);
+  if (d == 0 && a.lse)
+    a.lse[to] = l == 0.0f ? -__builtin_inff() : (m - kShift + log2_fast(l)) * kLn2;
+}
+
+// A split with nothing to do, for kv8_merge_kernel.
+__device__ __forceinline__ void no_share(const AttnArgs& a, const Tile& t, int h, int rows, int split) {
+  for (int rc = threadIdx.x; rc < rows; rc += kThreads)
+    store2(a.stat + out_row(a, t, h, rc) * a.splits + split, -__builtin_inff(), 0.0f);
+}
+
+// All threads call it after their stores of partial results.  buf: LDS of
+// rows * splits * 8 + 8192 bytes, free for use.
+template <typename T, int D>
+__device__ void join(const AttnArgs& a, const Tile& t, int h, int rows, int splits, uint32_t* counter,
+                     float* buf) {
+  const int tid = threadIdx.x;
+  __shared__ int is_last;
+  __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wavefront's stores are done
+  __syncthreads();
+  if (tid == 0) {
+    const uint32_t before =
+        __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    is_last = before == (uint32_t)(splits - 1);
+    if (is_last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (!is_last) return;
+  float* stat = buf;                        // [rows][splits][m, l]
+  floatx8* sums = reinterpret_cast<floatx8*>(buf + rows * splits * 2);
+  for (int i = tid; i < rows * splits; i += kThreads) {
+    const int rc = i / splits;
+    float m, l;
+    load2(a.stat + out_row(a, t, h, rc) * a.splits + (i - rc * splits), &m, &l);
+    stat[2 * i] = m;
+    stat[2 * i + 1] = l;
+  }
+  __syncthreads();
+  // One thread per row and eight dimensions; where that leaves threads over,
+  // `ways` of them share the splits and meet in LDS.
+  const int units = rows * (D / 8);
+  int ways = 1;
+  while (units * ways * 2 <= kThreads && ways * 2 <= splits) ways *= 2;
+  for (int u0 = 0; u0 < units; u0 += kThreads) {
+    const int way = ways == 1 ? 0 : tid / units, u = u0 + (ways == 1 ? tid : tid - way * units);
+    const bool on = u < units && way < ways;
+    const int rc = on ? u / (D / 8) : 0, d = u % (D / 8) * 8;
+    float m = -__builtin_inff(), l = 0.0f;
+    floatx8 o = 0.0f;
+    const int64_t to = out_row(a, t, h, rc);
+    if (on) {
+      const float* st = stat + rc * splits * 2;
+      for (int s = 0; s < splits; ++s) m = fmaxf(m, st[2 * s]);
+      const float* part = a.part + to * a.splits * D + d;
+#pragma unroll 4
+      for (int s = way; s < splits; s += ways) {
+        floatx8 x;
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+          float lo, hi;
+          load2(part + (int64_t)s * D + j, &lo, &hi);
+          x[j] = lo;
+          x[j + 1] = hi;
+        }
+        const float f = exp2_fast(st[2 * s] - safe(m));
+        l += st[2 * s + 1] * f;
+        o += x * f;
+      }
+    }
+    if (ways > 1) {
+      // (units <= 128 here: one turn of the outer loop)
+      sums[tid] = o;
+      __syncthreads();
+      if (on && way == 0) {
+        for (int w = 1; w < ways; ++w) o += sums[tid + w * units];
+        l = 0.0f;
+        const float* st = stat + rc * splits * 2;
+        for (int s = 0; s < splits; ++s) l += st[2 * s + 1] * exp2_fast(st[2 * s] - safe(m));
+      }
+    }
+    if (on && way == 0) finish<T>(a, to, D, d, o, m, l);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -188,7 +377,7 @@ constexpr int kWaves = 4;
 template <int D>
 struct Bytes {
   uint4 k[D / 32], v[D / 32];
-  float ks, vs;
+  uint32_t ks, vs;
 };
 
 template <int D>
@@ -200,9 +389,8 @@ __device__ __forceinline__ void fetch(const AttnArgs& a, const Group& g, int lan
   for (int i = 0; i < D / 32; ++i) b.k[i] = load_u4_stream(kp + i * kTileBytes + lane * 16);
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) b.v[i] = load_u4_stream(vp + i * kTileBytes + lane * 16);
-  const float nan = __builtin_nanf("");
-  b.ks = g.ok ? a.ks[g.at] : nan;
-  b.vs = g.ok ? a.vs[g.at] : nan;
+  b.ks = scale_bits(a.ks, g);
+  b.vs = scale_bits(a.vs, g);
 }
 
 template <typename T, int D, int RT>
@@ -210,29 +398,37 @@ __global__ __launch_bounds__(kWaves* kWave) void kv8_decode_kernel(AttnArgs a) {
   constexpr int R = 16 * RT;
   __shared__ __align__(16) float red[kWaves][16][D + 4];
   __shared__ float red_m[kWaves][R], red_l[kWaves][R];
-  __shared__ float red_v[kWaves];
   const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int col = lane % 16, lg = lane / 16;
-  int64_t id = blockIdx.x;
-  const int h = (int)(id % a.hk);
-  id /= a.hk;
-  const int split = (int)(id % a.splits);
+  const unsigned id = blockIdx.x, pair = id / (unsigned)a.hk;
+  const int h = (int)(id - pair * a.hk), x = (int)(pair / (unsigned)a.splits);
   Tile t;
-  if (!find_tile<R>(a, id / a.splits, &t)) return;
-  const int64_t rows = t.queries * a.group;
+  if (!find_tile<R>(a, x, &t)) return;
+  const int rows = min(t.queries * a.group - t.row0, R);  // of this tile
+  // its first and last rows bound what any row sees
+  int lo_min, lo_max, hi_min, hi_max;
+  seen(a, t, t.row0, &lo_min, &hi_min);
+  seen(a, t, t.row0 + rows - 1, &lo_max, &hi_max);
+  lo_max = uniform(lo_max), hi_min = uniform(hi_min);
+  const int split = (int)(pair - (unsigned)x * a.splits);
+  const Share share = share_of(a, lo_min >> 5, (hi_max + 31) >> 5, split);
+  if (split >= share.splits) {
+    if (a.merge) no_share(a, t, h, rows, split);
+    return;
+  }
+  const int begin = uniform(share.begin), end = uniform(share.end);
+  const bool partial = share.splits > 1 || a.merge;
 
   // ---- queries, as B operands: column = row, 16 dimensions 64 kb + 16 lg + ..
   half8 q[RT][D / 32];
   float factor[RT];
-  int64_t lo[RT], hi[RT];
-  int64_t lo_min = INT64_MAX, lo_max = 0, hi_min = INT64_MAX, hi_max = 0;
+  int lo[RT], hi[RT];
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
-    int64_t row = t.row0 + 16 * r + col;
-    if (row >= rows) row = rows - 1;
-    const int64_t qi = row / a.group;
-    const uint8_t* p = a.q + (t.first_token + qi) * a.q_ts +
-                       (h * a.group + (row - qi * a.group)) * a.q_hs + lg * 32;
+    const int row = t.row0 + min(16 * r + col, rows - 1);
+    const int qi = (int)((unsigned)row / (unsigned)a.group);
+    const uint8_t* p = a.q + (int64_t)(t.first_token + qi) * a.q_ts +
+                       (int64_t)(h * a.group + (row - qi * a.group)) * a.q_hs + lg * 32;
     uint4 raw[D / 32];
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) raw[i] = load_u4(p + (i / 2) * 128 + (i % 2) * 16);
@@ -255,24 +451,9 @@ __global__ __launch_bounds__(kWaves* kWave) void kv8_decode_kernel(AttnArgs a) {
     }
     seen(a, t, row, &lo[r], &hi[r]);
   }
-  // the tile's first and last rows bound what any row sees
-  {
-    const int64_t last = min(t.row0 + R, rows) - 1;
-    seen(a, t, t.row0, &lo_min, &hi_min);
-    seen(a, t, last, &lo_max, &hi_max);
-  }
-  const int g_lo = (int)(lo_min >> 5), g_hi = (int)((hi_max + 31) >> 5);
-  int begin = g_lo, end = g_hi;
-  if (a.splits > 1) {
-    const int n = g_hi - g_lo;
-    const int per = max((n + a.splits - 1) / a.splits, kWaves);
-    begin = min(g_lo + split * per, g_hi);
-    end = min(begin + per, g_hi);
-  }
-
   floatx4 acc[RT][D / 16];
   Running run[RT];
-  float top = 0.0f;  // largest vs so far
+  Top top;
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     run[r] = {-__builtin_inff(), 0.0f};
@@ -297,31 +478,48 @@ __global__ __launch_bounds__(kWaves* kWave) void kv8_decode_kernel(AttnArgs a) {
         }
       }
     }
-    const int64_t t0 = (int64_t)g << 5;
+    uint32_t ks = b.ks, vs = b.vs;
+    if (not_finite(ks, vs)) {
+      keep_branch();
+      ks = kOneBits;
+      vs = 0;
+#pragma unroll
+      for (int r = 0; r < RT; ++r) s[r][0] = s[r][1] = __builtin_nanf("");
+    }
+    const int t0 = opaque(g << 5);
     const bool edge = t0 < lo_max || t0 + 32 > hi_min;
-    bool raise = larger(b.vs, top);
+    bool raise = vs > top.bits;
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-      const float c = b.ks * factor[r];
+      const float c = as_float(ks) * factor[r];
+      const int first = lo[r] - t0 - 4 * lg, past = hi[r] - t0 - 4 * lg;
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt) s[r][tt] *= c;
+      if (edge) {
+        keep_branch();
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int tok = 16 * tt + i;  // past t0 + 4 lg
+            s[r][tt][i] = (tok < first) | (tok >= past) ? -__builtin_inff() : s[r][tt][i];
+          }
+      }
       float mx = -__builtin_inff();
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float x = s[r][tt][i] * c;
-          if (edge) {
-            const int64_t tok = t0 + 16 * tt + 4 * lg + i;
-            if (tok < lo[r] || tok >= hi[r]) x = -__builtin_inff();
-          }
-          s[r][tt][i] = x;
-          mx = fmaxf(mx, x);
-        }
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[r][tt][i]);
       raise |= mx > run[r].m + (run[r].m == -__builtin_inff() ? 0.0f : kRaise);
     }
     if (__ballot(raise)) {
-      const float to = larger(b.vs, top) ? b.vs : top;
-      const float fv = to > 0.0f ? top / to : 1.0f;
-      top = to;
+      float fv = 1.0f;
+      if (vs > top.bits) {
+        const float log = log2_fast(as_float(vs));
+        fv = exp2_fast(top.log - log);
+        top.bits = vs;
+        top.log = log;
+      }
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
         float mx = run[r].m;
@@ -339,7 +537,7 @@ __global__ __launch_bounds__(kWaves* kWave) void kv8_decode_kernel(AttnArgs a) {
         for (int i = 0; i < D / 16; ++i) acc[r][i] *= fa;
       }
     }
-    const float lr = ratio_log2(b.vs, top), back = exp2_fast(-lr);
+    const float lr = ratio_log2(vs, top), back = exp2_fast(-lr);
     half8 p[RT];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
@@ -350,11 +548,10 @@ __global__ __launch_bounds__(kWaves* kWave) void kv8_decode_kernel(AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float e = exp2_fast(s[r][tt][i] + off);
-          if (edge && s[r][tt][i] == -__builtin_inff()) e = 0.0f;
           sum += e;
           p[r][tt * 4 + i] = (_Float16)e;
         }
-      run[r].l += sum == 0.0f ? 0.0f : sum * back;  // (0 of a group whose scale is not finite)
+      run[r].l += sum * back;
     }
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) {
@@ -401,7 +598,6 @@ __global__ __launch_bounds__(kWaves* kWave) void kv8_decode_kernel(AttnArgs a) {
       red_l[wave][16 * r + col] = l;
     }
   }
-  if (lane == 0) red_v[wave] = top;
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     __syncthreads();
@@ -410,15 +606,14 @@ __global__ __launch_bounds__(kWaves* kWave) void kv8_decode_kernel(AttnArgs a) {
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) m = fmaxf(m, red_m[w][rr]);
     // nothing seen by this wavefront: its sums are 0 and their factor too
-    const float f = exp2_fast(run[r].m - safe(m)) * top;
+    const float f = exp2_fast(run[r].m - safe(m)) * as_float(top.bits);
 #pragma unroll
     for (int i = 0; i < D / 16; ++i)
       *reinterpret_cast<floatx4*>(&red[wave][col][16 * i + 4 * lg]) = acc[r][i] * f;
     __syncthreads();
     for (int it = tid; it < 16 * (D / 8); it += kWaves * kWave) {
       const int c = it / (D / 8), d = it % (D / 8) * 8, rc = 16 * r + c;
-      const int64_t row = t.row0 + rc;
-      if (row >= rows) continue;
+      if (rc >= rows) continue;
       float mm = red_m[0][rc];
 #pragma unroll
       for (int w = 1; w < kWaves; ++w) mm = fmaxf(mm, red_m[w][rc]);
@@ -431,21 +626,19 @@ __global__ __launch_bounds__(kWaves* kWave) void kv8_decode_kernel(AttnArgs a) {
         const floatx4 y = *reinterpret_cast<const floatx4*>(&red[w][c][d + 4]);
         o += __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
       }
-      const int64_t qi = row / a.group;
-      const int64_t to = (t.first_token + qi) * a.hq + h * a.group + (row - qi * a.group);
-      if (a.splits > 1) {
+      const int64_t to = out_row(a, t, h, rc);
+      if (partial) {
         float* part = a.part + (to * a.splits + split) * D + d;
-        *reinterpret_cast<floatx8*>(part) = o;
-        if (d == 0) a.stat[to * a.splits + split] = floatx4{mm, l, 0, 0};
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) store2(part + j, o[j], o[j + 1]);
+        if (d == 0) store2(a.stat + to * a.splits + split, mm, l);
       } else {
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        if (l == 0.0f) o = 0.0f;
-        Eight<T>::store(a.out + (to * D + d) * 2, o * inv);
-        if (d == 0 && a.lse)
-          a.lse[to] = l == 0.0f ? -__builtin_inff() : (mm - kShift + __builtin_amdgcn_logf(l)) * kLn2;
+        finish<T>(a, to, D, d, o, mm, l);
       }
     }
   }
+  if (partial && !a.merge)
+    join<T, D>(a, t, h, rows, share.splits, a.counters + (unsigned)x * a.hk + h, &red[0][0][0]);
 }
 
 // ---------------------------------------------------------------------------
@@ -465,21 +658,33 @@ __attribute__((amdgpu_waves_per_eu(RT == 1 ? 2 : 1))) void kv8_prefill_kernel(At
   constexpr int NG = D <= 128 ? 2 : 1;          // 32-token groups of a step
   constexpr int kBuf = NG * 32 * D * 2 * 2;     // bytes of a step's K and V in fp16
   constexpr int kChunks = NG * D / 128;         // 16-byte chunks of K (and of V) per thread
+  constexpr bool kQLds = D > 128;               // see below
+  // (sized at the launch: with the size known here the register allocator
+  // trades registers for it, and spills)
   extern __shared__ __align__(16) uint8_t lds[];
   const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int col = lane % 32, lh = lane / 32;
-  int64_t id = blockIdx.x;
-  const int h = (int)(id % a.hk);
-  id /= a.hk;
-  const int split = (int)(id % a.splits);
-  Tile t;
+  const unsigned id = blockIdx.x, pair = id / (unsigned)a.hk;
+  const int h = (int)(id - pair * a.hk), turn = (int)(pair / (unsigned)a.splits);
+  const int split = (int)(pair - (unsigned)turn * a.splits);
   // the last tiles of a request see the most tokens: they begin first
-  if (!find_tile<R>(a, a.tiles - 1 - id / a.splits, &t)) return;
-  const int64_t rows = t.queries * a.group;
+  const int x = a.tiles - 1 - turn;
+  Tile t;
+  if (!find_tile<R>(a, x, &t)) return;
+  const int rows = min(t.queries * a.group - t.row0, R);  // of this tile
+  int lo_min, hi_max, unused;
+  seen(a, t, t.row0, &lo_min, &unused);
+  seen(a, t, t.row0 + rows - 1, &unused, &hi_max);
+  const Share share = share_of(a, lo_min >> 5, (hi_max + 31) >> 5, split);
+  if (split >= share.splits) {
+    no_share(a, t, h, rows, split);
+    return;
+  }
+  const int begin = uniform(share.begin), end = uniform(share.end);
+  const bool partial = a.splits > 1;  // kv8_merge_kernel adds them
 
   // Size 256: the sums take 128 registers, so the queries stay in LDS, where
   // each lane reads its own.
-  constexpr bool kQLds = D > 128;
   half8 q[RT][kQLds ? 1 : D / 16];
   half8* q_lds = reinterpret_cast<half8*>(lds + 2 * kBuf) + wave * (RT * D / 16) * kWave + lane;
   const auto put_q = [&](int r, int i, half8 v) {
@@ -491,16 +696,14 @@ __attribute__((amdgpu_waves_per_eu(RT == 1 ? 2 : 1))) void kv8_prefill_kernel(At
     else return q[r][i];
   };
   float factor[RT];
-  int64_t lo[RT], hi[RT];
-  int64_t my_lo_min, my_lo_max, my_hi_min, my_hi_max, lo_min, hi_max, unused;
-  const int64_t wrow = t.row0 + wave * 32 * RT;
+  int lo[RT], hi[RT];
+  const int wrow = wave * 32 * RT;  // this wavefront's first row of the tile
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
-    int64_t row = wrow + 32 * r + col;
-    if (row >= rows) row = rows - 1;
-    const int64_t qi = row / a.group;
-    const uint8_t* p = a.q + (t.first_token + qi) * a.q_ts +
-                       (h * a.group + (row - qi * a.group)) * a.q_hs + lh * 16;
+    const int row = t.row0 + min(wrow + 32 * r + col, rows - 1);
+    const int qi = (int)((unsigned)row / (unsigned)a.group);
+    const uint8_t* p = a.q + (int64_t)(t.first_token + qi) * a.q_ts +
+                       (int64_t)(h * a.group + (row - qi * a.group)) * a.q_hs + lh * 16;
     uint4 raw[D / 16];
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) raw[i] = load_u4(p + i * 32);
@@ -522,23 +725,16 @@ __attribute__((amdgpu_waves_per_eu(RT == 1 ? 2 : 1))) void kv8_prefill_kernel(At
     }
     seen(a, t, row, &lo[r], &hi[r]);
   }
-  seen(a, t, t.row0, &lo_min, &unused);
-  seen(a, t, min(t.row0 + R, rows) - 1, &unused, &hi_max);
   const bool idle = wrow >= rows;
-  seen(a, t, idle ? rows - 1 : wrow, &my_lo_min, &my_hi_min);
-  seen(a, t, min(wrow + 32 * RT, rows) - 1, &my_lo_max, &my_hi_max);
-  const int g_lo = (int)(lo_min >> 5), g_hi = (int)((hi_max + 31) >> 5);
-  int begin = g_lo, end = g_hi;
-  if (a.splits > 1) {
-    const int n = g_hi - g_lo;
-    const int per = max((n + a.splits - 1) / a.splits, NG);
-    begin = min(g_lo + split * per, g_hi);
-    end = min(begin + per, g_hi);
-  }
+  int my_lo_min, my_lo_max, my_hi_min, my_hi_max;
+  seen(a, t, t.row0 + min(wrow, rows - 1), &my_lo_min, &my_hi_min);
+  seen(a, t, t.row0 + min(wrow + 32 * RT, rows) - 1, &my_lo_max, &my_hi_max);
+  my_lo_min = uniform(my_lo_min), my_lo_max = uniform(my_lo_max);
+  my_hi_min = uniform(my_hi_min), my_hi_max = uniform(my_hi_max);
 
   floatx16 acc[RT][D / 32];
   Running run[RT];
-  float top = 0.0f;
+  Top top;
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     run[r] = {-__builtin_inff(), 0.0f};
@@ -546,16 +742,28 @@ __attribute__((amdgpu_waves_per_eu(RT == 1 ? 2 : 1))) void kv8_prefill_kernel(At
     for (int i = 0; i < D / 32; ++i) acc[r][i] = 0.0f;
   }
 
-  // Chunk c of this wavefront is 1 KB tile c * kWaves + wave of the step.
+  // Chunk c of this wavefront is 1 KB tile c * kWaves + wave of the step.  A
+  // step's bytes and scales are loaded one step ahead, its block ids two.
   uint4 kr[kChunks], vr[kChunks];
-  const auto load = [&](int g) {
+  Group ids[NG];
+  uint32_t ks_next[NG], vs_next[NG];
+  const auto look = [&](int g) {
+#pragma unroll
+    for (int n = 0; n < NG; ++n) ids[n] = group_of(a, t, h, min(g + n, end - 1));
+  };
+  const auto load = [&] {
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
       const int tile = c * kWaves + wave;
-      const Group gr = group_of(a, t, h, min(g + tile / (D / 32), end - 1));
+      const Group& gr = NG == 1 || (D == 64 ? wave < 2 : c == 0) ? ids[0] : ids[NG - 1];
       const int64_t at = (gr.at << a.shift) * D + gr.sub * (32 * D) + tile % (D / 32) * kTileBytes + lane * 16;
       kr[c] = load_u4(a.k + at);
       vr[c] = load_u4(a.v + at);
+    }
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      ks_next[n] = scale_bits(a.ks, ids[n]);
+      vs_next[n] = scale_bits(a.vs, ids[n]);
     }
   };
   const int g16 = lane / 16, l16 = lane % 16;
@@ -578,14 +786,12 @@ __attribute__((amdgpu_waves_per_eu(RT == 1 ? 2 : 1))) void kv8_prefill_kernel(At
       }
     }
   };
-  const auto step = [&](const uint8_t* buf, int g) {
+  const auto step = [&](const uint8_t* buf, int g, const uint32_t (&kss)[NG], const uint32_t (&vss)[NG]) {
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
-      const int64_t t0 = (int64_t)(g + n) << 5;
+      const int t0 = opaque((g + n) << 5);
       if (g + n >= end || idle || t0 >= my_hi_max || t0 + 32 <= my_lo_min) continue;
-      const Group gr = group_of(a, t, h, g + n);
-      const float nan = __builtin_nanf("");
-      const float ks = gr.ok ? a.ks[gr.at] : nan, vs = gr.ok ? a.vs[gr.at] : nan;
+      uint32_t ks = kss[n], vs = vss[n];
       floatx16 s[RT];
 #pragma unroll
       for (int r = 0; r < RT; ++r) s[r] = 0.0f;
@@ -595,27 +801,41 @@ __attribute__((amdgpu_waves_per_eu(RT == 1 ? 2 : 1))) void kv8_prefill_kernel(At
 #pragma unroll
         for (int r = 0; r < RT; ++r) s[r] = mfma32x32x16(k, get_q(r, i), s[r]);
       }
+      if (not_finite(ks, vs)) {
+        keep_branch();
+        ks = kOneBits;
+        vs = 0;
+#pragma unroll
+        for (int r = 0; r < RT; ++r) s[r] = __builtin_nanf("");
+      }
       const bool edge = t0 < my_lo_max || t0 + 32 > my_hi_min;
-      bool raise = larger(vs, top);
+      bool raise = vs > top.bits;
       float c[RT];
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
-        c[r] = ks == 0.0f ? 1.0f : ks * factor[r];  // (a block of zeros: every score is 0)
+        const int first = lo[r] - t0 - 4 * lh, past = hi[r] - t0 - 4 * lh;
+        c[r] = ks == 0 ? 1.0f : as_float(ks) * factor[r];  // (a block of zeros: every score is 0)
+        if (edge) {
+          keep_branch();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int tok = 16 * (i / 4 % 2) + 8 * (i / 8) + i % 4;  // past t0 + 4 lh
+            s[r][i] = (tok < first) | (tok >= past) ? -__builtin_inff() : s[r][i];
+          }
+        }
         float mx = -__builtin_inff();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          if (edge) {
-            const int64_t tok = t0 + 16 * (i / 4 % 2) + 4 * (2 * (i / 8) + lh) + i % 4;
-            if (tok < lo[r] || tok >= hi[r]) s[r][i] = -__builtin_inff();
-          }
-          mx = fmaxf(mx, s[r][i]);
-        }
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[r][i]);
         raise |= mx * c[r] > run[r].m + (run[r].m == -__builtin_inff() ? 0.0f : kRaise);
       }
       if (__ballot(raise)) {
-        const float to = larger(vs, top) ? vs : top;
-        const float fv = to > 0.0f ? top / to : 1.0f;
-        top = to;
+        float fv = 1.0f;
+        if (vs > top.bits) {
+          const float log = log2_fast(as_float(vs));
+          fv = exp2_fast(top.log - log);
+          top.bits = vs;
+          top.log = log;
+        }
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
           float mx = -__builtin_inff();
@@ -631,7 +851,14 @@ __attribute__((amdgpu_waves_per_eu(RT == 1 ? 2 : 1))) void kv8_prefill_kernel(At
           for (int i = 0; i < D / 32; ++i) acc[r][i] *= fa;
         }
       }
-      const float lr = ratio_log2(vs, top), back = exp2_fast(-lr);
+      // (a branch the compiler cannot fold: in one block with the merge above it
+      // would keep the sums twice, 241 registers instead of 189, and spill at 256)
+      float lr = 0.0f;
+      if (vs != top.bits) {
+        lr = ratio_log2(vs, top);
+        asm volatile("" : "+v"(lr));
+      }
+      const float back = exp2_fast(-lr);
       half8 p[RT][2];
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
@@ -640,11 +867,10 @@ __attribute__((amdgpu_waves_per_eu(RT == 1 ? 2 : 1))) void kv8_prefill_kernel(At
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           float e = exp2_fast(__builtin_fmaf(s[r][i], c[r], off));
-          if (edge && s[r][i] == -__builtin_inff()) e = 0.0f;
           sum += e;
           p[r][i / 8][i % 8] = (_Float16)e;
         }
-        run[r].l += sum == 0.0f ? 0.0f : sum * back;  // (0 of a group whose scale is not finite)
+        run[r].l += sum * back;
       }
 #pragma unroll
       for (int i = 0; i < D / 32; ++i)
@@ -659,92 +885,115 @@ __attribute__((amdgpu_waves_per_eu(RT == 1 ? 2 : 1))) void kv8_prefill_kernel(At
   };
 
   if (begin < end) {
-    load(begin);
+    look(begin);
+    load();
+    look(begin + NG);
     stage(lds);
     __syncthreads();
     int at = 0;
     for (int g = begin; g < end; g += NG) {
-      const bool more = g + NG < end;
-      if (more) load(g + NG);
-      step(lds + at * kBuf, g);
-      if (more) stage(lds + (1 - at) * kBuf);
+      uint32_t ks[NG], vs[NG];
+#pragma unroll
+      for (int n = 0; n < NG; ++n) {
+        ks[n] = ks_next[n];
+        vs[n] = vs_next[n];
+      }
+      load();  // (past the end: the last group again, not used)
+      look(g + 2 * NG);
+      step(lds + at * kBuf, g, ks, vs);
+      stage(lds + (1 - at) * kBuf);
       __syncthreads();
       at = 1 - at;
     }
   }
 
+  // Rows go out through LDS (each wavefront its own part, free after the last
+  // barrier), 64 dimensions at a time: straight from the registers every lane
+  // would store four values of another row.
+  constexpr int kPitch = 64 + 4;
+  float* mine = reinterpret_cast<float*>(lds) + wave * 32 * kPitch;
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
-    const int64_t row = wrow + 32 * r + col;
     float l = run[r].l;
     l += __shfl_xor(l, 32);
-    if (row >= rows) continue;
-    const int64_t qi = row / a.group;
-    const int64_t to = (t.first_token + qi) * a.hq + h * a.group + (row - qi * a.group);
-    const float f = a.splits > 1 ? top : l == 0.0f ? 0.0f : top / l;
+    const int left = rows - wrow - 32 * r;  // rows of this wavefront's tile
+    const float f = partial ? as_float(top.bits) : l == 0.0f ? 0.0f : as_float(top.bits) / l;
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i)
+    for (int i = 0; i < D / 32; i += 2) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 8; ++j) {
         floatx4 o;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) o[c] = acc[r][i][4 * j + c] * f;
-        const int d = 32 * i + 8 * j + 4 * lh;
-        if (a.splits > 1) {
-          *reinterpret_cast<floatx4*>(a.part + (to * a.splits + split) * D + d) = o;
+        for (int c = 0; c < 4; ++c) o[c] = acc[r][i + j / 4][4 * (j % 4) + c] * f;
+        *reinterpret_cast<floatx4*>(mine + col * kPitch + 8 * j + 4 * lh) = o;
+      }
+      const int d = lane % 8 * 8;
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const int rr = 8 * n + lane / 8;
+        if (rr >= left) continue;
+        const float* src = mine + rr * kPitch + d;
+        const floatx4 x = *reinterpret_cast<const floatx4*>(src);
+        const floatx4 y = *reinterpret_cast<const floatx4*>(src + 4);
+        const int64_t to = out_row(a, t, h, wrow + 32 * r + rr);
+        if (partial) {
+          float* part = a.part + (to * a.splits + split) * D + 32 * i + d;
+          *reinterpret_cast<floatx4*>(part) = x;
+          *reinterpret_cast<floatx4*>(part + 4) = y;
         } else {
-          typedef T tx4 __attribute__((ext_vector_type(4)));
-          *reinterpret_cast<tx4*>(a.out + (to * D + d) * 2) = __builtin_convertvector(o, tx4);
+          Eight<T>::store(a.out + (to * D + 32 * i + d) * 2,
+                          __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
         }
       }
-    if (lh == 0) {
-      if (a.splits > 1) a.stat[to * a.splits + split] = floatx4{run[r].m, l, 0, 0};
+    }
+    if (lh == 0 && col < left) {
+      const int64_t to = out_row(a, t, h, wrow + 32 * r + col);
+      if (partial) store2(a.stat + to * a.splits + split, run[r].m, l);
       else if (a.lse)
-        a.lse[to] = l == 0.0f ? -__builtin_inff() : (run[r].m - kShift + __builtin_amdgcn_logf(l)) * kLn2;
+        a.lse[to] = l == 0.0f ? -__builtin_inff() : (run[r].m - kShift + log2_fast(l)) * kLn2;
     }
   }
 }
 
 // ---------------------------------------------------------------------------
-// The splits of one row, in their order: eight dimensions a thread.
+// The splits of every row, in their order: eight dimensions a thread.
 // ---------------------------------------------------------------------------
 template <typename T, int D>
-__global__ __launch_bounds__(256) void kv8_merge_kernel(AttnArgs a) {
-  const int64_t it = (int64_t)blockIdx.x * 256 + threadIdx.x;
+__global__ __launch_bounds__(kThreads) void kv8_merge_kernel(AttnArgs a) {
+  const int64_t it = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   const int64_t row = it / (D / 8);
   const int d = it % (D / 8) * 8;
-  if (row >= a.tokens * a.hq) return;
-  const floatx4* stat = a.stat + row * a.splits;
+  if (row >= (int64_t)a.tokens * a.hq) return;
+  typedef float floatx2 __attribute__((ext_vector_type(2)));
+  const floatx2* stat = reinterpret_cast<const floatx2*>(a.stat) + row * a.splits;
+  const float* part = a.part + row * a.splits * D + d;
   float m = -__builtin_inff();
   for (int s = 0; s < a.splits; ++s) m = fmaxf(m, stat[s][0]);
   float l = 0.0f;
   floatx8 o = 0.0f;
+#pragma unroll 4
   for (int s = 0; s < a.splits; ++s) {
-    const float f = exp2_fast(stat[s][0] - safe(m));
-    l += stat[s][1] * f;
-    const floatx8 x = *reinterpret_cast<const floatx8*>(a.part + (row * a.splits + s) * D + d);
+    const float ls = stat[s][1], f = exp2_fast(stat[s][0] - safe(m));
+    floatx8 x = *reinterpret_cast<const floatx8*>(part + (int64_t)s * D);
+    if (ls == 0.0f) x = 0.0f;  // (not written)
+    l += ls * f;
     o += x * f;
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  if (l == 0.0f) o = 0.0f;
-  Eight<T>::store(a.out + (row * D + d) * 2, o * inv);
-  if (d == 0 && a.lse)
-    a.lse[row] = l == 0.0f ? -__builtin_inff() : (m - kShift + __builtin_amdgcn_logf(l)) * kLn2;
+  finish<T>(a, row, D, d, o, m, l);
 }
 
 template <typename T, int D>
 hipError_t launch_sized(const AttnArgs& a, const Kv8AttnPlan& p, hipStream_t stream) {
   const unsigned grid = (unsigned)(p.tiles * a.hk * a.splits);
-  if (p.kernel == 0) {
-    if (p.rows == 16) kv8_decode_kernel<T, D, 1><<<grid, kWaves * kWave, 0, stream>>>(a);
-    else if constexpr (D <= 128) kv8_decode_kernel<T, D, 2><<<grid, kWaves * kWave, 0, stream>>>(a);
-  } else {
-    const size_t lds = 2 * (D <= 128 ? 2 : 1) * 32 * D * 2 * 2 + (D > 128 ? kWaves * 32 * D * 2 : 0);
-    kv8_prefill_kernel<T, D, 1><<<grid, kWaves * kWave, lds, stream>>>(a);
-  }
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.splits == 1) return e;
-  kv8_merge_kernel<T, D><<<(unsigned)ceil_div(a.tokens * a.hq * (D / 8), 256), 256, 0, stream>>>(a);
+  constexpr size_t kLds = D == 64 ? kWaves * 32 * 68 * 4
+                                  : 2 * (D <= 128 ? 2 : 1) * 32 * D * 2 * 2 + (D > 128 ? 128 * D * 2 : 0);
+  if (p.kernel == 1) kv8_prefill_kernel<T, D, 1><<<grid, kThreads, kLds, stream>>>(a);
+  else if (p.rows == 16) kv8_decode_kernel<T, D, 1><<<grid, kThreads, 0, stream>>>(a);
+  else if constexpr (D <= 128) kv8_decode_kernel<T, D, 2><<<grid, kThreads, 0, stream>>>(a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || !a.merge) return e;
+  kv8_merge_kernel<T, D>
+      <<<(unsigned)ceil_div((int64_t)a.tokens * a.hq * (D / 8), kThreads), kThreads, 0, stream>>>(a);
   return hipGetLastError();
 }
 
@@ -752,7 +1001,7 @@ hipError_t launch_sized(const AttnArgs& a, const Kv8AttnPlan& p, hipStream_t str
 
 Kv8AttnPlan plan_kv8_attention(const rf_kv8_attention_args& a, int cus) {
   Kv8AttnPlan p;
-  const int64_t group = a.q.heads / a.cache.kv_heads;
+  const int64_t group = a.q.heads / a.cache.kv_heads, hk = a.cache.kv_heads;
   int64_t most_q = a.cu_q ? a.max_q_len : ceil_div(a.tokens, a.requests);
   if (most_q < 1 || most_q > a.tokens) most_q = a.tokens;
   const int64_t most_rows = most_q * group;
@@ -764,17 +1013,21 @@ Kv8AttnPlan plan_kv8_attention(const rf_kv8_attention_args& a, int cus) {
   int64_t most_kv = a.width * a.cache.block_size;
   if (a.max_kv_len > 0 && a.max_kv_len < most_kv) most_kv = a.max_kv_len;
   if (a.window > 0 && a.window + most_q < most_kv) most_kv = a.window + most_q;
-  // Useful tiles, of which each is cut along its tokens until the launch has
-  // about `want` workgroups, in pieces of at least `least` groups.
+  // Useful tiles, each cut along its tokens until the launch has about `want`
+  // workgroups (more where requests may differ in length, so that the longest
+  // does not run on alone), in pieces of at least `least` groups.
   const int64_t tiles = p.kernel ? ceil_div(a.tokens * group, p.rows) : a.requests * ceil_div(most_rows, p.rows);
-  const int64_t busy = tiles * a.cache.kv_heads;
-  const int64_t want = p.kernel ? 2 * cus : 4 * cus, least = p.kernel ? 16 : 4;
-  const int64_t groups = ceil_div(most_kv, RF_KV8_GROUP);
-  int64_t s = want / (busy > 0 ? busy : 1);
-  if (s > groups / least) s = groups / least;
-  p.splits = (int)(s < 1 ? 1 : s > 128 ? 128 : s);
-  const int64_t D = a.cache.head_dim;
-  p.workspace = p.splits == 1 ? 0 : (size_t)(a.tokens * a.q.heads * p.splits) * (D + 4) * 4;
+  const int64_t busy = tiles * hk, groups = ceil_div(most_kv, RF_KV8_GROUP);
+  const int64_t want = 2 * cus * (a.requests > 1 && !p.kernel ? 3 : 1);
+  const int64_t cap = p.rows == 16 ? 64 : p.rows == 32 ? 32 : 16;  // what join()'s LDS holds
+  int64_t s = busy > 0 ? want / busy : 1;
+  p.least = 4;
+  if (s > groups / p.least) s = groups / p.least;
+  s = s < 1 ? 1 : s > cap ? cap : s;
+  const int64_t rows = most_rows < p.rows ? most_rows : p.rows;
+  p.merge = s > 1 && (p.kernel == 1 || p.tiles * hk > kMaxSplitCounters || rows * s * a.cache.head_dim > (1 << 15));
+  p.splits = (int)s;
+  p.workspace = s == 1 ? 0 : (size_t)(a.tokens * a.q.heads * s) * (a.cache.head_dim + 2) * 4;
   return p;
 }
 
@@ -794,12 +1047,17 @@ hipError_t launch_kv8_attention(const rf_kv8_attention_args& in, const Kv8AttnPl
   a.out = (uint8_t*)in.out;
   a.lse = in.lse;
   const int D = in.cache.head_dim;
-  const int64_t rows = in.tokens * in.q.heads * p.splits;
-  a.stat = (floatx4*)in.workspace;
-  a.part = (float*)in.workspace + rows * 4;
-  a.tokens = in.tokens;
+  a.counters = nullptr;
+  a.stat = nullptr;
+  a.part = nullptr;
+  if (p.splits > 1) {
+    a.counters = (uint32_t*)in.scratch->counters;
+    a.part = (float*)in.scratch->partials;
+    a.stat = (uint64_t*)(a.part + in.tokens * in.q.heads * p.splits * D);
+  }
   a.table_stride = in.table_stride;
-  a.num_blocks = in.cache.num_blocks;
+  a.num_blocks = (int)in.cache.num_blocks;
+  a.tokens = (int)in.tokens;
   a.requests = (int)in.requests;
   a.width = (int)in.width;
   a.hq = in.q.heads;
@@ -808,9 +1066,11 @@ hipError_t launch_kv8_attention(const rf_kv8_attention_args& in, const Kv8AttnPl
   a.shift = __builtin_ctz((unsigned)in.cache.block_size);
   a.per_request = in.cu_q ? 0 : (int)(in.tokens / in.requests);
   a.splits = p.splits;
+  a.least = p.least;
+  a.merge = p.merge;
   a.tiles = (int)p.tiles;
   a.causal = in.causal;
-  a.window = in.window;
+  a.window = in.window > (1 << 30) ? 1 << 30 : (int)in.window;
   a.scale_log2e = in.scale * kLog2e;
   const bool f16 = in.dtype == RF_W8A16_DTYPE_F16;
   if (D == 64)

@@ -44,14 +44,15 @@ int check_attention(const rf_kv8_attention_args* a) {
   if (a->q.heads % a->cache.kv_heads) return RF_W8A16_EINVAL;
   if (a->tokens < 0 || a->tokens > kMaxSize || a->requests < 1 || a->requests > kMaxSize)
     return RF_W8A16_EINVAL;
+  if (a->tokens * a->q.heads > 0x7fffffff) return RF_W8A16_EINVAL;
   if (!a->cu_q && a->tokens % a->requests) return RF_W8A16_EINVAL;
-  if (a->width < 1 || a->table_stride < a->width || a->width > 0x7fffffff / a->cache.block_size)
+  if (a->width < 1 || a->table_stride < a->width || a->width > kMaxSize / a->cache.block_size)
     return RF_W8A16_EINVAL;
   if (!(a->scale > 0.0f) || !(a->scale < __builtin_inff())) return RF_W8A16_EINVAL;
   if (a->window < 0 || (a->window > 0 && !a->causal)) return RF_W8A16_EINVAL;
   if (a->max_q_len < 0 || a->max_kv_len < 0) return RF_W8A16_EINVAL;
-  if (!aligned(a->out, 16) || !aligned(a->lse, 4) || !aligned(a->workspace, 16) ||
-      !aligned(a->cu_q, 4) || !aligned(a->kv_lens, 4) || !aligned(a->block_table, 4))
+  if (!aligned(a->out, 16) || !aligned(a->lse, 4) || !aligned(a->cu_q, 4) ||
+      !aligned(a->kv_lens, 4) || !aligned(a->block_table, 4))
     return RF_W8A16_EALIGN;
   return RF_W8A16_OK;
 }
@@ -163,10 +164,12 @@ int rf_kv8_attention(const rf_kv8_attention_args* a, void* stream) {
   st = check_device(&dev);
   if (st != RF_W8A16_OK) return st;
   const Kv8AttnPlan p = plan_kv8_attention(*a, dev.cus);
-  if (p.workspace > 0 && (!a->workspace || a->workspace_bytes < p.workspace)) return RF_W8A16_EWORKSPACE;
-  if (p.tiles * a->cache.kv_heads * p.splits > 0x7fffffff ||
-      a->tokens * a->q.heads > (int64_t)0x7fffffff * 256 / (a->cache.head_dim / 8))
-    return RF_W8A16_EINVAL;
+  if (p.workspace > 0) {
+    const rf_w8a16_scratch* w = a->scratch;
+    if (!w || !w->counters || !w->partials || w->partial_bytes < p.workspace) return RF_W8A16_EWORKSPACE;
+    if (!aligned(w->counters, 4) || !aligned(w->partials, 16)) return RF_W8A16_EALIGN;
+  }
+  if (p.tiles * a->cache.kv_heads * p.splits > 0x7fffffff) return RF_W8A16_EINVAL;
   return status_of(launch_kv8_attention(*a, p, static_cast<hipStream_t>(stream)));
 }
 

@@ -54,7 +54,9 @@ struct Kv8AttnPlan {
   int rows;       // rows of a tile
   int64_t tiles;  // upper bound of tiles per key/value head
   int splits;
-  size_t workspace;
+  int least;      // 32-token groups of a split, at least
+  bool merge;     // a second kernel adds the splits
+  size_t workspace;  // bytes of partial results
 };
 Kv8AttnPlan plan_kv8_attention(const rf_kv8_attention_args& a, int cus);
 hipError_t launch_kv8_attention(const rf_kv8_attention_args& a, const Kv8AttnPlan& p,

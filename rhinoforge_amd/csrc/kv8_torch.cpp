@@ -23,6 +23,7 @@
 #include <vector>
 
 #include "../../include/kv8.h"
+#include "torch_scratch.h"
 
 namespace {
 
@@ -416,7 +417,7 @@ Two attention_hip(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& v
   at::Tensor lse = return_lse ? at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat))
                               : at::empty({0}, q.options().dtype(at::kFloat));
   if (q.size(0) == 0) return {out, lse};
-  at::Tensor keep, workspace;
+  at::Tensor keep;
   a.q = heads_of(q, &keep);
   if (given(cu)) a.cu_q = cu->data_ptr<int32_t>();
   a.kv_lens = lens.data_ptr<int32_t>();
@@ -433,13 +434,15 @@ Two attention_hip(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& v
   a.causal = causal;
   a.window = window;
   a.scale = (float)scale;
-  const size_t bytes = rf_kv8_attention_workspace(&a);
-  if (bytes > 0) {  // from the stream's own pool, returned to it in order
-    workspace = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
-    a.workspace = workspace.data_ptr();
-    a.workspace_bytes = bytes;
-  }
-  check_status(rf_kv8_attention(&a, stream_of(q)), op);
+  void* stream = stream_of(q);
+  const int st = rf_torch::with_scratch(
+      q.device(), stream, op,
+      [&](const rf_w8a16_scratch* scratch) {
+        a.scratch = scratch;
+        return rf_kv8_attention(&a, stream);
+      },
+      [&] { return rf_kv8_attention_workspace(&a) + RF_W8A16_WS_COUNTER_BYTES; });
+  check_status(st, op);
   return {out, lse};
 }
 

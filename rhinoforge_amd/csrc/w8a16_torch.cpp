@@ -37,20 +37,20 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 
-#include <map>
-#include <mutex>
 #include <utility>
 #include <vector>
 
 #include "../../include/w8a16.h"
+#include "torch_scratch.h"
 
 namespace {
+
+using rf_torch::with_scratch;
 
 void check_status(int st, const char* what) {
   TORCH_CHECK(st == RF_W8A16_OK, what, ": ", rf_w8a16_status_str(st), " (status ", st, ")");
 }
 
-int64_t ceil_to(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // Symbolic sizes (FakeTensor tracing with dynamic shapes) round the same way.
 c10::SymInt ceil_div(const c10::SymInt& a, int64_t b) { return (a + (b - 1)) / b; }
@@ -71,83 +71,6 @@ void check_packed(const at::Tensor& packed, at::ScalarType dtype,
               packed.scalar_type());
   TORCH_CHECK(packed.sizes() == at::IntArrayRef(want), op, ": packed must have shape ", want,
               ", got ", packed.sizes());
-}
-
-// Scratch per (device, stream), in two parts (the C ABI's rf_w8a16_scratch).
-// Calls on one stream are ordered and leave the counters zero, so one set per
-// stream is safe to reuse.
-//   counters  allocated and cleared once, on the stream itself; for a stream
-//             first seen under graph capture the library's own, which nothing
-//             has to clear.  Never replaced: a fill recorded into a graph would
-//             clear them on that graph's replays only, and every other call on
-//             the stream might find anything.
-//   partials  at least kMinPartials bytes, never cleared.  A buffer that has to
-//             grow, under capture too, is retired, never freed: a HIP graph
-//             captured earlier on that stream may still reference it.
-constexpr int64_t kMinPartials = 16 << 20;
-
-bool capturing(void* stream) {
-  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-  return hipStreamIsCapturing(static_cast<hipStream_t>(stream), &st) == hipSuccess &&
-         st != hipStreamCaptureStatusNone;
-}
-
-struct ScratchCache {
-  std::mutex mu;
-  std::map<std::pair<int, void*>, rf_w8a16_scratch> sets;
-  std::vector<at::Tensor> kept;  // every buffer handed out, until the process ends
-
-  void* keep(at::Tensor t) {
-    kept.push_back(t);
-    return t.data_ptr();
-  }
-
-  // The stream's scratch with at least `bytes` of partials (current device: dev).
-  rf_w8a16_scratch get(const at::Device& dev, void* stream, size_t bytes, const char* op) {
-    std::lock_guard<std::mutex> g(mu);
-    rf_w8a16_scratch& s = sets[std::make_pair((int)dev.index(), stream)];
-    const auto opts = at::TensorOptions().dtype(at::kByte).device(dev);
-    if (!s.counters) {
-      if (capturing(stream)) {
-        const int st = rf_w8a16_stream_counters(stream, &s.counters);
-        TORCH_CHECK(st == RF_W8A16_OK, op, ": no split-K counters for a stream first used under "
-                    "graph capture (status ", st, "); make one call on it before the capture "
-                    "begins");
-      } else {
-        s.counters = keep(at::zeros({RF_W8A16_WS_COUNTER_BYTES}, opts));
-      }
-    }
-    if (!s.partials || s.partial_bytes < bytes) {
-      const int64_t sz = ceil_to(std::max<int64_t>((int64_t)bytes, kMinPartials), 1 << 20);
-      s.partials = keep(at::empty({sz}, opts));
-      s.partial_bytes = (size_t)sz;
-    }
-    return s;
-  }
-};
-
-ScratchCache& scratch_cache() {
-  static ScratchCache* c = new ScratchCache();  // lives until process exit
-  return *c;
-}
-
-// Runs call(scratch) with the stream's cached scratch.  The C ABI refuses one
-// that is too small with RF_W8A16_EWORKSPACE before it launches anything; only
-// then is the size the shape needs queried (a second launch plan: need()
-// returns the one-buffer size, counters included), the partials grown and the
-// call repeated.
-template <typename Call, typename Need>
-int with_scratch(const at::Device& dev, void* stream, const char* op, Call call, Need need) {
-  ScratchCache& cache = scratch_cache();
-  rf_w8a16_scratch s = cache.get(dev, stream, 0, op);
-  int st = call(&s);
-  if (st == RF_W8A16_EWORKSPACE) {
-    const size_t bytes = need();
-    TORCH_CHECK(bytes > RF_W8A16_WS_COUNTER_BYTES, op, ": ", rf_w8a16_status_str(RF_W8A16_EINVAL));
-    s = cache.get(dev, stream, bytes - RF_W8A16_WS_COUNTER_BYTES, op);
-    st = call(&s);
-  }
-  return st;
 }
 
 struct Checked {

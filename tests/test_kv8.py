@@ -299,7 +299,7 @@ def _c_heads(heads=2, **kw):
 
 
 def _c_attention(cache=None, q=None, **kw):
-    a = dict(cu_q=P, kv_lens=P, block_table=P, out=P, lse=None, workspace=None, workspace_bytes=0,
+    a = dict(cu_q=P, kv_lens=P, block_table=P, out=P, lse=None, scratch=None,
              tokens=4, requests=2, width=3, table_stride=3, max_q_len=0, max_kv_len=0, dtype=0, causal=1,
              window=0, scale=0.1)
     return capi.KV8AttentionArgs(cache=cache or _c_cache(), q=q or _c_heads(4), **{**a, **kw})
@@ -313,7 +313,8 @@ def _c_attention(cache=None, q=None, **kw):
     (capi.EINVAL, dict(q=dict(data=None))), (capi.EALIGN, dict(q=dict(data=P + 2))),
     (capi.EALIGN, dict(q=dict(token_stride=12))), (capi.EINVAL, dict(dtype=2)),
     (capi.EINVAL, dict(kv_lens=None)), (capi.EINVAL, dict(out=None)), (capi.EALIGN, dict(out=P + 8)),
-    (capi.EALIGN, dict(lse=P + 2)), (capi.EALIGN, dict(workspace=P + 4)), (capi.EINVAL, dict(tokens=-1)),
+    (capi.EALIGN, dict(lse=P + 2)), (capi.EINVAL, dict(tokens=-1)), (capi.EINVAL, dict(tokens=2 ** 29 + 2)),
+    (capi.EINVAL, dict(width=2 ** 25, table_stride=2 ** 25)),
     (capi.EINVAL, dict(tokens=5, cu_q=None)), (capi.EINVAL, dict(requests=0)), (capi.EINVAL, dict(width=0)),
     (capi.EINVAL, dict(table_stride=2)), (capi.EINVAL, dict(scale=0.0)), (capi.EINVAL, dict(scale=float("nan"))),
     (capi.EINVAL, dict(scale=float("inf"))), (capi.EINVAL, dict(window=-1)),
