@@ -260,16 +260,32 @@ __device__ __forceinline__ void keep_branch() { asm volatile(""); }
 // of 50 queries, 8 heads of 256, 8 splits: 87 us with join(), 36 with it).
 // ---------------------------------------------------------------------------
 constexpr int kThreads = 256;
+constexpr int kDeviceScope = 16;  // sc1 of a buffer access
 
-__device__ __forceinline__ void store2(void* p, float a, float b) {
-  const uint64_t v = (uint64_t)__builtin_bit_cast(uint32_t, b) << 32 | __builtin_bit_cast(uint32_t, a);
-  __hip_atomic_store((uint64_t*)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ void load2(const void* p, float* a, float* b) {
-  const uint64_t v = __hip_atomic_load((uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  *a = __builtin_bit_cast(float, (uint32_t)v);
-  *b = __builtin_bit_cast(float, (uint32_t)(v >> 32));
-}
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+
+// Partial results, addressed by byte offsets below 2^31 (checked on the host).
+struct Partials {
+  __amdgpu_buffer_rsrc_t part, stat;
+  __device__ __forceinline__ Partials(const AttnArgs& a)
+      : part(__builtin_amdgcn_make_buffer_rsrc(a.part, 0, 0x7fffffff, 0x00027000)),
+        stat(__builtin_amdgcn_make_buffer_rsrc(a.stat, 0, 0x7fffffff, 0x00027000)) {}
+  __device__ __forceinline__ void store(int i, floatx4 v) const {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), part, i * 4, 0, kDeviceScope);
+  }
+  __device__ __forceinline__ floatx4 load(int i) const {
+    return __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(part, i * 4, 0, kDeviceScope));
+  }
+  __device__ __forceinline__ void store_stat(int i, float m, float l) const {
+    const floatx2 v = {m, l};
+    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, v), stat, i * 8, 0, kDeviceScope);
+  }
+  __device__ __forceinline__ floatx2 load_stat(int i) const {  // m, l
+    return __builtin_bit_cast(floatx2, __builtin_amdgcn_raw_buffer_load_b64(stat, i * 8, 0, kDeviceScope));
+  }
+};
 
 // Output row of tile row rc: token * heads + head.
 __device__ __forceinline__ int64_t out_row(const AttnArgs& a, const Tile& t, int h, int rc) {
@@ -278,26 +294,28 @@ __device__ __forceinline__ int64_t out_row(const AttnArgs& a, const Tile& t, int
 }
 
 template <typename T>
-__device__ __forceinline__ void finish(const AttnArgs& a, int64_t to, int D, int d, floatx8 o, float m,
+__device__ __forceinline__ void finish(const AttnArgs& a, int64_t to, int D, int d, floatx4 o, float m,
                                        float l) {
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   if (l == 0.0f) o = 0.0f;
-  Eight<T>::store(a.out + (to * D + d) * 2, o * inv);
+  typedef T tx4 __attribute__((ext_vector_type(4)));
+  *reinterpret_cast<tx4*>(a.out + (to * D + d) * 2) = __builtin_convertvector(o * inv, tx4);
   if (d == 0 && a.lse)
     a.lse[to] = l == 0.0f ? -__builtin_inff() : (m - kShift + log2_fast(l)) * kLn2;
 }
 
 // A split with nothing to do, for kv8_merge_kernel.
 __device__ __forceinline__ void no_share(const AttnArgs& a, const Tile& t, int h, int rows, int split) {
+  const Partials parts(a);
   for (int rc = threadIdx.x; rc < rows; rc += kThreads)
-    store2(a.stat + out_row(a, t, h, rc) * a.splits + split, -__builtin_inff(), 0.0f);
+    parts.store_stat((int)out_row(a, t, h, rc) * a.splits + split, -__builtin_inff(), 0.0f);
 }
 
 // All threads call it after their stores of partial results.  buf: LDS of
-// rows * splits * 8 + 8192 bytes, free for use.
+// rows * splits * 8 + 4096 bytes, free for use.
 template <typename T, int D>
-__device__ void join(const AttnArgs& a, const Tile& t, int h, int rows, int splits, uint32_t* counter,
-                     float* buf) {
+__device__ __forceinline__ void join(const AttnArgs& a, const Tile& t, int h, int rows, int splits,
+                                     uint32_t* counter, float* buf) {
   const int tid = threadIdx.x;
   __shared__ int is_last;
   __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wavefront's stores are done
@@ -310,57 +328,57 @@ __device__ void join(const AttnArgs& a, const Tile& t, int h, int rows, int spli
   }
   __syncthreads();
   if (!is_last) return;
-  float* stat = buf;                        // [rows][splits][m, l]
-  floatx8* sums = reinterpret_cast<floatx8*>(buf + rows * splits * 2);
-  for (int i = tid; i < rows * splits; i += kThreads) {
-    const int rc = i / splits;
-    float m, l;
-    load2(a.stat + out_row(a, t, h, rc) * a.splits + (i - rc * splits), &m, &l);
-    stat[2 * i] = m;
-    stat[2 * i + 1] = l;
-  }
-  __syncthreads();
-  // One thread per row and eight dimensions; where that leaves threads over,
-  // `ways` of them share the splits and meet in LDS.
-  const int units = rows * (D / 8);
+  const Partials parts(a);
+  // One thread per row and four dimensions; where that leaves threads over,
+  // `ways` of them share the splits and meet in LDS.  What counts is that many
+  // loads are in flight: a round trip takes longer than the bytes.
+  constexpr int kFlight = 8;
+  const int units = rows * (D / 4);
   int ways = 1;
   while (units * ways * 2 <= kThreads && ways * 2 <= splits) ways *= 2;
+  float* stat = buf;  // [rows][splits][m, l]
+  floatx4* sums = reinterpret_cast<floatx4*>(buf + (rows * splits * 2 + 3) / 4 * 4);
+  for (int i = tid; i < rows * splits; i += kThreads) {
+    const int rc = (int)((unsigned)i / (unsigned)splits);
+    *reinterpret_cast<floatx2*>(stat + 2 * i) =
+        parts.load_stat((int)out_row(a, t, h, rc) * a.splits + (i - rc * splits));
+  }
   for (int u0 = 0; u0 < units; u0 += kThreads) {
-    const int way = ways == 1 ? 0 : tid / units, u = u0 + (ways == 1 ? tid : tid - way * units);
+    const int way = ways == 1 ? 0 : (int)((unsigned)tid / (unsigned)units);
+    const int u = u0 + (ways == 1 ? tid : tid - way * units);
     const bool on = u < units && way < ways;
-    const int rc = on ? u / (D / 8) : 0, d = u % (D / 8) * 8;
-    float m = -__builtin_inff(), l = 0.0f;
-    floatx8 o = 0.0f;
-    const int64_t to = out_row(a, t, h, rc);
-    if (on) {
-      const float* st = stat + rc * splits * 2;
-      for (int s = 0; s < splits; ++s) m = fmaxf(m, st[2 * s]);
-      const float* part = a.part + to * a.splits * D + d;
-#pragma unroll 4
-      for (int s = way; s < splits; s += ways) {
-        floatx8 x;
+    const int rc = on ? u / (D / 4) : 0, d = u % (D / 4) * 4;
+    const int to = (int)out_row(a, t, h, rc);
+    const int at = to * a.splits * D + d;
+    floatx4 x[kFlight];
 #pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-          float lo, hi;
-          load2(part + (int64_t)s * D + j, &lo, &hi);
-          x[j] = lo;
-          x[j + 1] = hi;
-        }
-        const float f = exp2_fast(st[2 * s] - safe(m));
-        l += st[2 * s + 1] * f;
-        o += x * f;
+    for (int k = 0; k < kFlight; ++k) x[k] = parts.load(at + min(way + k * ways, splits - 1) * D);
+    if (u0 == 0) __syncthreads();  // stat
+    const float* st = stat + rc * splits * 2;
+    float m = -__builtin_inff(), l = 0.0f;
+    for (int s = 0; s < splits; ++s) m = fmaxf(m, st[2 * s]);
+    for (int s = 0; s < splits; ++s) l += st[2 * s + 1] * exp2_fast(st[2 * s] - safe(m));
+    floatx4 o = 0.0f;
+    for (int s0 = way; s0 < splits; s0 += kFlight * ways) {
+      floatx4 y[kFlight];
+#pragma unroll
+      for (int k = 0; k < kFlight; ++k) y[k] = x[k];
+      if (s0 + kFlight * ways < splits) {
+#pragma unroll
+        for (int k = 0; k < kFlight; ++k)
+          x[k] = parts.load(at + min(s0 + (kFlight + k) * ways, splits - 1) * D);
+      }
+#pragma unroll
+      for (int k = 0; k < kFlight; ++k) {
+        const int s = s0 + k * ways;
+        if (s < splits) o += y[k] * exp2_fast(st[2 * s] - safe(m));
       }
     }
-    if (ways > 1) {
-      // (units <= 128 here: one turn of the outer loop)
+    if (ways > 1) {  // (units < kThreads: one turn of the outer loop)
       sums[tid] = o;
       __syncthreads();
-      if (on && way == 0) {
+      if (on && way == 0)
         for (int w = 1; w < ways; ++w) o += sums[tid + w * units];
-        l = 0.0f;
-        const float* st = stat + rc * splits * 2;
-        for (int s = 0; s < splits; ++s) l += st[2 * s + 1] * exp2_fast(st[2 * s] - safe(m));
-      }
     }
     if (on && way == 0) finish<T>(a, to, D, d, o, m, l);
   }
@@ -389,12 +407,15 @@ __device__ __forceinline__ void fetch(const AttnArgs& a, const Group& g, int lan
   for (int i = 0; i < D / 32; ++i) b.k[i] = load_u4_stream(kp + i * kTileBytes + lane * 16);
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) b.v[i] = load_u4_stream(vp + i * kTileBytes + lane * 16);
+  // (the scales' wait would otherwise come before the bytes go out)
+  __builtin_amdgcn_sched_barrier(0);
   b.ks = scale_bits(a.ks, g);
   b.vs = scale_bits(a.vs, g);
 }
 
 template <typename T, int D, int RT>
-__global__ __launch_bounds__(kWaves* kWave) void kv8_decode_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kWaves* kWave)
+__attribute__((amdgpu_waves_per_eu(2))) void kv8_decode_kernel(AttnArgs a) {
   constexpr int R = 16 * RT;
   __shared__ __align__(16) float red[kWaves][16][D + 4];
   __shared__ float red_m[kWaves][R], red_l[kWaves][R];
@@ -537,7 +558,12 @@ __global__ __launch_bounds__(kWaves* kWave) void kv8_decode_kernel(AttnArgs a) {
         for (int i = 0; i < D / 16; ++i) acc[r][i] *= fa;
       }
     }
-    const float lr = ratio_log2(vs, top), back = exp2_fast(-lr);
+    float lr = 0.0f;  // (see the prefill kernel)
+    if (vs != top.bits) {
+      lr = ratio_log2(vs, top);
+      asm volatile("" : "+v"(lr));
+    }
+    const float back = exp2_fast(-lr);
     half8 p[RT];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
@@ -611,27 +637,25 @@ __global__ __launch_bounds__(kWaves* kWave) void kv8_decode_kernel(AttnArgs a) {
     for (int i = 0; i < D / 16; ++i)
       *reinterpret_cast<floatx4*>(&red[wave][col][16 * i + 4 * lg]) = acc[r][i] * f;
     __syncthreads();
-    for (int it = tid; it < 16 * (D / 8); it += kWaves * kWave) {
-      const int c = it / (D / 8), d = it % (D / 8) * 8, rc = 16 * r + c;
+    for (int it = tid; it < 16 * (D / 4); it += kThreads) {
+      const int c = it / (D / 4), d = it % (D / 4) * 4, rc = 16 * r + c;
       if (rc >= rows) continue;
       float mm = red_m[0][rc];
 #pragma unroll
       for (int w = 1; w < kWaves; ++w) mm = fmaxf(mm, red_m[w][rc]);
       float l = 0.0f;
-      floatx8 o = 0.0f;
+      floatx4 o = 0.0f;
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) {
         l += red_l[w][rc] * exp2_fast(red_m[w][rc] - safe(mm));
-        const floatx4 x = *reinterpret_cast<const floatx4*>(&red[w][c][d]);
-        const floatx4 y = *reinterpret_cast<const floatx4*>(&red[w][c][d + 4]);
-        o += __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+        o += *reinterpret_cast<const floatx4*>(&red[w][c][d]);
       }
       const int64_t to = out_row(a, t, h, rc);
       if (partial) {
-        float* part = a.part + (to * a.splits + split) * D + d;
-#pragma unroll
-        for (int j = 0; j < 8; j += 2) store2(part + j, o[j], o[j + 1]);
-        if (d == 0) store2(a.stat + to * a.splits + split, mm, l);
+        const Partials parts(a);
+        const int i = (int)to * a.splits + split;
+        parts.store(i * D + d, o);
+        if (d == 0) parts.store_stat(i, mm, l);
       } else {
         finish<T>(a, to, D, d, o, mm, l);
       }
@@ -948,7 +972,7 @@ __attribute__((amdgpu_waves_per_eu(RT == 1 ? 2 : 1))) void kv8_prefill_kernel(At
     }
     if (lh == 0 && col < left) {
       const int64_t to = out_row(a, t, h, wrow + 32 * r + col);
-      if (partial) store2(a.stat + to * a.splits + split, run[r].m, l);
+      if (partial) Partials(a).store_stat((int)to * a.splits + split, run[r].m, l);
       else if (a.lse)
         a.lse[to] = l == 0.0f ? -__builtin_inff() : (run[r].m - kShift + log2_fast(l)) * kLn2;
     }
@@ -956,25 +980,24 @@ __attribute__((amdgpu_waves_per_eu(RT == 1 ? 2 : 1))) void kv8_prefill_kernel(At
 }
 
 // ---------------------------------------------------------------------------
-// The splits of every row, in their order: eight dimensions a thread.
+// The splits of every row, in their order: four dimensions a thread.
 // ---------------------------------------------------------------------------
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads) void kv8_merge_kernel(AttnArgs a) {
   const int64_t it = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int64_t row = it / (D / 8);
-  const int d = it % (D / 8) * 8;
+  const int64_t row = it / (D / 4);
+  const int d = it % (D / 4) * 4;
   if (row >= (int64_t)a.tokens * a.hq) return;
-  typedef float floatx2 __attribute__((ext_vector_type(2)));
   const floatx2* stat = reinterpret_cast<const floatx2*>(a.stat) + row * a.splits;
   const float* part = a.part + row * a.splits * D + d;
   float m = -__builtin_inff();
   for (int s = 0; s < a.splits; ++s) m = fmaxf(m, stat[s][0]);
   float l = 0.0f;
-  floatx8 o = 0.0f;
-#pragma unroll 4
+  floatx4 o = 0.0f;
+#pragma unroll 8
   for (int s = 0; s < a.splits; ++s) {
     const float ls = stat[s][1], f = exp2_fast(stat[s][0] - safe(m));
-    floatx8 x = *reinterpret_cast<const floatx8*>(part + (int64_t)s * D);
+    floatx4 x = *reinterpret_cast<const floatx4*>(part + (int64_t)s * D);
     if (ls == 0.0f) x = 0.0f;  // (not written)
     l += ls * f;
     o += x * f;
@@ -993,7 +1016,7 @@ hipError_t launch_sized(const AttnArgs& a, const Kv8AttnPlan& p, hipStream_t str
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || !a.merge) return e;
   kv8_merge_kernel<T, D>
-      <<<(unsigned)ceil_div((int64_t)a.tokens * a.hq * (D / 8), kThreads), kThreads, 0, stream>>>(a);
+      <<<(unsigned)ceil_div((int64_t)a.tokens * a.hq * (D / 4), kThreads), kThreads, 0, stream>>>(a);
   return hipGetLastError();
 }
 
@@ -1028,6 +1051,11 @@ Kv8AttnPlan plan_kv8_attention(const rf_kv8_attention_args& a, int cus) {
   p.merge = s > 1 && (p.kernel == 1 || p.tiles * hk > kMaxSplitCounters || rows * s * a.cache.head_dim > (1 << 15));
   p.splits = (int)s;
   p.workspace = s == 1 ? 0 : (size_t)(a.tokens * a.q.heads * s) * (a.cache.head_dim + 2) * 4;
+  if (p.workspace > 0x7fffffff) {  // (partials are addressed by 31 bits)
+    p.splits = 1;
+    p.merge = false;
+    p.workspace = 0;
+  }
   return p;
 }
 
