@@ -408,7 +408,7 @@ __device__ __forceinline__ void fetch(const AttnArgs& a, const Group& g, int lan
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) b.v[i] = load_u4_stream(vp + i * kTileBytes + lane * 16);
   // (the scales' wait would otherwise come before the bytes go out)
-  __builtin_amdgcn_sched_barrier(0);
+  if constexpr (D <= 128) __builtin_amdgcn_sched_barrier(0);
   b.ks = scale_bits(a.ks, g);
   b.vs = scale_bits(a.vs, g);
 }

@@ -8,9 +8,14 @@ namespace rf {
 namespace {
 
 // ---------------------------------------------------------------------------
-// Norms and rotation.  LP lanes hold one head, eight dimensions each (16-byte
-// loads and stores); a wavefront takes 64 / LP heads of one token at a time,
-// with that token's cos and sin and both weights in registers for all of them.
+// Norms and rotation.  LP lanes hold one head; a lane's eight dimensions are
+// two runs of four, a0.. and b0.., which with halves as pairs are each other's
+// partners, so the rotation needs no other lane and one set of four cosines.
+// A wavefront walks query heads or key heads of one token, kHeads at a time,
+// with that token's cos and sin and the weight in registers and the next heads'
+// loads in flight; heads advance a scalar base, so they cost no address math
+// (4001 tokens of 64 + 8 heads: 46 us with per-lane addresses and IEEE square
+// root and division, ROPE so).
 // ---------------------------------------------------------------------------
 struct RopeArgs {
   const uint8_t *q, *k;
@@ -19,95 +24,128 @@ struct RopeArgs {
   const uint8_t *qw, *kw;
   const float *cos, *sin;
   const void* pos;
-  int64_t tokens, table_rows;
-  int pos64, hq, hk, D, rot, interleaved;
-  int per_wave;  // heads of a wavefront
+  int64_t table_rows;
+  int tokens, pos64, hq, hk, D, rot;
+  int turns;           // of kHeads heads each, per wavefront
+  int q_parts, parts;  // wavefronts of one token: for q, for both
   float eps;
 };
 
-template <typename T, int LP>
-__global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeArgs a) {
-  constexpr int kHeads = kWave / LP;
-  const int lane = threadIdx.x % kWave, sub = lane % LP;
-  const int64_t t = blockIdx.x;
-  const int heads = a.hq + a.hk;
-  const int first = (blockIdx.y * (blockDim.x / kWave) + threadIdx.x / kWave) * a.per_wave;
-  if (first >= heads) return;
-  const int end = min(first + a.per_wave, heads);
-  const int d0 = sub * 8;
-  const bool mine = d0 < a.D;
+// Sum over the LP lanes of a head, in all of them.
+template <int LP>
+__device__ __forceinline__ float sum_lanes(float v) {
+  const auto add = [&](auto ctrl) {
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl(),
+                                                               0xf, 0xf, true));
+  };
+  add([] { return 0xB1; } );   // lanes 1, 0, 3, 2 of a quad
+  add([] { return 0x4E; });    // 2, 3, 0, 1
+  add([] { return 0x141; });   // mirrored in eight
+  if (LP >= 16) add([] { return 0x140; });  // mirrored in sixteen
+  if (LP >= 32) v += __shfl_xor(v, 16);
+  if (LP >= 64) v += __shfl_xor(v, 32);
+  return v;
+}
 
-  // cos and sin of this lane's eight dimensions; signs so that y' = y c + partner s.
-  floatx8 c = 1.0f, s = 0.0f;
-  int src = lane;
-  const int half = a.rot / 2;
+template <typename T, int LP, bool kInterleaved>
+__global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeArgs a) {
+  constexpr int kHeads = kWave / LP, kAhead = 4;
+  typedef T tx4 __attribute__((ext_vector_type(4)));
+  const int lane = threadIdx.x % kWave, sub = lane % LP;
+  const unsigned w = blockIdx.x * (256 / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int t = (int)(w / (unsigned)a.parts), part = (int)(w - (unsigned)t * a.parts);
+  if (t >= a.tokens) return;
+  const bool isq = part < a.q_parts;
+  const int heads = isq ? a.hq : a.hk, first = (isq ? part : part - a.q_parts) * a.turns * kHeads;
+  const int left = heads - first;  // heads from here on
+  const bool mine = sub * 8 < a.D, turned = sub < a.rot / 8;
+  const int a0 = turned ? 4 * sub : a.rot + 4 * (sub - a.rot / 8);
+  const int b0 = a0 + (turned ? a.rot / 2 : (a.D - a.rot) / 2);
+  const int64_t hs = isq ? a.q_hs : a.k_hs;
+  const uint8_t* src = (isq ? a.q + t * a.q_ts : a.k + t * a.k_ts) + first * hs;
+  uint8_t* dst = (isq ? a.q_out : a.k_out) + ((int64_t)t * heads + first) * a.D * 2;
+  const int64_t in_a = lane / LP * hs + a0 * 2, in_b = lane / LP * hs + b0 * 2;
+  const int out_a = (lane / LP * a.D + a0) * 2, out_b = (lane / LP * a.D + b0) * 2;
+  const int turns = min(a.turns, (left + kHeads - 1) / kHeads);
+
+  // The first heads go out before the position's and the table's round trips.
+  tx4 xa[kAhead], xb[kAhead];
+  const auto load = [&](int u, int turn) {
+    if (mine && turn * kHeads + lane / LP < left) {
+      const uint8_t* p = src + turn * (kHeads * hs);
+      xa[u] = *reinterpret_cast<const tx4*>(p + in_a);
+      xb[u] = *reinterpret_cast<const tx4*>(p + in_b);
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) {
+    xa[u] = xb[u] = (T)0.0f;
+    if (u < turns) load(u, u);
+  }
+
+  floatx4 ca = 1.0f, sa = 0.0f, cb = 1.0f, sb = 0.0f;  // (halves as pairs: ca and sa only)
   if (a.rot > 0) {
     const int64_t row = a.pos == nullptr ? t
                         : a.pos64        ? reinterpret_cast<const int64_t*>(a.pos)[t]
                                          : reinterpret_cast<const int32_t*>(a.pos)[t];
     const bool ok = row >= 0 && row < a.table_rows;
-    const float* cr = a.cos + (ok ? row : 0) * half;
-    const float* sr = a.sin + (ok ? row : 0) * half;
-    const float bad = ok ? 0.0f : __builtin_nanf("");
-    c = 1.0f + bad;
-    if (d0 >= a.rot) {
-    } else if (a.interleaved) {
-      const floatx4 cv = *reinterpret_cast<const floatx4*>(cr + d0 / 2);
-      const floatx4 sv = *reinterpret_cast<const floatx4*>(sr + d0 / 2);
+    const float* cr = a.cos + (ok ? row : 0) * (a.rot / 2);
+    const float* sr = a.sin + (ok ? row : 0) * (a.rot / 2);
+    if (turned) {
+      if (kInterleaved) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        c[2 * i] = c[2 * i + 1] = cv[i] + bad;
-        s[2 * i] = -sv[i];
-        s[2 * i + 1] = sv[i];
-      }
-    } else {
-      const bool low = d0 < half;
-      const int at = low ? d0 : d0 - half;
-      src = low ? lane + half / 8 : lane - half / 8;
-#pragma unroll
-      for (int i = 0; i < 8; i += 4) {
-        const floatx4 cv = *reinterpret_cast<const floatx4*>(cr + at + i);
-        const floatx4 sv = *reinterpret_cast<const floatx4*>(sr + at + i);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          c[i + j] = cv[j] + bad;
-          s[i + j] = low ? -sv[j] : sv[j];
+        for (int i = 0; i < 4; ++i) {
+          ca[i] = cr[a0 / 2 + i / 2], cb[i] = cr[b0 / 2 + i / 2];
+          sa[i] = sr[a0 / 2 + i / 2], sb[i] = sr[b0 / 2 + i / 2];
         }
+      } else {
+        ca = *reinterpret_cast<const floatx4*>(cr + a0);
+        sa = *reinterpret_cast<const floatx4*>(sr + a0);
       }
     }
+    if (!ok) ca = cb = __builtin_nanf("");
   }
-  floatx8 qw = 1.0f, kw = 1.0f;
-  if (mine && a.qw) qw = Eight<T>::load(a.qw + d0 * 2);
-  if (mine && a.kw) kw = Eight<T>::load(a.kw + d0 * 2);
+  if (!kInterleaved) cb = ca;
+  const uint8_t* weight = isq ? a.qw : a.kw;
+  floatx4 wa = 1.0f, wb = 1.0f;
+  if (mine && weight) {
+    wa = __builtin_convertvector(*reinterpret_cast<const tx4*>(weight + a0 * 2), floatx4);
+    wb = __builtin_convertvector(*reinterpret_cast<const tx4*>(weight + b0 * 2), floatx4);
+  }
+  const float over = 1.0f / (float)a.D;
 
-  for (int h0 = first; h0 < end; h0 += kHeads) {
-    const int h = h0 + lane / LP;
-    const bool on = mine && h < end;
-    const bool isq = h < a.hq;
-    const uint8_t* in = isq ? a.q + t * a.q_ts + h * a.q_hs : a.k + t * a.k_ts + (h - a.hq) * a.k_hs;
-    floatx8 x = 0.0f;
-    if (on) x = Eight<T>::load(in + d0 * 2);
-    if (isq ? a.qw != nullptr : a.kw != nullptr) {
-      float ss = 0.0f;
+  for (int turn0 = 0; turn0 < turns; turn0 += kAhead) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
+    for (int u = 0; u < kAhead; ++u) {
+      const int turn = turn0 + u;
+      if (turn >= turns) break;
+      floatx4 x = __builtin_convertvector(xa[u], floatx4), y = __builtin_convertvector(xb[u], floatx4);
+      if (turn + kAhead < turns) load(u, turn + kAhead);
+      if (weight) {
+        const floatx4 sq = x * x + y * y;
+        const float ss = sum_lanes<LP>((sq[0] + sq[1]) + (sq[2] + sq[3]));
+        const float r = __builtin_amdgcn_rsqf(ss * over + a.eps);  // (within 2^-23)
+        x = x * r * wa;
+        y = y * r * wb;
+      }
+      floatx4 xo, yo;
+      if (kInterleaved) {
 #pragma unroll
-      for (int m = 1; m < LP; m <<= 1) ss += __shfl_xor(ss, m);
-      const float r = 1.0f / sqrtf(ss / (float)a.D + a.eps);
-      x = x * r * (isq ? qw : kw);
-    }
-    floatx8 y;
-    if (a.interleaved) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = x[i] * c[i] + x[i ^ 1] * s[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = x[i] * c[i] + __shfl(x[i], src) * s[i];
-    }
-    if (on) {
-      uint8_t* out = isq ? a.q_out + (t * a.hq + h) * (int64_t)a.D * 2
-                         : a.k_out + (t * a.hk + (h - a.hq)) * (int64_t)a.D * 2;
-      Eight<T>::store(out + d0 * 2, y);
+        for (int i = 0; i < 4; i += 2) {
+          xo[i] = x[i] * ca[i] - x[i + 1] * sa[i];
+          xo[i + 1] = x[i + 1] * ca[i] + x[i] * sa[i];
+          yo[i] = y[i] * cb[i] - y[i + 1] * sb[i];
+          yo[i + 1] = y[i + 1] * cb[i] + y[i] * sb[i];
+        }
+      } else {
+        xo = x * ca - y * sa;
+        yo = y * cb + x * sa;
+      }
+      if (mine && turn * kHeads + lane / LP < left) {
+        uint8_t* out = dst + (int64_t)turn * kHeads * a.D * 2;
+        *reinterpret_cast<tx4*>(out + out_a) = __builtin_convertvector(xo, tx4);
+        *reinterpret_cast<tx4*>(out + out_b) = __builtin_convertvector(yo, tx4);
+      }
     }
   }
 }
@@ -221,9 +259,8 @@ __global__ __launch_bounds__(kPlanThreads) void kv8_plan_kernel(rf_kv8_plan_args
 
 // ---------------------------------------------------------------------------
 // Append.  A run is a maximal sequence of consecutive slots inside one block
-// among consecutive tokens; one workgroup quantizes one head of it, k or v:
-// the largest magnitude, the new scale, the held values again if the scale
-// rose, the new ones.  v is gathered by tiles of dimensions, through LDS.
+// among consecutive tokens; for one head of it, k or v: the largest magnitude,
+// the new scale, the held values again if the scale rose, the new ones.
 // ---------------------------------------------------------------------------
 struct AppendArgs {
   const uint8_t* x[2];     // k, v
@@ -233,17 +270,28 @@ struct AppendArgs {
   const int32_t* slots;
   int64_t tokens, num_blocks;
   int heads, shift;        // log2(block size)
-  int chunk;               // consecutive tokens whose runs one workgroup begins
+  int chunk;               // long runs: consecutive tokens whose runs a workgroup begins
 };
 
 constexpr float kLeastAmax = 0x1p-100f;
 
-// rint(x / step) as a stored byte.  x / step by a correctly rounded reciprocal
-// and one correction, t + r (x - t step) (Markstein 1990).
-__device__ __forceinline__ uint32_t quant_byte(float x, float step, float r) {
+// b is i slots after a (slots reach up to 2^31)
+__device__ __forceinline__ bool follows(int32_t a, int i, int32_t b) {
+  return (uint32_t)b - (uint32_t)a == (uint32_t)i;
+}
+
+// x / step, correctly rounded, plus 1.5 * 2^23 + 128: the sum rounds the
+// quotient to the nearest integer (ties to even), and its low byte is the
+// stored byte.  The quotient comes from a correctly rounded reciprocal and one
+// correction, t + r (x - t step) (Markstein 1990); |x / step| < 127.0001.
+__device__ __forceinline__ uint32_t quant_bits(float x, float step, float r) {
   const float t = x * r;
-  const float q = rintf(__builtin_fmaf(__builtin_fmaf(-t, step, x), r, t));
-  return (uint32_t)((int)fminf(fmaxf(q, -127.0f), 127.0f) + 128);
+  return __builtin_bit_cast(uint32_t, __builtin_fmaf(__builtin_fmaf(-t, step, x), r, t) + 12583040.0f);
+}
+// The low bytes of four words, in order.
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  const uint32_t lo = __builtin_amdgcn_perm(b, a, 0x0c0c0400u), hi = __builtin_amdgcn_perm(d, c, 0x04000c0cu);
+  return lo | hi;
 }
 __device__ __forceinline__ uint32_t requant_byte(uint32_t u, float ratio) {
   return (uint32_t)((int)rintf((float)((int)u - 128) * ratio) + 128) & 0xffu;
@@ -253,131 +301,259 @@ __device__ __forceinline__ uint32_t byte_of(uint4 v, int i) {
   return (w >> (8 * (i & 3))) & 0xffu;
 }
 
-template <typename T, int D, int NT>
-__global__ __launch_bounds__(NT) void kv8_append_kernel(AppendArgs a) {
-  extern __shared__ uint8_t staged[];  // v: [tokens of the run][D] bytes
-  __shared__ uint32_t wave_amax[NT / kWave];
-  const int tid = threadIdx.x, lane = tid % kWave;
-  const int h = blockIdx.y, side = blockIdx.z;
+// What a block's scale becomes.
+struct Step {
+  float step, ratio;  // held values change by `ratio` where `rise`
+  float r;            // 1 / step, 0 where everything is stored as 0
+  bool rise, some;
+  __device__ __forceinline__ Step(float amax, bool held, float scale) {
+    const float before = held ? scale : 0.0f;
+    const float fresh = amax < kLeastAmax ? 0.0f : amax * (1.0f / 127.0f);
+    // the larger; either one not finite makes the block not finite
+    step = before >= fresh || before != before ? before : fresh;
+    rise = held && !(step == before) && before == before;
+    ratio = rise ? before / step : 1.0f;
+    some = step > 0.0f && step < __builtin_inff();
+    r = some ? 1.0f / step : 0.0f;
+  }
+  __device__ __forceinline__ uint2 bytes(floatx8 f) const {
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = quant_bits(f[j], step, r);
+    return some ? make_uint2(low_bytes(w[0], w[1], w[2], w[3]), low_bytes(w[4], w[5], w[6], w[7]))
+                : make_uint2(0x80808080u, 0x80808080u);
+  }
+};
+
+// Bits of the largest |x| of eight values (a NaN is above infinity).
+__device__ __forceinline__ uint32_t top_bits(uint4 v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) top = max(top, max(w[j] & 0x7fffu, (w[j] >> 16) & 0x7fffu));
+  return top;
+}
+
+// Byte offsets within a head's block.
+template <int D>
+__device__ __forceinline__ int k_at(int o, int d) {  // 16 bytes for d % 16 == 0
+  return (o >> 5) * (32 * D) + ((o >> 4 & 1) * (D / 64) + (d >> 6)) * kTileBytes +
+         ((d >> 4 & 3) * 16 + (o & 15)) * 16 + (d & 15);
+}
+template <int D>
+__device__ __forceinline__ int v_at(int o, int d) {
+  return (o >> 5) * (32 * D) + (d >> 5) * kTileBytes + ((o >> 2 & 3) * 16 + (d & 15)) * 16 +
+         (d >> 4 & 1) * 8 + (o >> 4 & 1) * 4 + (o & 3);
+}
+
+// Held bytes of tokens [0, o0) rounded to a larger step: `count` threads, this
+// one `tid`; v chunks hold tokens past o0 too, whose bytes stay.
+template <int D>
+__device__ __forceinline__ void requantize(uint8_t* dst, int side, int o0, float ratio, int tid,
+                                           int count) {
+  const int groups = (o0 + 31) >> 5;
+  for (int it = tid; it < groups * 2 * D; it += count) {
+    uint8_t* p = dst + it * 16;
+    // 16 bytes of one token (k), or of tokens tok + c and tok + 16 + c (v)
+    const int gr = it / (2 * D), l = it % kWave;
+    const int tok = gr * 32 + (side ? 4 * (l / 16) : (it % (2 * D) / kWave / (D / 64)) * 16 + l % 16);
+    if (tok >= o0) continue;
+    const uint4 v = load_u4(p);
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      w[j] = 0;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const uint32_t u = byte_of(v, 4 * j + b);
+        const bool held = !side || tok + 16 * (j & 1) + b < o0;
+        w[j] |= (held ? requant_byte(u, ratio) : u) << (8 * b);
+      }
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// Short runs (single tokens): one wavefront for each run, head and side.  The
+// time is its chain of round trips: slots and the first values together, then
+// the scale, then the stores (bytes for v, which need no read).
+template <typename T, int D>
+__global__ __launch_bounds__(kWave) void kv8_append_short_kernel(AppendArgs a) {
+  constexpr int kRow = D / 8;  // lanes of one token
+  const int lane = threadIdx.x, h = blockIdx.y, side = blockIdx.z;
+  const int64_t t = blockIdx.x;
   const int bs = 1 << a.shift;
-  const uint8_t* x0 = a.x[side] + h * a.hs[side];
+  const uint8_t* x0 = a.x[side] + h * a.hs[side] + t * a.ts[side];
+  const int d = lane % kRow * 8;
+  // lane 0 the slot before, lane 1 this one, then those after
+  const int64_t at = t - 1 + lane;
+  const int32_t mine = at >= 0 && at < a.tokens ? a.slots[at] : -1;
+  uint4 ahead = make_uint4(0, 0, 0, 0);
+  if (t + lane / kRow < a.tokens) ahead = load_u4(x0 + (lane / kRow) * a.ts[side] + d * 2);
+  const int32_t slot = __builtin_amdgcn_readlane(mine, 1), prev = __builtin_amdgcn_readlane(mine, 0);
+  const int64_t block = slot >> a.shift;
+  const int o0 = slot & (bs - 1);
+  if (slot < 0 || block >= a.num_blocks) return;
+  if (o0 != 0 && t > 0 && follows(prev, 1, slot)) return;
+  float* scale = a.scale[side] + block * a.heads + h;
+  const float held_scale = *scale;
+  const int room = bs - o0;
+  const uint64_t same = __ballot(lane == 0 || (at < a.tokens && follows(slot, lane - 1, mine))) >> 1;
+  int n = min(~same == 0 ? kWave : (int)__builtin_ctzll(~same), room);
+  for (bool more = n == kWave - 1 && n < room; more;) {
+    const int i = n + lane;
+    const uint64_t b = __ballot(i < room && t + i < a.tokens && follows(slot, i, a.slots[t + i]));
+    const int len = ~b == 0 ? kWave : (int)__builtin_ctzll(~b);
+    n += len;
+    more = len == kWave;
+  }
+  uint32_t top = lane / kRow < n ? top_bits(ahead) : 0;
+  for (int it = lane + kWave; it < n * kRow; it += kWave)
+    top = max(top, top_bits(load_u4(x0 + (it / kRow) * a.ts[side] + it % kRow * 16)));
+#pragma unroll
+  for (int m = 1; m < kWave; m <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m));
+  const Step s((float)__builtin_bit_cast(T, (uint16_t)top), o0 > 0, held_scale);
+  uint8_t* dst = a.store[side] + (block * a.heads + h) * ((int64_t)D << a.shift);
+  if (s.rise) {
+    requantize<D>(dst, side, o0, s.ratio, lane, kWave);
+    __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");  // before the bytes among them
+  }
+  if (lane == 0) *scale = s.step;
+  for (int it = lane; it < n * kRow; it += kWave) {
+    const int i = it / kRow, dd = it % kRow * 8;
+    const uint4 raw = it < kWave ? ahead : load_u4(x0 + i * a.ts[side] + dd * 2);
+    const uint2 q = s.bytes(Eight<T>::load(&raw));
+    if (side == 0) {
+      *reinterpret_cast<uint2*>(dst + k_at<D>(o0 + i, dd)) = q;
+    } else {
+      uint8_t* p = dst + v_at<D>(o0 + i, dd);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) p[j * 16] = (uint8_t)((j < 4 ? q.x : q.y) >> (8 * (j & 3)));
+    }
+  }
+}
+
+// Long runs: a workgroup begins the runs of `chunk` consecutive tokens; a run's
+// values are read once, stay in registers until its scale is known, and go out
+// through LDS in 16-byte chunks.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void kv8_append_long_kernel(AppendArgs a) {
+  constexpr int kRow = D / 8, kItems = 128 * kRow / 256, kPitch = D + 16;
+  __shared__ int32_t near_slots[256];
+  __shared__ uint32_t wave_top[4];
+  extern __shared__ __align__(16) uint8_t staged[];  // [tokens of the run][kPitch]
+  const int tid = threadIdx.x, lane = tid % kWave, h = blockIdx.y, side = blockIdx.z;
+  const int bs = 1 << a.shift;
+  const int64_t t0 = (int64_t)blockIdx.x * a.chunk;
+  {  // token t0 - 1 + tid (chunk + 128 < 256)
+    const int64_t at = t0 - 1 + tid;
+    near_slots[tid] = at >= 0 && at < a.tokens ? a.slots[at] : -1;
+  }
+  __syncthreads();
   const int64_t ts = a.ts[side];
-  const int64_t t_end = min((int64_t)(blockIdx.x + 1) * a.chunk, a.tokens);
-  for (int64_t t = (int64_t)blockIdx.x * a.chunk; t < t_end; ++t) {
-    // ---- the run that begins at t, if one does (the same in every wavefront)
-    const int32_t slot = a.slots[t];
+  // tokens of the chunk that begin a run
+  uint64_t begins;
+  {
+    const int32_t slot = near_slots[min(lane + 1, 255)], prev = near_slots[min(lane, 255)];
+    const int64_t block = slot >> a.shift;
+    const bool first = (slot & (bs - 1)) == 0 || t0 + lane == 0 || !follows(prev, 1, slot);
+    begins = __ballot(lane < a.chunk && slot >= 0 && block < a.num_blocks && first);
+  }
+  for (; begins != 0; begins &= begins - 1) {
+    const int c = (int)__builtin_ctzll(begins);
+    const int32_t slot = __builtin_amdgcn_readfirstlane(near_slots[c + 1]);
     const int64_t block = slot >> a.shift;
     const int o0 = slot & (bs - 1);
-    if (slot < 0 || block >= a.num_blocks) continue;
-    if (o0 != 0 && t > 0 && a.slots[t - 1] == slot - 1) continue;
     int n = 0;
-    for (bool more = true; more && n < bs - o0;) {
+    for (bool more = true; more && n < bs - o0;) {  // (slots past the batch are -1 there)
       const int i = n + lane;
-      const bool same = i < bs - o0 && t + i < a.tokens && a.slots[t + i] == slot + i;
-      const uint64_t b = __ballot(same);
-      const int len = b == ~0ull ? kWave : __builtin_ctzll(~b);
+      const uint64_t b = __ballot(i < bs - o0 && follows(slot, i, near_slots[min(c + 1 + i, 255)]));
+      const int len = ~b == 0 ? kWave : (int)__builtin_ctzll(~b);
       n += len;
       more = len == kWave;
     }
-    // ---- the largest magnitude, as the bits of |x| (a NaN is above infinity)
+    const uint8_t* x0 = a.x[side] + h * a.hs[side] + (t0 + c) * ts;
+    float* scale = a.scale[side] + block * a.heads + h;
+    const float held_scale = o0 > 0 ? *scale : 0.0f;
+    uint4 raw[kItems];
     uint32_t top = 0;
-    for (int it = tid; it < n * (D / 8); it += NT) {
-      const int i = it / (D / 8), d = it % (D / 8) * 8;
-      const uint4 v = load_u4(x0 + (t + i) * ts + d * 2);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        top = max(top, max(w[j] & 0x7fffu, (w[j] >> 16) & 0x7fffu));
+    for (int k = 0; k < kItems; ++k) {
+      const int it = k * 256 + tid;
+      if (it < n * kRow) raw[k] = load_u4(x0 + (it / kRow) * ts + it % kRow * 16);
     }
+#pragma unroll
+    for (int k = 0; k < kItems; ++k)
+      if (k * 256 + tid < n * kRow) top = max(top, top_bits(raw[k]));
 #pragma unroll
     for (int m = 1; m < kWave; m <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m));
-    if (lane == 0) wave_amax[tid / kWave] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < NT / kWave; ++w) top = max(top, wave_amax[w]);
-    const float amax = (float)__builtin_bit_cast(T, (uint16_t)top);
-    float* scale = a.scale[side] + block * a.heads + h;
-    const float before = o0 > 0 ? *scale : 0.0f;
-    const float fresh = amax < kLeastAmax ? 0.0f : amax * (1.0f / 127.0f);
-    // max of the two; either one not finite makes the block not finite
-    const float step = before >= fresh || before != before ? before : fresh;
-    const bool rise = o0 > 0 && !(step == before) && before == before;
-    const float ratio = rise ? before / step : 1.0f;
-    const bool some = step > 0.0f && step < __builtin_inff();  // else all zeros
-    const float r = some ? 1.0f / step : 0.0f;
-    __syncthreads();  // every thread has read the scale and wave_amax
-    if (tid == 0) *scale = step;
+    if (lane == 0) wave_top[tid / kWave] = top;
+    __syncthreads();  // (and the scale has been read)
+    top = max(max(wave_top[0], wave_top[1]), max(wave_top[2], wave_top[3]));
+    const Step s((float)__builtin_bit_cast(T, (uint16_t)top), o0 > 0, held_scale);
+    if (tid == 0) *scale = s.step;
     uint8_t* dst = a.store[side] + (block * a.heads + h) * ((int64_t)D << a.shift);
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      const int it = k * 256 + tid;
+      if (it < n * kRow)
+        *reinterpret_cast<uint2*>(staged + it / kRow * kPitch + it % kRow * 8) =
+            s.bytes(Eight<T>::load(&raw[k]));
+    }
+    if (s.rise) requantize<D>(dst, side, o0, s.ratio, tid, 256);
+    __syncthreads();  // staged; the held bytes are written
     if (side == 0) {
-      // 16 dimensions of one token are 16 consecutive bytes.
-      const int begin = rise ? 0 : o0 * (D / 16);
-      for (int it = begin + tid; it < (o0 + n) * (D / 16); it += NT) {
-        const int o = it / (D / 16), dc = it % (D / 16);  // token, 16 dimensions
-        uint8_t* p = dst + (o >> 5) * (32 * D) + ((o >> 4 & 1) * (D / 64) + (dc >> 2)) * kTileBytes +
-                     ((dc & 3) * 16 + (o & 15)) * 16;
-        uint32_t w[4];
-        if (o < o0) {
-          const uint4 v = load_u4(p);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            w[j] = 0;
-#pragma unroll
-            for (int b = 0; b < 4; ++b) w[j] |= requant_byte(byte_of(v, 4 * j + b), ratio) << (8 * b);
-          }
-        } else {
-          const uint8_t* src = x0 + (t + (o - o0)) * ts + dc * 32;
-          const floatx8 f[2] = {Eight<T>::load(src), Eight<T>::load(src + 16)};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            w[j] = 0;
-#pragma unroll
-            for (int b = 0; b < 4; ++b)
-              w[j] |= (some ? quant_byte(f[j / 2][(4 * j + b) & 7], step, r) : 128u) << (8 * b);
-          }
-        }
-        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+      // chunks in memory order: 16 dimensions of one token each
+      const int g0 = o0 >> 4, g1 = (o0 + n - 1) >> 4;  // 16-token tiles
+      for (int it = tid; it < (g1 - g0 + 1) * D; it += 256) {
+        const int o = (g0 + it / D) * 16 + it % 16, dd = it % D / 16 * 16;
+        if (o < o0 || o >= o0 + n) continue;
+        *reinterpret_cast<uint4*>(dst + k_at<D>(o, dd)) =
+            *reinterpret_cast<const uint4*>(staged + (o - o0) * kPitch + dd);
       }
     } else {
-      for (int it = tid; it < n * (D / 8); it += NT) {
-        const int i = it / (D / 8), d = it % (D / 8) * 8;
-        const floatx8 f = Eight<T>::load(x0 + (t + i) * ts + d * 2);
-        uint32_t w[2] = {0, 0};
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          w[j / 4] |= (some ? quant_byte(f[j], step, r) : 128u) << (8 * (j & 3));
-        *reinterpret_cast<uint2*>(staged + i * D + d) = make_uint2(w[0], w[1]);
-      }
-      __syncthreads();
-      // 16 bytes: two dimensions (e) of tokens q + c and 16 + q + c (h4).
-      const int g0 = rise ? 0 : o0 >> 5, g1 = (o0 + n - 1) >> 5;
-      for (int it = tid; it < (g1 - g0 + 1) * (2 * D); it += NT) {
-        const int gr = g0 + it / (2 * D), c16 = it % (2 * D);
-        const int dt = c16 / kWave, l = c16 % kWave;
-        const int tok = gr * 32 + 4 * (l / 16), dim = dt * 32 + l % 16;
-        const auto is_new = [&](int o) { return o >= o0 && o < o0 + n; };
+      // Four dimensions of eight tokens a thread: bytes [token][dimension] of
+      // LDS become 8 bytes [token] of each dimension's chunk.
+      const int g0 = o0 >> 5, g1 = (o0 + n - 1) >> 5;
+      for (int it = tid; it < (g1 - g0 + 1) * D; it += 256) {
+        const int gr = g0 + it / D, dq = it % 4, e = it / 4 % 2, g = it / 8 % 4, dt = it % D / 32;
+        const int tok = gr * 32 + 4 * g, dim = dt * 32 + 16 * e + 4 * dq;
+        const auto fresh = [&](int o) { return o >= o0 && o < o0 + n; };
         const bool any = (tok < o0 + n && tok + 4 > o0) || (tok + 16 < o0 + n && tok + 20 > o0);
-        if (!any && !(rise && tok < o0)) continue;
-        uint8_t* p = dst + gr * (32 * D) + c16 * 16;
-        const bool all = is_new(tok) && is_new(tok + 19);
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (!all) v = load_u4(p);
-        uint32_t w[4];
+        if (!any) continue;
+        uint8_t* p = dst + gr * (32 * D) + dt * kTileBytes + (g * 16 + 4 * dq) * 16 + 8 * e;
+        uint32_t out[4][2];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          w[j] = 0;
+        for (int half = 0; half < 2; ++half) {
+          uint32_t w[4];
 #pragma unroll
           for (int b = 0; b < 4; ++b) {
-            const int o = tok + 16 * (j & 1) + b, d = dim + 16 * (j >> 1);
-            uint32_t u = byte_of(v, 4 * j + b);
-            if (is_new(o)) u = staged[(o - o0) * D + d];
-            else if (rise && o < o0) u = requant_byte(u, ratio);
-            w[j] |= u << (8 * b);
+            const int o = min(max(tok + 16 * half + b - o0, 0), n - 1);
+            w[b] = *reinterpret_cast<const uint32_t*>(staged + o * kPitch + dim);
           }
+          const uint32_t l01 = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u);  // dims 0, 1 of tokens 0, 1
+          const uint32_t h01 = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u);  // dims 2, 3
+          const uint32_t l23 = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u);
+          const uint32_t h23 = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+          out[0][half] = __builtin_amdgcn_perm(l23, l01, 0x05040100u);
+          out[1][half] = __builtin_amdgcn_perm(l23, l01, 0x07060302u);
+          out[2][half] = __builtin_amdgcn_perm(h23, h01, 0x05040100u);
+          out[3][half] = __builtin_amdgcn_perm(h23, h01, 0x07060302u);
         }
-        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        if (fresh(tok) && fresh(tok + 19)) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<uint2*>(p + j * 16) = make_uint2(out[j][0], out[j][1]);
+        } else {  // the run begins or ends among these tokens
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int b = 0; b < 8; ++b)
+              if (fresh(tok + 16 * (b / 4) + b % 4)) p[j * 16 + b] = (uint8_t)(out[j][b / 4] >> (8 * (b % 4)));
+        }
       }
     }
-    __syncthreads();  // staged and wave_amax are reused by the next run
+    __syncthreads();  // staged and wave_top are reused by the next run
   }
 }
 
@@ -395,24 +571,18 @@ struct ReadArgs {
 
 template <typename T, int D>
 __global__ __launch_bounds__(256) void kv8_read_kernel(ReadArgs a) {
-  const int64_t it = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int d = it % (D / 8) * 8;
-  const int64_t th = it / (D / 8), t = th / a.heads;
-  const int h = (int)(th % a.heads);
+  constexpr int kRow = D / 8;
+  const int d = threadIdx.x % kRow * 8, h = blockIdx.y;
+  const int64_t t = (int64_t)blockIdx.x * (256 / kRow) + threadIdx.x / kRow;
   if (t >= a.n) return;
   const int32_t slot = a.slots[t];
   const int64_t block = slot >> a.shift;
   floatx8 kf = 0.0f, vf = 0.0f;
   if (slot >= 0 && block < a.num_blocks) {
     const int o = slot & ((1 << a.shift) - 1);
-    const int64_t at = block * a.heads + h;
-    const uint8_t* kp = a.k + at * ((int64_t)D << a.shift) + (o >> 5) * (32 * D) +
-                        ((o >> 4 & 1) * (D / 64) + d / 64) * kTileBytes +
-                        ((d / 16 & 3) * 16 + (o & 15)) * 16 + (d & 8);
-    const uint2 kb = *reinterpret_cast<const uint2*>(kp);
-    const uint8_t* vp = a.v + at * ((int64_t)D << a.shift) + (o >> 5) * (32 * D) +
-                        d / 32 * kTileBytes + ((o >> 2 & 3) * 16 + (d & 8)) * 16 + (d >> 4 & 1) * 8 +
-                        (o >> 4 & 1) * 4 + (o & 3);
+    const int64_t at = block * a.heads + h, base = at * ((int64_t)D << a.shift);
+    const uint2 kb = *reinterpret_cast<const uint2*>(a.k + base + k_at<D>(o, d));
+    const uint8_t* vp = a.v + base + v_at<D>(o, d);
     const float ks = a.ks[at], vs = a.vs[at];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -420,41 +590,49 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(ReadArgs a) {
       vf[j] = (float)((int)vp[j * 16] - 128) * vs;
     }
   }
-  const int64_t to = (th * D + d) * (int64_t)sizeof(T);
+  const int64_t to = ((t * a.heads + h) * D + d) * (int64_t)sizeof(T);
   Eight<T>::store(a.k_out + to, kf);
   Eight<T>::store(a.v_out + to, vf);
 }
 
 inline int log2i(int v) { return __builtin_ctz((unsigned)v); }
 
-template <typename T>
-hipError_t rope_typed(const RopeArgs& r, dim3 grid, int threads, hipStream_t stream) {
-  if (r.D <= 64) qk_norm_rope_kernel<T, 8><<<grid, threads, 0, stream>>>(r);
-  else if (r.D <= 128) qk_norm_rope_kernel<T, 16><<<grid, threads, 0, stream>>>(r);
-  else if (r.D <= 256) qk_norm_rope_kernel<T, 32><<<grid, threads, 0, stream>>>(r);
-  else qk_norm_rope_kernel<T, 64><<<grid, threads, 0, stream>>>(r);
+template <typename T, int LP>
+hipError_t rope_sized(const RopeArgs& r, bool interleaved, unsigned grid, hipStream_t stream) {
+  if (interleaved) qk_norm_rope_kernel<T, LP, true><<<grid, 256, 0, stream>>>(r);
+  else qk_norm_rope_kernel<T, LP, false><<<grid, 256, 0, stream>>>(r);
   return hipGetLastError();
+}
+
+template <typename T>
+hipError_t rope_typed(const RopeArgs& r, bool interleaved, unsigned grid, hipStream_t stream) {
+  return r.D <= 64    ? rope_sized<T, 8>(r, interleaved, grid, stream)
+         : r.D <= 128 ? rope_sized<T, 16>(r, interleaved, grid, stream)
+         : r.D <= 256 ? rope_sized<T, 32>(r, interleaved, grid, stream)
+                      : rope_sized<T, 64>(r, interleaved, grid, stream);
 }
 
 template <typename T, int D>
-hipError_t append_sized(const AppendArgs& a, bool wide, hipStream_t stream) {
-  const dim3 grid((unsigned)ceil_div(a.tokens, a.chunk), (unsigned)a.heads, 2);
-  const size_t lds = wide ? (size_t)D << a.shift : (size_t)D << a.shift;
-  if (wide) kv8_append_kernel<T, D, 256><<<grid, 256, lds, stream>>>(a);
-  else kv8_append_kernel<T, D, 64><<<grid, 64, lds, stream>>>(a);
+hipError_t append_sized(const AppendArgs& a, bool many, hipStream_t stream) {
+  if (many) {
+    const dim3 grid((unsigned)ceil_div(a.tokens, a.chunk), (unsigned)a.heads, 2);
+    kv8_append_long_kernel<T, D><<<grid, 256, (size_t)(D + 16) << a.shift, stream>>>(a);
+  } else {
+    kv8_append_short_kernel<T, D><<<dim3((unsigned)a.tokens, (unsigned)a.heads, 2), kWave, 0, stream>>>(a);
+  }
   return hipGetLastError();
 }
 
 template <typename T>
-hipError_t append_typed(const AppendArgs& a, int D, bool wide, hipStream_t stream) {
-  return D == 64 ? append_sized<T, 64>(a, wide, stream)
-         : D == 128 ? append_sized<T, 128>(a, wide, stream)
-                    : append_sized<T, 256>(a, wide, stream);
+hipError_t append_typed(const AppendArgs& a, int D, bool many, hipStream_t stream) {
+  return D == 64 ? append_sized<T, 64>(a, many, stream)
+         : D == 128 ? append_sized<T, 128>(a, many, stream)
+                    : append_sized<T, 256>(a, many, stream);
 }
 
 template <typename T>
 hipError_t read_typed(const ReadArgs& a, int D, hipStream_t stream) {
-  const unsigned grid = (unsigned)ceil_div(a.n * a.heads * (D / 8), 256);
+  const dim3 grid((unsigned)ceil_div(a.n, 256 / (D / 8)), (unsigned)a.heads);
   if (D == 64) kv8_read_kernel<T, 64><<<grid, 256, 0, stream>>>(a);
   else if (D == 128) kv8_read_kernel<T, 128><<<grid, 256, 0, stream>>>(a);
   else kv8_read_kernel<T, 256><<<grid, 256, 0, stream>>>(a);
@@ -478,22 +656,27 @@ hipError_t launch_qk_norm_rope(const rf_kv8_rope_args& a, hipStream_t stream) {
   r.cos = a.cos;
   r.sin = a.sin;
   r.pos = a.positions;
-  r.tokens = a.tokens;
+  r.tokens = (int)a.tokens;
   r.table_rows = a.table_rows;
   r.pos64 = a.positions64;
   r.hq = a.q.heads;
   r.hk = a.k.heads;
   r.D = a.head_dim;
   r.rot = a.rot;
-  r.interleaved = a.interleaved;
   r.eps = a.eps;
-  const int lanes = a.head_dim <= 64 ? 8 : a.head_dim <= 128 ? 16 : a.head_dim <= 256 ? 32 : 64;
-  const int at_once = kWave / lanes, heads = r.hq + r.hk;
-  r.per_wave = at_once;
-  const int waves = 4;
-  const dim3 grid((unsigned)a.tokens, (unsigned)ceil_div(heads, (int64_t)r.per_wave * waves));
-  return a.dtype == RF_W8A16_DTYPE_F16 ? rope_typed<_Float16>(r, grid, waves * kWave, stream)
-                                       : rope_typed<__bf16>(r, grid, waves * kWave, stream);
+  const int lanes = r.D <= 64 ? 8 : r.D <= 128 ? 16 : r.D <= 256 ? 32 : 64;
+  // Few tokens: a wavefront per kHeads heads.  Many: as many heads per wavefront
+  // as leave about 16 wavefronts for each CU.
+  const int64_t at_once = kWave / lanes, q_turns = ceil_div(r.hq, at_once), k_turns = ceil_div(r.hk, at_once);
+  int64_t each = r.tokens * (q_turns + k_turns) / 4096;
+  each = each < 1 ? 1 : each > q_turns ? q_turns : each;
+  r.turns = (int)each;
+  r.q_parts = (int)ceil_div(q_turns, each);
+  r.parts = r.q_parts + (int)ceil_div(k_turns, each);
+  const int64_t grid = ceil_div((int64_t)r.tokens * r.parts, 256 / kWave);
+  return a.dtype == RF_W8A16_DTYPE_F16
+             ? rope_typed<_Float16>(r, a.interleaved, (unsigned)grid, stream)
+             : rope_typed<__bf16>(r, a.interleaved, (unsigned)grid, stream);
 }
 
 hipError_t launch_kv8_plan(const rf_kv8_plan_args& a, hipStream_t stream) {
@@ -522,10 +705,10 @@ hipError_t launch_kv8_append(const rf_kv8_cache& c, const rf_kv8_heads& k, const
   a.num_blocks = c.num_blocks;
   a.heads = c.kv_heads;
   a.shift = log2i(c.block_size);
-  a.chunk = 1;
-  const bool wide = false;
-  return dtype == RF_W8A16_DTYPE_F16 ? append_typed<_Float16>(a, c.head_dim, wide, stream)
-                                     : append_typed<__bf16>(a, c.head_dim, wide, stream);
+  a.chunk = 16;
+  const bool many = tokens > 1024;
+  return dtype == RF_W8A16_DTYPE_F16 ? append_typed<_Float16>(a, c.head_dim, many, stream)
+                                     : append_typed<__bf16>(a, c.head_dim, many, stream);
 }
 
 hipError_t launch_kv8_read(const rf_kv8_cache& c, const int32_t* slots, int64_t n, int dtype,
