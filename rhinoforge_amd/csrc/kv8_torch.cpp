@@ -16,6 +16,7 @@
 // the manner of w8a16_torch.cpp: dtype and shape first (shared with the Meta
 // kernels), then devices; invalid input raises, there is no CPU computation.
 #include <ATen/ATen.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
@@ -66,6 +67,12 @@ void check_same_device(const at::Tensor& t, const at::Tensor& first, const char*
 
 void* stream_of(const at::Tensor& t) {
   return c10::hip::getCurrentHIPStream(t.device().index()).stream();
+}
+
+// A new contiguous tensor, straight from the caching allocator (at::empty's way
+// there through the dispatcher is a third of what a single-token call costs).
+at::Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType dtype, const at::Tensor& like) {
+  return at::detail::empty_cuda(sizes, dtype, like.device(), c10::nullopt);
 }
 
 bool aligned16(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
@@ -144,7 +151,7 @@ Two rope_hip(const at::Tensor& q, const at::Tensor& k, const OptTensor& qw, cons
   rf_kv8_rope_args a{};
   a.q = heads_of(q, &keep[0]);
   a.k = heads_of(k, &keep[1]);
-  at::Tensor qo = at::empty(q.sizes(), q.options()), ko = at::empty(k.sizes(), k.options());
+  at::Tensor qo = new_tensor(q.sizes(), q.scalar_type(), q), ko = new_tensor(k.sizes(), k.scalar_type(), k);
   a.q_out = qo.data_ptr();
   a.k_out = ko.data_ptr();
   if (given(qw)) a.q_weight = (keep[2] = aligned_copy(*qw)).data_ptr();
@@ -222,7 +229,9 @@ Five plan_hip(at::Tensor& table, const at::Tensor& cached, const at::Tensor& fre
   check_same_device(free_blocks, table, op, "free_blocks");
   check_same_device(start, table, op, "free_start");
   c10::DeviceGuard dev_guard(table.device());
-  Five out = plan_outputs(cached, tokens);
+  const int64_t B = cached.size(0);
+  const auto ints = [&](int64_t n) { return new_tensor({n}, at::kInt, table); };
+  Five out{ints(tokens), ints(tokens), ints(B + 1), ints(B), ints(1)};
   rf_kv8_plan_args a{};
   a.block_table = table.data_ptr<int32_t>();
   a.cached = cached.data_ptr<int32_t>();
@@ -331,13 +340,18 @@ void append_cpu(at::Tensor& kc, at::Tensor& vc, at::Tensor& ks, at::Tensor& vs, 
   no_cpu("kv8::append");
 }
 
-Two read_outputs(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks,
-                 const at::Tensor& vs, const at::Tensor& slots, at::ScalarType dtype) {
+void check_read(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks,
+                const at::Tensor& vs, const at::Tensor& slots, at::ScalarType dtype) {
   const char* op = "kv8::read";
   check_cache(kc, vc, ks, vs, op);
   check_ints(slots, 1, op, "slots");
   TORCH_CHECK(dtype == at::kHalf || dtype == at::kBFloat16 || dtype == at::kFloat, op,
               ": dtype must be float16, bfloat16 or float32, got ", dtype);
+}
+
+Two read_meta(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks, const at::Tensor& vs,
+              const at::Tensor& slots, at::ScalarType dtype) {
+  check_read(kc, vc, ks, vs, slots, dtype);
   const std::vector<c10::SymInt> shape = {slots.sym_size(0), kc.sym_size(1), kc.sym_size(3) * 32};
   const auto o = kc.options().dtype(dtype);
   return {at::empty_symint(shape, o), at::empty_symint(shape, o)};
@@ -347,7 +361,9 @@ Two read_hip(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks, c
              const at::Tensor& slots, at::ScalarType dtype) {
   RECORD_FUNCTION("kv8::read", {});
   const char* op = "kv8::read";
-  Two out = read_outputs(kc, vc, ks, vs, slots, dtype);
+  check_read(kc, vc, ks, vs, slots, dtype);
+  const std::vector<int64_t> shape = {slots.size(0), kc.size(1), kc.size(3) * 32};
+  Two out{new_tensor(shape, dtype, kc), new_tensor(shape, dtype, kc)};
   const rf_kv8_cache c = cache_of(kc, vc, ks, vs, op);
   check_same_device(slots, kc, op, "slots");
   if (slots.numel() == 0) return out;
@@ -360,7 +376,7 @@ Two read_hip(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks, c
 
 Two read_cpu(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks, const at::Tensor& vs,
              const at::Tensor& slots, at::ScalarType dtype) {
-  read_outputs(kc, vc, ks, vs, slots, dtype);
+  check_read(kc, vc, ks, vs, slots, dtype);
   no_cpu("kv8::read");
 }
 
@@ -413,9 +429,8 @@ Two attention_hip(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& v
   check_same_device(lens, q, op, "kv_lens");
   if (given(cu)) check_same_device(*cu, q, op, "cu_q");
   c10::DeviceGuard dev_guard(q.device());
-  at::Tensor out = at::empty(q.sizes(), q.options());
-  at::Tensor lse = return_lse ? at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat))
-                              : at::empty({0}, q.options().dtype(at::kFloat));
+  at::Tensor out = new_tensor(q.sizes(), q.scalar_type(), q);
+  at::Tensor lse = return_lse ? new_tensor({q.size(0), q.size(1)}, at::kFloat, q) : new_tensor({0}, at::kFloat, q);
   if (q.size(0) == 0) return {out, lse};
   at::Tensor keep;
   a.q = heads_of(q, &keep);
@@ -492,7 +507,7 @@ TORCH_LIBRARY_IMPL(kv8, Meta, m) {
   m.impl("qk_norm_rope", TORCH_FN(rope_meta));
   m.impl("plan", TORCH_FN(plan_meta));
   m.impl("append", TORCH_FN(append_meta));
-  m.impl("read", TORCH_FN(read_outputs));
+  m.impl("read", TORCH_FN(read_meta));
   m.impl("attention", TORCH_FN(attention_meta));
 }
 TORCH_LIBRARY_IMPL(kv8, CPU, m) {

@@ -20,6 +20,11 @@ from typing import NamedTuple
 
 import torch
 
+# (resolved once: single-token calls are bound by the host)
+_ops = torch.ops.kv8
+_qk_norm_rope, _plan, _append = _ops.qk_norm_rope.default, _ops.plan.default, _ops.append.default
+_read, _attention = _ops.read.default, _ops.attention.default
+
 GROUP = 32          # tokens of one group of tiles
 BLOCK_SIZES = (32, 64, 128)
 HEAD_DIMS = (64, 128, 256)
@@ -133,7 +138,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
     NaN.  Pairs are (i, i + rot / 2), with ``interleaved`` (2i, 2i + 1).
     fp32 throughout, one rounding.  Returns new contiguous (q, k).
     """
-    return torch.ops.kv8.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+    return _qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
 
 
 def rope_table(inv_freq: torch.Tensor, rows: int):
@@ -157,8 +162,8 @@ def kv8_plan(block_table: torch.Tensor, cached_lens: torch.Tensor, new_lens: tor
     ``free_next[0] > free_blocks.numel()`` says that the blocks ran out; tokens
     without a block have slot -1, which :func:`kv8_append` skips.
     """
-    return KV8Plan(*torch.ops.kv8.plan(block_table, cached_lens, new_lens, free_blocks, free_start,
-                                       num_tokens, block_size))
+    return KV8Plan(*_plan(block_table, cached_lens, new_lens, free_blocks, free_start, num_tokens,
+                          block_size))
 
 
 def kv8_append(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
@@ -172,13 +177,13 @@ def kv8_append(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.T
     consecutive in the batch, as :func:`kv8_plan` makes them.  A block that
     gets an infinity or NaN reads back as NaN (that head, k or v).
     """
-    torch.ops.kv8.append(*cache.tensors(), k, v, slots)
+    _append(*cache.tensors(), k, v, slots)
 
 
 def kv8_read(cache: KV8Cache, slots: torch.Tensor, dtype: torch.dtype = torch.float16):
     """Cached tokens as values: (k, v), each [n, kv_heads, head_dim] of fp16,
     bf16 or fp32, for int32 ``slots`` [n]; a slot outside the cache gives zeros."""
-    return torch.ops.kv8.read(*cache.tensors(), slots, dtype)
+    return _read(*cache.tensors(), slots, dtype)
 
 
 def kv8_attention(q: torch.Tensor, cache: KV8Cache, block_table: torch.Tensor,
@@ -202,6 +207,6 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, block_table: torch.Tensor,
     type, with ``return_lse`` also the natural log-sum-exp, fp32 [tokens, heads].
     """
     scale = cache.head_dim ** -0.5 if scale is None else scale
-    out, lse = torch.ops.kv8.attention(q, *cache.tensors(), block_table, kv_lens, cu_q, max_q_len,
-                                       max_kv_len, causal, window, scale, return_lse)
+    out, lse = _attention(q, *cache.tensors(), block_table, kv_lens, cu_q, max_q_len, max_kv_len,
+                          causal, window, scale, return_lse)
     return (out, lse) if return_lse else out
