@@ -19,6 +19,8 @@
 //     small weights stay normal.
 //   * vs goes into p as vs / max(vs so far): 2^log2 of it joins the exponent.
 //     The sum over p divides it out again.  m, the sums and o stay in fp32.
+#include <math.h>
+
 #include "kv8_common.h"
 
 namespace rf {
@@ -37,14 +39,15 @@ struct AttnArgs {
   const int32_t *cu, *lens, *table;
   uint8_t* out;
   float* lse;
-  uint32_t* counters;  // one per tile and key head, zero between launches
-  float* part;         // [tokens * heads][splits][D], unnormalized
-  uint64_t* stat;      // [tokens * heads][splits]: m, l
+  uint32_t* counters;  // one per tile and key head, at most, zero between launches
+  float* part;         // unnormalized, [tokens * heads][splits][D], or [workgroups][R][D]
+  uint64_t* stat;      // m, l, likewise
   int64_t table_stride;
   int num_blocks;
   int tokens, requests, width, hq, hk, group, shift;
   int per_request;     // cu == nullptr: queries of a request
   int splits, least, tiles;
+  int shares;          // find_share: of all tiles together (0: not used)
   bool merge;          // partial results are added by kv8_merge_kernel, else by join()
   int causal, window;  // window 0: none
   float scale_log2e;
@@ -146,6 +149,17 @@ __device__ __forceinline__ bool find_tile(const AttnArgs& a, int x, Tile* t) {
   return true;
 }
 
+// Sums and maxima over the lanes up to each one.
+template <typename Op>
+__device__ __forceinline__ int scan(int v, Op op) {  // op(v, 0) == v
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false));  // row_shr:1
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false));  // row_shr:2
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false));  // row_shr:4
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false));  // row_shr:8
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));  // row_bcast:15
+  return op(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));  // row_bcast:31
+}
+
 // Tokens [lo, hi) that row `row` of a request sees.
 __device__ __forceinline__ void seen(const AttnArgs& a, const Tile& t, int row, int* lo, int* hi) {
   *lo = 0;
@@ -157,14 +171,112 @@ __device__ __forceinline__ void seen(const AttnArgs& a, const Tile& t, int row, 
   }
 }
 
+// Split `split` of tile `tile` as workgroup x of a batch of unequal lengths
+// finds it.  Every tile is cut into shares of at most L groups, with the
+// smallest L that leaves no more than `shares` of them: a batch takes as long as
+// its mean, not as its longest request, and its workgroups fill the CUs evenly.
+// Each lane holds ceil(requests / 64) requests, so up to 64 of them cost one
+// memory round trip; for more, L is a bound that needs no search.
+template <int R>
+__device__ __forceinline__ bool find_share(const AttnArgs& a, int x, Tile* t, int* split, int* splits) {
+  struct Entry {
+    int first, queries, tiles, len, n;  // n: groups that its last tile sees
+  };
+  const int lane = threadIdx.x % kWave, entries = a.requests + (a.cu ? 1 : 0);
+  const int per = (int)((unsigned)(entries + kWave - 1) / kWave);
+  const auto entry = [&](int b) {  // (b == requests: the tokens past the batch, which see nothing)
+    Entry e;
+    e.len = b < a.requests ? min(max(a.lens[b], 0), a.width << a.shift) : 0;
+    e.first = a.cu ? cu_at(a, b) : b * a.per_request;
+    e.queries = b >= entries ? 0 : a.cu ? max(cu_at(a, b + 1) - e.first, 0) : a.per_request;
+    e.tiles = (int)(((unsigned)(e.queries * a.group) + R - 1) / R);
+    int lo = 0;
+    if (a.causal && a.window > 0) {
+      const int query = (int)((unsigned)(max(e.tiles - 1, 0) * R) / (unsigned)a.group);
+      lo = max(e.len - e.queries + query - a.window + 1, 0);
+    }
+    e.n = max(((e.len + 31) >> 5) - (lo >> 5), 0);
+    return e;
+  };
+  const auto add = [](int u, int v) { return u + v; };
+  const auto most = [](int u, int v) { return max(u, v); };
+  Entry e;
+  int work = 0, longest = 0, tiles = 0;
+  for (int j = 0; j < per; ++j) {
+    e = entry(lane * per + j);
+    work += e.tiles * e.n;
+    longest = max(longest, e.n);
+    tiles += e.tiles;
+  }
+  const auto all = [&](int v) { return __builtin_amdgcn_readlane(scan(v, add), kWave - 1); };
+  const unsigned total = (unsigned)all(work);
+  const int over = a.shares - all(tiles);  // sum ceil(n / L) < sum n / L + tiles
+  longest = __builtin_amdgcn_readlane(scan(longest, most), kWave - 1);
+  const auto ratio = [](unsigned u, unsigned v) { return (u + v - 1) / v; };
+  const unsigned least = max((unsigned)a.least, ratio((unsigned)longest, (unsigned)a.splits));
+  unsigned length = max(over > 0 ? min(ratio(total, (unsigned)over), (unsigned)longest) : (unsigned)longest, least);
+  // ceil(n / length) or, by rounding, one less (never more: there is room for
+  // `shares`); all workgroups come to the same
+  const auto cut = [](int n, unsigned length) {
+    const float inv = (1.0f - 0x1p-20f) * __builtin_amdgcn_rcpf((float)length);
+    return max((int)__builtin_ceilf((float)n * inv), 1);
+  };
+  if (per == 1) {
+    unsigned few = max(ratio(total, (unsigned)a.shares), least) - 1;  // too short, or not allowed
+    for (int i = 0; i < 7 && few + 1 < length; ++i) {
+      const unsigned mid = (few + length) / 2;
+      const bool fits = all(__mul24(e.tiles, cut(e.n, mid))) <= a.shares;
+      if (fits) length = mid;
+      else few = mid;
+    }
+  }
+  int count = 0;
+  if (per == 1) count = e.tiles * cut(e.n, length);
+  else
+    for (int j = 0; j < per; ++j) {
+      const Entry o = entry(lane * per + j);
+      count += o.tiles * cut(o.n, length);
+    }
+  const int upto = scan(count, add);
+  const int holder = __popcll(__ballot(upto <= x));
+  if (holder >= kWave) return false;
+  int rest = x - (__builtin_amdgcn_readlane(upto, holder) - __builtin_amdgcn_readlane(count, holder));
+  int b = holder * per;
+  if (per == 1) {
+    e.first = __builtin_amdgcn_readlane(e.first, b);
+    e.queries = __builtin_amdgcn_readlane(e.queries, b);
+    e.len = __builtin_amdgcn_readlane(e.len, b);
+    e.n = __builtin_amdgcn_readlane(e.n, b);
+  } else {
+    for (int j = 0; j < per; ++j, ++b) {
+      e = entry(b);
+      const int its = e.tiles * cut(e.n, length);
+      if (rest < its || j == per - 1) break;
+      rest -= its;
+    }
+  }
+  const int c = cut(e.n, length), tile = (int)((unsigned)rest / (unsigned)c);
+  *split = uniform(rest - tile * c);
+  *splits = uniform(c);
+  b = uniform(b);
+  t->first_token = uniform(e.first);
+  t->queries = uniform(e.queries);
+  t->row0 = uniform(tile * R);
+  t->kv_len = uniform(e.len);
+  t->table = a.table + (b < a.requests ? b * a.table_stride : 0);
+  // (offsets that are not in order may ask for more tiles than there is room
+  // for: then a tile runs with all of its shares or not at all)
+  return t->row0 < t->queries * a.group && x - *split + *splits <= a.shares;
+}
+
 // The 32-token groups [begin, end) of one split of a tile, and how many splits
 // the tile has: the launch's, or fewer of at least `least` groups.
 struct Share {
   int begin, end, splits;
 };
-__device__ __forceinline__ Share share_of(const AttnArgs& a, int g_lo, int g_hi, int split) {
+__device__ __forceinline__ Share share_of(const AttnArgs& a, int g_lo, int g_hi, int split, int splits) {
   const int n = max(g_hi - g_lo, 0);
-  const int per = max((n + a.splits - 1) / a.splits, a.least);
+  const int per = max((n + splits - 1) / splits, a.least);
   Share r;
   r.begin = g_lo + min(split * per, n);
   r.end = min(r.begin + per, g_lo + n);
@@ -312,10 +424,11 @@ __device__ __forceinline__ void no_share(const AttnArgs& a, const Tile& t, int h
 }
 
 // All threads call it after their stores of partial results.  buf: LDS of
-// rows * splits * 8 + 4096 bytes, free for use.
+// rows * splits * 8 + 4096 bytes, free for use.  Row rc of split s is at
+// first + s * stride + rc of the partial results.
 template <typename T, int D>
 __device__ __forceinline__ void join(const AttnArgs& a, const Tile& t, int h, int rows, int splits,
-                                     uint32_t* counter, float* buf) {
+                                     int first, int stride, uint32_t* counter, float* buf) {
   const int tid = threadIdx.x;
   __shared__ int is_last;
   __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wavefront's stores are done
@@ -341,18 +454,18 @@ __device__ __forceinline__ void join(const AttnArgs& a, const Tile& t, int h, in
   for (int i = tid; i < rows * splits; i += kThreads) {
     const int rc = (int)((unsigned)i / (unsigned)splits);
     *reinterpret_cast<floatx2*>(stat + 2 * i) =
-        parts.load_stat((int)out_row(a, t, h, rc) * a.splits + (i - rc * splits));
+        parts.load_stat(first + (i - rc * splits) * stride + rc);
   }
   for (int u0 = 0; u0 < units; u0 += kThreads) {
     const int way = ways == 1 ? 0 : (int)((unsigned)tid / (unsigned)units);
     const int u = u0 + (ways == 1 ? tid : tid - way * units);
     const bool on = u < units && way < ways;
     const int rc = on ? u / (D / 4) : 0, d = u % (D / 4) * 4;
-    const int to = (int)out_row(a, t, h, rc);
-    const int at = to * a.splits * D + d;
+    const int64_t to = out_row(a, t, h, rc);
+    const int at = (first + rc) * D + d, next = stride * D;
     floatx4 x[kFlight];
 #pragma unroll
-    for (int k = 0; k < kFlight; ++k) x[k] = parts.load(at + min(way + k * ways, splits - 1) * D);
+    for (int k = 0; k < kFlight; ++k) x[k] = parts.load(at + min(way + k * ways, splits - 1) * next);
     if (u0 == 0) __syncthreads();  // stat
     const float* st = stat + rc * splits * 2;
     float m = -__builtin_inff(), l = 0.0f;
@@ -366,7 +479,7 @@ __device__ __forceinline__ void join(const AttnArgs& a, const Tile& t, int h, in
       if (s0 + kFlight * ways < splits) {
 #pragma unroll
         for (int k = 0; k < kFlight; ++k)
-          x[k] = parts.load(at + min(s0 + (kFlight + k) * ways, splits - 1) * D);
+          x[k] = parts.load(at + min(s0 + (kFlight + k) * ways, splits - 1) * next);
       }
 #pragma unroll
       for (int k = 0; k < kFlight; ++k) {
@@ -422,17 +535,24 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_decode_kernel(AttnArgs a) {
   const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int col = lane % 16, lg = lane / 16;
   const unsigned id = blockIdx.x, pair = id / (unsigned)a.hk;
-  const int h = (int)(id - pair * a.hk), x = (int)(pair / (unsigned)a.splits);
+  const int h = (int)(id - pair * a.hk);
+  int split, splits;
   Tile t;
-  if (!find_tile<R>(a, x, &t)) return;
+  if (a.shares) {
+    if (!find_share<R>(a, (int)pair, &t, &split, &splits)) return;
+  } else {
+    const int x = (int)(pair / (unsigned)a.splits);
+    if (!find_tile<R>(a, x, &t)) return;
+    splits = a.splits;
+    split = (int)(pair - (unsigned)x * splits);
+  }
   const int rows = min(t.queries * a.group - t.row0, R);  // of this tile
   // its first and last rows bound what any row sees
   int lo_min, lo_max, hi_min, hi_max;
   seen(a, t, t.row0, &lo_min, &hi_min);
   seen(a, t, t.row0 + rows - 1, &lo_max, &hi_max);
   lo_max = uniform(lo_max), hi_min = uniform(hi_min);
-  const int split = (int)(pair - (unsigned)x * a.splits);
-  const Share share = share_of(a, lo_min >> 5, (hi_max + 31) >> 5, split);
+  const Share share = share_of(a, lo_min >> 5, (hi_max + 31) >> 5, split, splits);
   if (split >= share.splits) {
     if (a.merge) no_share(a, t, h, rows, split);
     return;
@@ -653,7 +773,7 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_decode_kernel(AttnArgs a) {
       const int64_t to = out_row(a, t, h, rc);
       if (partial) {
         const Partials parts(a);
-        const int i = (int)to * a.splits + split;
+        const int i = a.merge ? (int)to * a.splits + split : (int)id * R + rc;
         parts.store(i * D + d, o);
         if (d == 0) parts.store_stat(i, mm, l);
       } else {
@@ -662,7 +782,8 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_decode_kernel(AttnArgs a) {
     }
   }
   if (partial && !a.merge)
-    join<T, D>(a, t, h, rows, share.splits, a.counters + (unsigned)x * a.hk + h, &red[0][0][0]);
+    join<T, D>(a, t, h, rows, share.splits, ((int)id - split * a.hk) * R, a.hk * R,
+               a.counters + (id - (unsigned)(split * a.hk)), &red[0][0][0]);
 }
 
 // ---------------------------------------------------------------------------
@@ -699,7 +820,7 @@ __attribute__((amdgpu_waves_per_eu(RT == 1 ? 2 : 1))) void kv8_prefill_kernel(At
   int lo_min, hi_max, unused;
   seen(a, t, t.row0, &lo_min, &unused);
   seen(a, t, t.row0 + rows - 1, &unused, &hi_max);
-  const Share share = share_of(a, lo_min >> 5, (hi_max + 31) >> 5, split);
+  const Share share = share_of(a, lo_min >> 5, (hi_max + 31) >> 5, split, a.splits);
   if (split >= share.splits) {
     no_share(a, t, h, rows, split);
     return;
@@ -767,46 +888,49 @@ __attribute__((amdgpu_waves_per_eu(RT == 1 ? 2 : 1))) void kv8_prefill_kernel(At
   }
 
   // Chunk c of this wavefront is 1 KB tile c * kWaves + wave of the step.  A
-  // step's bytes and scales are loaded one step ahead, its block ids two.
-  uint4 kr[kChunks], vr[kChunks];
+  // step's bytes and scales are loaded two steps ahead (a short share is bound
+  // by their round trip), its block ids three.
+  struct Ahead {
+    uint4 k[kChunks], v[kChunks];
+    uint32_t ks[NG], vs[NG];
+  };
   Group ids[NG];
-  uint32_t ks_next[NG], vs_next[NG];
   const auto look = [&](int g) {
 #pragma unroll
     for (int n = 0; n < NG; ++n) ids[n] = group_of(a, t, h, min(g + n, end - 1));
   };
-  const auto load = [&] {
+  const auto load = [&](Ahead& x) {
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
       const int tile = c * kWaves + wave;
       const Group& gr = NG == 1 || (D == 64 ? wave < 2 : c == 0) ? ids[0] : ids[NG - 1];
       const int64_t at = (gr.at << a.shift) * D + gr.sub * (32 * D) + tile % (D / 32) * kTileBytes + lane * 16;
-      kr[c] = load_u4(a.k + at);
-      vr[c] = load_u4(a.v + at);
+      x.k[c] = load_u4(a.k + at);
+      x.v[c] = load_u4(a.v + at);
     }
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
-      ks_next[n] = scale_bits(a.ks, ids[n]);
-      vs_next[n] = scale_bits(a.vs, ids[n]);
+      x.ks[n] = scale_bits(a.ks, ids[n]);
+      x.vs[n] = scale_bits(a.vs, ids[n]);
     }
   };
   const int g16 = lane / 16, l16 = lane % 16;
-  const auto stage = [&](uint8_t* buf) {
+  const auto stage = [&](uint8_t* buf, const Ahead& x) {
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
       const int tile = c * kWaves + wave, gr = tile / (D / 32), i = tile % (D / 32);
       {  // token row order: see the file's head (16 tt + 4 x + c -> 16 (x / 2) + 8 tt + 4 (x % 2) + c)
-        const int tt = i / (D / 64), kb = i % (D / 64), x = l16 / 4;
-        const int row = 16 * (x / 2) + 8 * tt + 4 * (x % 2) + l16 % 4;
+        const int tt = i / (D / 64), kb = i % (D / 64), quad = l16 / 4;
+        const int row = 16 * (quad / 2) + 8 * tt + 4 * (quad % 2) + l16 % 4;
         uint8_t* p = buf + ((gr * (D / 16) + kb * 4 + g16) * kWave + row) * 16;
-        *reinterpret_cast<half8*>(p) = dequant8(kr[c].x, kr[c].y);
-        *reinterpret_cast<half8*>(p + 32 * 16) = dequant8(kr[c].z, kr[c].w);
+        *reinterpret_cast<half8*>(p) = dequant8(x.k[c].x, x.k[c].y);
+        *reinterpret_cast<half8*>(p + 32 * 16) = dequant8(x.k[c].z, x.k[c].w);
       }
       {
         uint8_t* p = buf + kBuf / 2 +
                      (((gr * (D / 32) + i) * 2 + g16 / 2) * kWave + (g16 % 2) * 32 + l16) * 16;
-        *reinterpret_cast<half8*>(p) = dequant8(vr[c].x, vr[c].y);
-        *reinterpret_cast<half8*>(p + 16 * 16) = dequant8(vr[c].z, vr[c].w);
+        *reinterpret_cast<half8*>(p) = dequant8(x.v[c].x, x.v[c].y);
+        *reinterpret_cast<half8*>(p + 16 * 16) = dequant8(x.v[c].z, x.v[c].w);
       }
     }
   };
@@ -909,25 +1033,31 @@ __attribute__((amdgpu_waves_per_eu(RT == 1 ? 2 : 1))) void kv8_prefill_kernel(At
   };
 
   if (begin < end) {
+    // (past the end the last group is loaded again, and not used)
+    Ahead x0, x1;
     look(begin);
-    load();
+    load(x0);
     look(begin + NG);
-    stage(lds);
+    load(x1);
+    look(begin + 2 * NG);
+    stage(lds, x0);
     __syncthreads();
-    int at = 0;
-    for (int g = begin; g < end; g += NG) {
+    const auto turn = [&](Ahead& now, Ahead& next, const uint8_t* in, uint8_t* out, int g) {
       uint32_t ks[NG], vs[NG];
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
-        ks[n] = ks_next[n];
-        vs[n] = vs_next[n];
+        ks[n] = now.ks[n];
+        vs[n] = now.vs[n];
       }
-      load();  // (past the end: the last group again, not used)
-      look(g + 2 * NG);
-      step(lds + at * kBuf, g, ks, vs);
-      stage(lds + (1 - at) * kBuf);
+      load(now);
+      look(g + 3 * NG);
+      step(in, g, ks, vs);
+      stage(out, next);
       __syncthreads();
-      at = 1 - at;
+    };
+    for (int g = begin; g < end; g += 2 * NG) {
+      turn(x0, x1, lds, lds + kBuf, g);
+      if (g + NG < end) turn(x1, x0, lds + kBuf, lds, g + NG);
     }
   }
 
@@ -1007,7 +1137,7 @@ __global__ __launch_bounds__(kThreads) void kv8_merge_kernel(AttnArgs a) {
 
 template <typename T, int D>
 hipError_t launch_sized(const AttnArgs& a, const Kv8AttnPlan& p, hipStream_t stream) {
-  const unsigned grid = (unsigned)(p.tiles * a.hk * a.splits);
+  const unsigned grid = (unsigned)p.grid;
   constexpr size_t kLds = D == 64 ? kWaves * 32 * 68 * 4
                                   : 2 * (D <= 128 ? 2 : 1) * 32 * D * 2 * 2 + (D > 128 ? 128 * D * 2 : 0);
   if (p.kernel == 1) kv8_prefill_kernel<T, D, 1><<<grid, kThreads, kLds, stream>>>(a);
@@ -1022,38 +1152,142 @@ hipError_t launch_sized(const AttnArgs& a, const Kv8AttnPlan& p, hipStream_t str
 
 }  // namespace
 
+// The launch: which kernel, and in how many splits each tile's tokens (batches
+// of unequal lengths cut them into equal shares, below).  Both
+// kernels' times follow from the number of workgroups W and the turns each makes
+// (decode: four 32-token groups, one per wavefront; prefill: one step), with the
+// constants below fitted to 18 shapes at 1, 2, 4, 8 and 16 splits on either
+// kernel.  Small batches of a few hundred rows run on the decode kernel (4 x 50
+// queries, 32 + 8 heads, 1018 tokens: 13.9 us unsplit, the prefill kernel 25.6
+// at its best split), prompts that fill the chip on the prefill kernel (7999
+// tokens: 1.1 ms, the decode kernel's rate would be half).
+namespace {
+
+// Splits of a tile that join()'s LDS holds.
+int most_splits(int rows) { return rows == 32 ? 48 : 64; }
+// Requests up to which every workgroup adds up their lengths: eight round trips.
+constexpr int64_t kShareRequests = 512;
+
+struct Estimate {
+  double us;
+  int splits;
+  bool merge;
+};
+
+Estimate estimate(bool prefill, int rows, double tiles, double groups, double tokens_heads, bool ragged,
+                  double shared, int most_rows, int D, int hk, int cus) {
+  // us of a turn at `per_cu` workgroups on each CU; slots: workgroups per CU
+  const double base = prefill ? (D == 64 ? 1.1 : D == 128 ? 1.5 : 1.35)
+                              : D == 256 ? 1.1 : (rows == 16 ? 0.55 : 0.85) * (D == 64 ? 0.75 : 1.0);
+  const double more = prefill ? (D == 256 ? 0.6 : 0.4) : D == 256 ? 1.2 : (rows == 16 ? 0.25 : 0.58) * (D == 64 ? 0.6 : 1.0);
+  const int per_turn = prefill ? (D == 256 ? 1 : 2) : kWaves;
+  const double slots = cus * (prefill || D == 256 || rows > 16 ? 2.0 : 3.0);
+  const int held = rows < most_rows ? rows : most_rows;
+  const int cap = most_splits(rows);
+  Estimate best{1e30, 1, false};
+  for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+    if (s > cap || (s > 1 && s > groups)) break;
+    const double turns = ceil(ceil(groups / s) / per_turn), w = tiles * hk * s;
+    const auto round = [&](double n) {  // n workgroups at a time
+      // the cache's bytes of a turn, at 6.5 TB/s, where they come from memory
+      const double bytes = n * per_turn * 64.0 * D * shared / 6.5e6;
+      const double turn = base + more * (n / cus);
+      return 2.5 + turns * (turn > bytes ? turn : bytes);
+    };
+    const double full = floor(w / slots), rest = w - full * slots;
+    double us = 3.0 + (prefill ? 1.0 : 0.0) + full * round(slots) + (rest >= 1 ? round(rest) : 0.0);
+    if (ragged) us += 0.1 * round(w < slots ? w : slots);  // the longest request runs on
+    bool merge = false;
+    if (s > 1) {
+      const double units = held * (D / 4), ways = units < kThreads ? kThreads / units : 1.0;
+      const double join = 2.0 + 1.2 * ceil(units / kThreads) * ceil(s / (8.0 * ways));
+      const double second = 5.0 + tokens_heads * s * D * 8.0 / 3e6;
+      merge = prefill || second < join || tiles * hk > kMaxSplitCounters;
+      us += merge ? second : join;
+    }
+    if (us < best.us) best = {us, s, merge};
+  }
+  return best;
+}
+
+}  // namespace
+
 Kv8AttnPlan plan_kv8_attention(const rf_kv8_attention_args& a, int cus) {
   Kv8AttnPlan p;
   const int64_t group = a.q.heads / a.cache.kv_heads, hk = a.cache.kv_heads;
-  int64_t most_q = a.cu_q ? a.max_q_len : ceil_div(a.tokens, a.requests);
+  const int D = a.cache.head_dim;
+  int64_t most_q = a.cu_q ? a.max_q_len : a.tokens / a.requests;
   if (most_q < 1 || most_q > a.tokens) most_q = a.tokens;
   const int64_t most_rows = most_q * group;
-  p.kernel = most_rows > 64 ? 1 : 0;
-  // (two tiles of 16 rows of size 256 would not fit the registers)
-  p.rows = p.kernel ? 128 : most_rows <= 16 || a.cache.head_dim > 128 ? 16 : 32;
-  p.tiles = a.cu_q ? a.tokens * group / p.rows + a.requests + 1
-                   : a.requests * ceil_div(most_rows, p.rows);
   int64_t most_kv = a.width * a.cache.block_size;
   if (a.max_kv_len > 0 && a.max_kv_len < most_kv) most_kv = a.max_kv_len;
   if (a.window > 0 && a.window + most_q < most_kv) most_kv = a.window + most_q;
-  // Useful tiles, each cut along its tokens until the launch has about `want`
-  // workgroups (more where requests may differ in length, so that the longest
-  // does not run on alone), in pieces of at least `least` groups.
-  const int64_t tiles = p.kernel ? ceil_div(a.tokens * group, p.rows) : a.requests * ceil_div(most_rows, p.rows);
-  const int64_t busy = tiles * hk, groups = ceil_div(most_kv, RF_KV8_GROUP);
-  const int64_t want = 2 * cus * (a.requests > 1 && !p.kernel ? 3 : 1);
-  const int64_t cap = p.rows == 16 ? 64 : p.rows == 32 ? 32 : 16;  // what join()'s LDS holds
-  int64_t s = busy > 0 ? want / busy : 1;
-  p.least = 4;
-  if (s > groups / p.least) s = groups / p.least;
-  s = s < 1 ? 1 : s > cap ? cap : s;
-  const int64_t rows = most_rows < p.rows ? most_rows : p.rows;
-  p.merge = s > 1 && (p.kernel == 1 || p.tiles * hk > kMaxSplitCounters || rows * s * a.cache.head_dim > (1 << 15));
-  p.splits = (int)s;
-  p.workspace = s == 1 ? 0 : (size_t)(a.tokens * a.q.heads * s) * (a.cache.head_dim + 2) * 4;
-  if (p.workspace > 0x7fffffff) {  // (partials are addressed by 31 bits)
+  const bool ragged = a.cu_q && a.requests > 1;
+  // tiles that have work, and the upper bound that the grid covers
+  const auto useful = [&](int rows) {
+    const int64_t each = a.requests * ceil_div(most_rows, rows), all = a.tokens * group / rows + a.requests;
+    return each < all ? each : all;
+  };
+  const auto bound = [&](int rows) {
+    return a.cu_q ? a.tokens * group / rows + a.requests + 1 : a.requests * ceil_div(most_rows, rows);
+  };
+  const auto groups = [&](int rows) {  // seen by a tile, on average
+    const double first = a.causal ? (most_q > rows / group ? most_q - rows / (double)group : 0.0) / 2 : 0.0;
+    const double n = most_kv - first;
+    return (n < 1 ? 1 : n) / RF_KV8_GROUP + 0.5;
+  };
+  const double tokens_heads = (double)a.tokens * a.q.heads;
+  // (two tiles of 16 rows of size 256 would not fit the registers)
+  const int few = most_rows <= 16 || D > 128 ? 16 : 32;
+  const int most = (int)(most_rows < 1024 ? most_rows : 1024);
+  Estimate e = estimate(false, few, (double)useful(few), groups(few), tokens_heads, ragged,
+                        1.0 / ceil_div(most_rows, few), most, D, (int)hk, cus);
+  p.kernel = 0;
+  p.rows = few;
+  if (most_rows > 16) {
+    const Estimate e1 = estimate(true, 128, (double)useful(128), groups(128), tokens_heads, ragged,
+                                 1.0 / ceil_div(most_rows, 128), most, D, (int)hk, cus);
+    if (e1.us < e.us) {
+      e = e1;
+      p.kernel = 1;
+      p.rows = 128;
+    }
+  }
+  p.tiles = bound(p.rows);
+  p.least = p.kernel ? (D == 256 ? 1 : 2) : kWaves;
+  p.splits = e.splits;
+  p.merge = e.merge;
+  p.grid = p.tiles * hk * p.splits;
+  // Partial results are addressed by 31 bits; joined tiles take a counter each.
+  const auto fits = [&](int64_t rows, int64_t grid) {
+    p.partials = rows;
+    p.workspace = (size_t)rows * (D + 2) * 4;
+    return p.workspace <= 0x7fffffff && (p.merge || grid <= kMaxSplitCounters);
+  };
+  // (the sums of tiles times groups fit, whatever the offsets say)
+  if (p.kernel == 0 && !p.merge && a.requests > 1 && a.requests < kShareRequests &&
+      (double)p.tiles * (double)a.requests * (double)(a.width * a.cache.block_size / RF_KV8_GROUP + 1) < 2147483647.0) {
+    // Workgroups: the multiple of the CUs that leaves tiles half a share each to
+    // cut (16 requests of 4 to 20 thousand tokens, 32 + 8 heads, 1, 1.25, 2 and 3
+    // workgroups a CU: 64.8, 74.8, 63.5, 65.4 us; 48 of up to 9000, 64 + 8 heads:
+    // 2, 2.5, 3 and 4: 95.9, 87.8, 83.5, 88.9).  Shares are long enough for the
+    // join they cost (32 requests of up to 500 tokens: 8.0 us, in shares of 8
+    // groups 11.5; 4 x 50 queries after 968 tokens, 32 rows: 14.0 and 20.9).
+    int64_t shares = ceil_div(3 * useful(p.rows) * hk, 2 * cus) * cus / hk;
+    if (shares < p.tiles) shares = p.tiles;
+    if (fits(shares * hk * p.rows, shares * hk)) {
+      p.shares = (int)shares;
+      p.splits = most_splits(p.rows);
+      p.least = p.rows == 32 ? 32 : D == 256 ? 8 : 16;
+      p.grid = shares * hk;
+      return p;
+    }
+  }
+  if (p.splits == 1 || !fits(p.merge ? a.tokens * a.q.heads * p.splits : p.grid * p.rows, p.grid)) {
     p.splits = 1;
     p.merge = false;
+    p.grid = p.tiles * hk;
+    p.partials = 0;
     p.workspace = 0;
   }
   return p;
@@ -1078,10 +1312,10 @@ hipError_t launch_kv8_attention(const rf_kv8_attention_args& in, const Kv8AttnPl
   a.counters = nullptr;
   a.stat = nullptr;
   a.part = nullptr;
-  if (p.splits > 1) {
+  if (p.workspace > 0) {
     a.counters = (uint32_t*)in.scratch->counters;
     a.part = (float*)in.scratch->partials;
-    a.stat = (uint64_t*)(a.part + in.tokens * in.q.heads * p.splits * D);
+    a.stat = (uint64_t*)(a.part + p.partials * D);
   }
   a.table_stride = in.table_stride;
   a.num_blocks = (int)in.cache.num_blocks;
@@ -1096,6 +1330,7 @@ hipError_t launch_kv8_attention(const rf_kv8_attention_args& in, const Kv8AttnPl
   a.splits = p.splits;
   a.least = p.least;
   a.merge = p.merge;
+  a.shares = p.shares;
   a.tiles = (int)p.tiles;
   a.causal = in.causal;
   a.window = in.window > (1 << 30) ? 1 << 30 : (int)in.window;

@@ -169,7 +169,7 @@ int rf_kv8_attention(const rf_kv8_attention_args* a, void* stream) {
     if (!w || !w->counters || !w->partials || w->partial_bytes < p.workspace) return RF_W8A16_EWORKSPACE;
     if (!aligned(w->counters, 4) || !aligned(w->partials, 16)) return RF_W8A16_EALIGN;
   }
-  if (p.tiles * a->cache.kv_heads * p.splits > 0x7fffffff) return RF_W8A16_EINVAL;
+  if (p.grid > 0x7fffffff) return RF_W8A16_EINVAL;
   return status_of(launch_kv8_attention(*a, p, static_cast<hipStream_t>(stream)));
 }
 

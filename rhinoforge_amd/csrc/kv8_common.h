@@ -53,10 +53,13 @@ struct Kv8AttnPlan {
   int kernel;     // 0: tokens split over the wavefronts (few rows), 1: rows split over them
   int rows;       // rows of a tile
   int64_t tiles;  // upper bound of tiles per key/value head
-  int splits;
+  int splits;     // of a tile: all of them, or at most where `shares` is set
   int least;      // 32-token groups of a split, at least
   bool merge;     // a second kernel adds the splits
-  size_t workspace;  // bytes of partial results
+  int shares = 0; // of all tiles of a key/value head together, for batches of unequal lengths
+  int64_t grid;   // workgroups
+  int64_t partials;  // rows of partial results
+  size_t workspace;  // their bytes
 };
 Kv8AttnPlan plan_kv8_attention(const rf_kv8_attention_args& a, int cus);
 hipError_t launch_kv8_attention(const rf_kv8_attention_args& a, const Kv8AttnPlan& p,

@@ -621,3 +621,60 @@ def test_refusals_on_the_device():
         rf.kv8_plan(table, lens.cpu(), lens, lens, lens, 1, 32)
     with pytest.raises(RuntimeError, match="int32"):
         rf.kv8_attention(q, cache, table.long(), lens)
+
+
+# ---- attention of many requests of unequal lengths -------------------------------
+
+@pytest.mark.parametrize("b", [2, 48, 63, 64, 65, 130, 511, 700, 2500])
+@pytest.mark.parametrize("new", [1, 3, 20])
+@pytest.mark.parametrize("hints", [False, True])
+def test_attention_of_many_requests(b, new, hints):
+    """Most requests short or empty, a few long: shares of all sizes, and every
+    way of finding them (up to 64 requests at once, several a lane, searched for)."""
+    _say("many", b, new, hints)
+    d, bs, hq, hk = (64, 32, 4, 2) if b != 130 else (256, 64, 8, 1)
+    r = np.random.default_rng(b * 7 + new)
+    lens = r.integers(0, 60, b)
+    long = r.integers(0, b, 2)
+    lens[long] = r.integers(1500, 3001, 2)
+    lens = [int(x) for x in lens]
+    news = [new] * b if new == 1 else [int(x) for x in r.integers(0, new + 1, b)]
+    opt = {"window": 777} if new == 3 else {}
+    table, cu, nb, spare = _batch(lens, news, bs, b + new)
+    kq, ks, vq, vs = _filled(nb, hk, bs, d, b)
+    for i in spare:
+        ks[i], vs[i] = float("nan"), float("nan")
+    cache = rf.KV8Cache.from_quantized(*(t.to(DEV) for t in (kq, ks, vq, vs)))
+    q = torch.randn(int(cu[-1]), hq, d, generator=_rng(b)).half()
+    args = (q.to(DEV), cache, torch.from_numpy(table).to(DEV),
+            torch.tensor(lens, dtype=torch.int32, device=DEV))
+    args += () if new == 1 else (torch.from_numpy(cu).to(DEV),)
+    kw = {**opt, **({"max_kv_len": max(lens)} if hints else {}),
+          **({"max_q_len": max(news)} if hints and new > 1 else {})}
+    out, lse = rf.kv8_attention(*args, return_lse=True, **kw)
+    for _ in range(3):
+        assert torch.equal(rf.kv8_attention(*args, **kw), out)
+    _check_attention(q, (kq.numpy(), ks.numpy(), vq.numpy(), vs.numpy()), table, lens, cu, out, lse,
+                     torch.float16, scale=d ** -0.5, **opt)
+
+
+def test_attention_offsets_out_of_order_leave_the_next_call_right():
+    """Offsets that go back ask for more tiles than the batch has: what such a call
+    returns is not said, but it ends, and the calls after it are right."""
+    d, bs, hq, hk, b = 64, 32, 4, 2, 40
+    lens, news = [2000] * b, [9] * b
+    table, cu, nb, _ = _batch(lens, news, bs, 3)
+    kq, ks, vq, vs = _filled(nb, hk, bs, d, 3)
+    cache = rf.KV8Cache.from_quantized(*(t.to(DEV) for t in (kq, ks, vq, vs)))
+    q = torch.randn(int(cu[-1]), hq, d, generator=_rng(3)).half()
+    args = (q.to(DEV), cache, torch.from_numpy(table).to(DEV),
+            torch.tensor(lens, dtype=torch.int32, device=DEV))
+    good = torch.from_numpy(cu).to(DEV)
+    want = rf.kv8_attention(*args, good, max_q_len=9)
+    bad = good.clone()
+    bad[1:b:2] = 360
+    for hint in (9, 0):
+        rf.kv8_attention(*args, bad, max_q_len=hint)
+        assert torch.equal(rf.kv8_attention(*args, good, max_q_len=9), want)
+    _check_attention(q, (kq.numpy(), ks.numpy(), vq.numpy(), vs.numpy()), table, lens, cu, want, None,
+                     torch.float16, scale=d ** -0.5)
