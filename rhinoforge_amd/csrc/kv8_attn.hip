@@ -787,19 +787,25 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_decode_kernel(AttnArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// Many rows (prompts): four wavefronts of 32 * RT rows each.  A step's K and V
-// bytes are loaded once per workgroup, turned into fp16 on their way into LDS,
-// in operand order (a wavefront reads 1 KB in lane order per MFMA), and the
-// next step's are loaded meanwhile.
+// Many rows (prompts): four wavefronts of 32 rows each.  A step's K and V bytes
+// are loaded once per workgroup, turned into fp16 on their way into LDS, in
+// operand order (a wavefront reads 1 KB in lane order per MFMA), and those of
+// the next two steps are loaded meanwhile.  7999 tokens, 64 + 8 heads of 128:
+// 1149 us, 913 TFLOP/s, where a library product of 16384^3 reaches 1300.
+// Vector units 62% and matrix units 43% busy at 1.9 of 2.4 GHz: the clock gives
+// way to the power they draw.  Variants with other orders of the same
+// instructions (products and weights interleaved one by one, operands read
+// ahead, loads one step ahead instead of two) differ by up to 6% in cycles and
+// by 1% in time.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ floatx16 mfma32x32x16(half8 a, half8 b, floatx16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
-template <typename T, int D, int RT>
+template <typename T, int D>
 __global__ __launch_bounds__(kWaves* kWave)
-__attribute__((amdgpu_waves_per_eu(RT == 1 ? 2 : 1))) void kv8_prefill_kernel(AttnArgs a) {
-  constexpr int R = 32 * RT * kWaves;
+__attribute__((amdgpu_waves_per_eu(2))) void kv8_prefill_kernel(AttnArgs a) {
+  constexpr int R = 32 * kWaves;
   constexpr int NG = D <= 128 ? 2 : 1;          // 32-token groups of a step
   constexpr int kBuf = NG * 32 * D * 2 * 2;     // bytes of a step's K and V in fp16
   constexpr int kChunks = NG * D / 128;         // 16-byte chunks of K (and of V) per thread
@@ -830,29 +836,27 @@ __attribute__((amdgpu_waves_per_eu(RT == 1 ? 2 : 1))) void kv8_prefill_kernel(At
 
   // Size 256: the sums take 128 registers, so the queries stay in LDS, where
   // each lane reads its own.
-  half8 q[RT][kQLds ? 1 : D / 16];
-  half8* q_lds = reinterpret_cast<half8*>(lds + 2 * kBuf) + wave * (RT * D / 16) * kWave + lane;
-  const auto put_q = [&](int r, int i, half8 v) {
-    if constexpr (kQLds) q_lds[(r * (D / 16) + i) * kWave] = v;
-    else q[r][i] = v;
+  half8 q[kQLds ? 1 : D / 16];
+  half8* q_lds = reinterpret_cast<half8*>(lds + 2 * kBuf) + wave * (D / 16) * kWave + lane;
+  const auto put_q = [&](int i, half8 v) {
+    if constexpr (kQLds) q_lds[i * kWave] = v;
+    else q[i] = v;
   };
-  const auto get_q = [&](int r, int i) {
-    if constexpr (kQLds) return q_lds[(r * (D / 16) + i) * kWave];
-    else return q[r][i];
+  const auto get_q = [&](int i) {
+    if constexpr (kQLds) return q_lds[i * kWave];
+    else return q[i];
   };
-  float factor[RT];
-  int lo[RT], hi[RT];
-  const int wrow = wave * 32 * RT;  // this wavefront's first row of the tile
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    const int row = t.row0 + min(wrow + 32 * r + col, rows - 1);
+  float factor = a.scale_log2e;
+  int lo, hi;
+  const int wrow = wave * 32;  // this wavefront's first row of the tile
+  {
+    const int row = t.row0 + min(wrow + col, rows - 1);
     const int qi = (int)((unsigned)row / (unsigned)a.group);
     const uint8_t* p = a.q + (int64_t)(t.first_token + qi) * a.q_ts +
                        (int64_t)(h * a.group + (row - qi * a.group)) * a.q_hs + lh * 16;
     uint4 raw[D / 16];
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) raw[i] = load_u4(p + i * 32);
-    factor[r] = a.scale_log2e;
     if constexpr (!__is_same(T, _Float16)) {
       float m = 0.0f;
 #pragma unroll
@@ -862,30 +866,27 @@ __attribute__((amdgpu_waves_per_eu(RT == 1 ? 2 : 1))) void kv8_prefill_kernel(At
       const float f1 = pow2(-e1), f2 = pow2(-e2);
 #pragma unroll
       for (int i = 0; i < D / 16; ++i)
-        put_q(r, i, __builtin_convertvector(Eight<T>::load(&raw[i]) * f1 * f2, half8));
-      factor[r] = a.scale_log2e * pow2(e1) * pow2(e2);
+        put_q(i, __builtin_convertvector(Eight<T>::load(&raw[i]) * f1 * f2, half8));
+      factor = a.scale_log2e * pow2(e1) * pow2(e2);
     } else {
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) put_q(r, i, as_half8(raw[i]));
+      for (int i = 0; i < D / 16; ++i) put_q(i, as_half8(raw[i]));
     }
-    seen(a, t, row, &lo[r], &hi[r]);
+    seen(a, t, row, &lo, &hi);
+    hi = min(hi, end * 32);
   }
   const bool idle = wrow >= rows;
   int my_lo_min, my_lo_max, my_hi_min, my_hi_max;
   seen(a, t, t.row0 + min(wrow, rows - 1), &my_lo_min, &my_hi_min);
-  seen(a, t, t.row0 + min(wrow + 32 * RT, rows) - 1, &my_lo_max, &my_hi_max);
+  seen(a, t, t.row0 + min(wrow + 32, rows) - 1, &my_lo_max, &my_hi_max);
   my_lo_min = uniform(my_lo_min), my_lo_max = uniform(my_lo_max);
-  my_hi_min = uniform(my_hi_min), my_hi_max = uniform(my_hi_max);
+  my_hi_min = min(uniform(my_hi_min), end * 32), my_hi_max = min(uniform(my_hi_max), end * 32);
 
-  floatx16 acc[RT][D / 32];
-  Running run[RT];
+  floatx16 acc[D / 32];
+  Running run = {-__builtin_inff(), 0.0f};
   Top top;
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    run[r] = {-__builtin_inff(), 0.0f};
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) acc[r][i] = 0.0f;
-  }
+  for (int i = 0; i < D / 32; ++i) acc[i] = 0.0f;
 
   // Chunk c of this wavefront is 1 KB tile c * kWaves + wave of the step.  A
   // step's bytes and scales are loaded two steps ahead (a short share is bound
@@ -934,106 +935,124 @@ __attribute__((amdgpu_waves_per_eu(RT == 1 ? 2 : 1))) void kv8_prefill_kernel(At
       }
     }
   };
-  const auto step = [&](const uint8_t* buf, int g, const uint32_t (&kss)[NG], const uint32_t (&vss)[NG]) {
+  // One step of a wavefront: all of its scores, one look at their maximum, then
+  // the weights.  The products of a group with V are issued among the weights of
+  // the next group, the last ones among the conversion of the next step's bytes:
+  // those take the vector units, these the matrix units.
+  const auto step = [&](const uint8_t* buf, int g, const uint32_t (&kss)[NG], const uint32_t (&vss)[NG],
+                        uint8_t* out, const Ahead& next) {
+    const int t0 = opaque(g << 5);
+    if (idle || t0 >= my_hi_max || t0 + 32 * NG <= my_lo_min) {
+      stage(out, next);
+      return;
+    }
+    floatx16 s[NG];
+#pragma unroll
+    for (int n = 0; n < NG; ++n) s[n] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+      for (int n = 0; n < NG; ++n) {
+        const half8 k = *reinterpret_cast<const half8*>(buf + ((n * (D / 16) + i) * kWave + lane) * 16);
+        s[n] = mfma32x32x16(k, get_q(i), s[n]);
+      }
+    uint32_t ks[NG], vs[NG], vmax = 0;
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
-      const int t0 = opaque((g + n) << 5);
-      if (g + n >= end || idle || t0 >= my_hi_max || t0 + 32 <= my_lo_min) continue;
-      uint32_t ks = kss[n], vs = vss[n];
-      floatx16 s[RT];
-#pragma unroll
-      for (int r = 0; r < RT; ++r) s[r] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        const half8 k = *reinterpret_cast<const half8*>(buf + ((n * (D / 16) + i) * kWave + lane) * 16);
-#pragma unroll
-        for (int r = 0; r < RT; ++r) s[r] = mfma32x32x16(k, get_q(r, i), s[r]);
-      }
-      if (not_finite(ks, vs)) {
+      ks[n] = kss[n];
+      vs[n] = vss[n];
+      if (not_finite(ks[n], vs[n])) {
         keep_branch();
-        ks = kOneBits;
-        vs = 0;
-#pragma unroll
-        for (int r = 0; r < RT; ++r) s[r] = __builtin_nanf("");
+        ks[n] = kOneBits;
+        vs[n] = 0;
+        s[n] = __builtin_nanf("");
       }
-      const bool edge = t0 < my_lo_max || t0 + 32 > my_hi_min;
-      bool raise = vs > top.bits;
-      float c[RT];
+      vmax = vs[n] > vmax ? vs[n] : vmax;
+    }
+    if (t0 < my_lo_max || t0 + 32 * NG > my_hi_min) {
+      keep_branch();
+      const int first = lo - t0 - 4 * lh, past = hi - t0 - 4 * lh;
 #pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        const int first = lo[r] - t0 - 4 * lh, past = hi[r] - t0 - 4 * lh;
-        c[r] = ks == 0 ? 1.0f : as_float(ks) * factor[r];  // (a block of zeros: every score is 0)
-        if (edge) {
-          keep_branch();
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int tok = 16 * (i / 4 % 2) + 8 * (i / 8) + i % 4;  // past t0 + 4 lh
-            s[r][i] = (tok < first) | (tok >= past) ? -__builtin_inff() : s[r][i];
-          }
-        }
-        float mx = -__builtin_inff();
-#pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[r][i]);
-        raise |= mx * c[r] > run[r].m + (run[r].m == -__builtin_inff() ? 0.0f : kRaise);
-      }
-      if (__ballot(raise)) {
-        float fv = 1.0f;
-        if (vs > top.bits) {
-          const float log = log2_fast(as_float(vs));
-          fv = exp2_fast(top.log - log);
-          top.bits = vs;
-          top.log = log;
-        }
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          float mx = -__builtin_inff();
-#pragma unroll
-          for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[r][i]);
-          mx = fmaxf(run[r].m, mx * c[r]);
-          mx = fmaxf(mx, __shfl_xor(mx, 32));
-          const float f = exp2_fast(run[r].m - safe(mx));
-          run[r].m = mx;
-          run[r].l *= f;
-          const float fa = f * fv;
-#pragma unroll
-          for (int i = 0; i < D / 32; ++i) acc[r][i] *= fa;
-        }
-      }
-      // (a branch the compiler cannot fold: in one block with the merge above it
-      // would keep the sums twice, 241 registers instead of 189, and spill at 256)
-      float lr = 0.0f;
-      if (vs != top.bits) {
-        lr = ratio_log2(vs, top);
-        asm volatile("" : "+v"(lr));
-      }
-      const float back = exp2_fast(-lr);
-      half8 p[RT][2];
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        const float off = kShift + lr - safe(run[r].m);
-        float sum = 0.0f;
+      for (int n = 0; n < NG; ++n)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          float e = exp2_fast(__builtin_fmaf(s[r][i], c[r], off));
-          sum += e;
-          p[r][i / 8][i % 8] = (_Float16)e;
+          const int tok = 32 * n + 16 * (i / 4 % 2) + 8 * (i / 8) + i % 4;  // past t0 + 4 lh
+          s[n][i] = (tok < first) | (tok >= past) ? -__builtin_inff() : s[n][i];
         }
-        run[r].l += sum * back;
+    }
+    float c[NG], mx = -__builtin_inff();
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      c[n] = ks[n] == 0 ? 1.0f : as_float(ks[n]) * factor;  // (a block of zeros: every score is 0)
+      float most = -__builtin_inff();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) most = fmaxf(most, s[n][i]);
+      mx = fmaxf(mx, most * c[n]);
+    }
+    const bool raise = vmax > top.bits || mx > run.m + (run.m == -__builtin_inff() ? 0.0f : kRaise);
+    if (__ballot(raise)) {
+      float fv = 1.0f;
+      if (vmax > top.bits) {
+        const float log = log2_fast(as_float(vmax));
+        fv = exp2_fast(top.log - log);
+        top.bits = vmax;
+        top.log = log;
       }
+      mx = fmaxf(run.m, mx);
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      const float f = exp2_fast(run.m - safe(mx));
+      run.m = mx;
+      run.l *= f;
+      const float fa = f * fv;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) acc[i] *= fa;
+    }
+    // (a branch the compiler cannot fold: in one block with the merge above it
+    // would keep the sums twice, 241 registers instead of 189, and spill at 256)
+    float lr[NG];
+#pragma unroll
+    for (int n = 0; n < NG; ++n) lr[n] = 0.0f;
+    if (NG == 1 ? vs[0] != top.bits : vs[0] != top.bits || vs[NG - 1] != top.bits) {
+#pragma unroll
+      for (int n = 0; n < NG; ++n) {
+        lr[n] = ratio_log2(vs[n], top);
+        asm volatile("" : "+v"(lr[n]));
+      }
+    }
+    half8 p[2];
+    const auto weights = [&](int n) {
+      const float off = kShift + lr[n] - safe(run.m);
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float e = exp2_fast(__builtin_fmaf(s[n][i], c[n], off));
+        sum += e;
+        p[i / 8][i % 8] = (_Float16)e;
+      }
+      run.l += sum * exp2_fast(-lr[n]);
+    };
+    const auto add = [&](int n, const half8 (&p)[2]) {
 #pragma unroll
       for (int i = 0; i < D / 32; ++i)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const half8 v = *reinterpret_cast<const half8*>(
               buf + kBuf / 2 + (((n * (D / 32) + i) * 2 + u) * kWave + lane) * 16);
-#pragma unroll
-          for (int r = 0; r < RT; ++r) acc[r][i] = mfma32x32x16(v, p[r][u], acc[r][i]);
+          acc[i] = mfma32x32x16(v, p[u], acc[i]);
         }
+    };
+    weights(0);
+    if constexpr (NG == 2) {
+      const half8 p0[2] = {p[0], p[1]};
+      add(0, p0);
+      weights(1);
     }
+    add(NG - 1, p);
+    stage(out, next);
   };
 
   if (begin < end) {
-    // (past the end the last group is loaded again, and not used)
+    // (past the end the last group is loaded again, and masked)
     Ahead x0, x1;
     look(begin);
     load(x0);
@@ -1051,8 +1070,7 @@ __attribute__((amdgpu_waves_per_eu(RT == 1 ? 2 : 1))) void kv8_prefill_kernel(At
       }
       load(now);
       look(g + 3 * NG);
-      step(in, g, ks, vs);
-      stage(out, next);
+      step(in, g, ks, vs, out, next);
       __syncthreads();
     };
     for (int g = begin; g < end; g += 2 * NG) {
@@ -1066,46 +1084,43 @@ __attribute__((amdgpu_waves_per_eu(RT == 1 ? 2 : 1))) void kv8_prefill_kernel(At
   // would store four values of another row.
   constexpr int kPitch = 64 + 4;
   float* mine = reinterpret_cast<float*>(lds) + wave * 32 * kPitch;
+  float l = run.l;
+  l += __shfl_xor(l, 32);
+  const int left = rows - wrow;  // rows of this wavefront's tile
+  const float f = partial ? as_float(top.bits) : l == 0.0f ? 0.0f : as_float(top.bits) / l;
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    float l = run[r].l;
-    l += __shfl_xor(l, 32);
-    const int left = rows - wrow - 32 * r;  // rows of this wavefront's tile
-    const float f = partial ? as_float(top.bits) : l == 0.0f ? 0.0f : as_float(top.bits) / l;
+  for (int i = 0; i < D / 32; i += 2) {
 #pragma unroll
-    for (int i = 0; i < D / 32; i += 2) {
+    for (int j = 0; j < 8; ++j) {
+      floatx4 o;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        floatx4 o;
+      for (int c = 0; c < 4; ++c) o[c] = acc[i + j / 4][4 * (j % 4) + c] * f;
+      *reinterpret_cast<floatx4*>(mine + col * kPitch + 8 * j + 4 * lh) = o;
+    }
+    const int d = lane % 8 * 8;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) o[c] = acc[r][i + j / 4][4 * (j % 4) + c] * f;
-        *reinterpret_cast<floatx4*>(mine + col * kPitch + 8 * j + 4 * lh) = o;
-      }
-      const int d = lane % 8 * 8;
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const int rr = 8 * n + lane / 8;
-        if (rr >= left) continue;
-        const float* src = mine + rr * kPitch + d;
-        const floatx4 x = *reinterpret_cast<const floatx4*>(src);
-        const floatx4 y = *reinterpret_cast<const floatx4*>(src + 4);
-        const int64_t to = out_row(a, t, h, wrow + 32 * r + rr);
-        if (partial) {
-          float* part = a.part + (to * a.splits + split) * D + 32 * i + d;
-          *reinterpret_cast<floatx4*>(part) = x;
-          *reinterpret_cast<floatx4*>(part + 4) = y;
-        } else {
-          Eight<T>::store(a.out + (to * D + 32 * i + d) * 2,
-                          __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-        }
+    for (int n = 0; n < 4; ++n) {
+      const int rr = 8 * n + lane / 8;
+      if (rr >= left) continue;
+      const float* src = mine + rr * kPitch + d;
+      const floatx4 x = *reinterpret_cast<const floatx4*>(src);
+      const floatx4 y = *reinterpret_cast<const floatx4*>(src + 4);
+      const int64_t to = out_row(a, t, h, wrow + rr);
+      if (partial) {
+        float* part = a.part + (to * a.splits + split) * D + 32 * i + d;
+        *reinterpret_cast<floatx4*>(part) = x;
+        *reinterpret_cast<floatx4*>(part + 4) = y;
+      } else {
+        Eight<T>::store(a.out + (to * D + 32 * i + d) * 2,
+                        __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
       }
     }
-    if (lh == 0 && col < left) {
-      const int64_t to = out_row(a, t, h, wrow + 32 * r + col);
-      if (partial) Partials(a).store_stat((int)to * a.splits + split, run[r].m, l);
-      else if (a.lse)
-        a.lse[to] = l == 0.0f ? -__builtin_inff() : (run[r].m - kShift + log2_fast(l)) * kLn2;
-    }
+  }
+  if (lh == 0 && col < left) {
+    const int64_t to = out_row(a, t, h, wrow + col);
+    if (partial) Partials(a).store_stat((int)to * a.splits + split, run.m, l);
+    else if (a.lse)
+      a.lse[to] = l == 0.0f ? -__builtin_inff() : (run.m - kShift + log2_fast(l)) * kLn2;
   }
 }
 
@@ -1140,7 +1155,7 @@ hipError_t launch_sized(const AttnArgs& a, const Kv8AttnPlan& p, hipStream_t str
   const unsigned grid = (unsigned)p.grid;
   constexpr size_t kLds = D == 64 ? kWaves * 32 * 68 * 4
                                   : 2 * (D <= 128 ? 2 : 1) * 32 * D * 2 * 2 + (D > 128 ? 128 * D * 2 : 0);
-  if (p.kernel == 1) kv8_prefill_kernel<T, D, 1><<<grid, kThreads, kLds, stream>>>(a);
+  if (p.kernel == 1) kv8_prefill_kernel<T, D><<<grid, kThreads, kLds, stream>>>(a);
   else if (p.rows == 16) kv8_decode_kernel<T, D, 1><<<grid, kThreads, 0, stream>>>(a);
   else if constexpr (D <= 128) kv8_decode_kernel<T, D, 2><<<grid, kThreads, 0, stream>>>(a);
   const hipError_t e = hipGetLastError();
