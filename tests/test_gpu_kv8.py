@@ -678,3 +678,55 @@ def test_attention_offsets_out_of_order_leave_the_next_call_right():
         assert torch.equal(rf.kv8_attention(*args, good, max_q_len=9), want)
     _check_attention(q, (kq.numpy(), ks.numpy(), vq.numpy(), vs.numpy()), table, lens, cu, want, None,
                      torch.float16, scale=d ** -0.5)
+
+
+@pytest.mark.parametrize("run", [1, 2, 7, 8, 9, 16])
+@pytest.mark.parametrize("tokens", [15, 16, 17, 63, 65, 640, 2100])
+@pytest.mark.parametrize("d,hk,bs", [(64, 12, 32), (128, 8, 64), (256, 1, 128)])
+def test_append_of_many_short_runs(run, tokens, d, hk, bs):
+    """Runs of `run` tokens, each in its own block behind `seen` held ones, some
+    skipped: together, cut by chunk ends, at the ends of blocks."""
+    _say("runs", run, tokens, d, bs)
+    dt = torch.float16
+    r = np.random.default_rng(run * 1000 + tokens)
+    count = -(-tokens // run)
+    kq, ks, vq, vs = _filled(count, hk, bs, d, tokens + run)
+    cache = rf.KV8Cache.from_quantized(*(t.to(DEV) for t in (kq, ks, vq, vs)))
+    seen = r.choice([0, 1, 5, bs - run], count)
+    blocks = r.permutation(count)
+    slots = [int(b) * bs + int(s) + j for b, s in zip(blocks, seen) for j in range(run)][:tokens]
+    for i in range(count):
+        if r.random() < 0.1:
+            slots[i * run:(i + 1) * run] = [int(r.choice([-1, count * bs, 2 ** 31 - 200]))] * len(slots[i * run:(i + 1) * run])
+    k, v = (torch.randn(tokens, hk, d, generator=_rng(s)).to(dt) * 2.0 ** -(s % 3) for s in (tokens, run + 5))
+    rf.kv8_append(cache, k.to(DEV), v.to(DEV), torch.tensor(slots, dtype=torch.int32, device=DEV))
+    gk, gks, gv, gvs = cache.to_quantized()
+    for name, x, q0, s0, got, gscale in (("k", k, kq, ks, gk, gks), ("v", v, vq, vs, gv, gvs)):
+        q, scale, quot = o.append(q0.numpy(), s0.numpy(), _np(x), slots)
+        assert np.abs(_np(gscale) / scale - 1).max() <= 2.0 ** -22, name
+        diff = _np(got) - q
+        tie = np.abs(np.abs(quot - np.floor(quot)) - 0.5) < 2.0 ** -15
+        assert ((diff == 0) | (tie & (np.abs(diff) == 1))).all(), name
+
+
+@pytest.mark.parametrize("d,hk,bs", [(64, 3, 32), (128, 2, 64), (256, 1, 128)])
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16, torch.float32])
+def test_read_of_whole_groups_and_of_others(d, hk, bs, dt):
+    """32 slots in a row are read together where they are a group of a block."""
+    nb = 9
+    kq, ks, vq, vs = _filled(nb, hk, bs, d, d)
+    cache = rf.KV8Cache.from_quantized(*(t.to(DEV) for t in (kq, ks, vq, vs)))
+    r = np.random.default_rng(d)
+    group = lambda g: list(range(32 * g, 32 * g + 32))  # noqa: E731
+    last = nb * bs // 32 - 1
+    slots = group(last) + group(0) + group(3)[1:] + [5] + group(2)[::-1] + list(range(40, 72))
+    slots += [nb * bs + i for i in range(32)] + [-1] * 32 + [int(x) for x in r.integers(0, nb * bs, 32)]
+    slots += group(4)[:31] + [-1] + group(1)
+    for n in (len(slots), len(slots) - 1, 33, 32, 31):
+        rk, rv = rf.kv8_read(cache, torch.tensor(slots[:n], dtype=torch.int32, device=DEV), dt)
+        for got, q, s in ((rk, kq, ks), (rv, vq, vs)):
+            want = torch.zeros(n, hk, d)
+            for i, sl in enumerate(slots[:n]):
+                if 0 <= sl < nb * bs:
+                    want[i] = q[sl // bs, :, sl % bs].float() * s[sl // bs][:, None]
+            assert torch.equal(got.cpu(), want.to(dt))
