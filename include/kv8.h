@@ -16,6 +16,8 @@
  *   k_scale,
  *   v_scale     : fp32 [num_blocks][kv_heads]
  *   A stored byte u stands for (u - 128) * scale, |u - 128| <= 127.
+ *   Scales are +0 or positive; attention gives NaN where a query sees tokens of a
+ *   block whose scale is negative, infinite or NaN.
  *   slot = block * block_size + token within the block.
  *
  * Byte order inside one head's block (RF_KV8_TILE): groups of 32 tokens, each

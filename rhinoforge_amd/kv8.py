@@ -48,6 +48,8 @@ class KV8Cache:
     ``[num_blocks, kv_heads, block_size / 32, head_dim / 32, 1024]``, see
     include/kv8.h); :meth:`to_quantized` and :meth:`from_quantized` convert to
     and from row-major int8 ``[num_blocks, kv_heads, block_size, head_dim]``.
+    Scales are zero or positive; :func:`kv8_attention` gives NaN to queries that
+    see tokens of a block whose scale is negative, infinite or NaN.
     """
 
     def __init__(self, num_blocks: int, kv_heads: int, head_dim: int, block_size: int = 64, *,
