@@ -794,9 +794,14 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_decode_kernel(AttnArgs a) {
 // Many rows (prompts): four wavefronts of 32 rows each.  A step's K and V bytes
 // are loaded once per workgroup, turned into fp16 on their way into LDS, in
 // operand order (a wavefront reads 1 KB in lane order per MFMA), and those of
-// the next two steps are loaded meanwhile.  7999 tokens, 64 + 8 heads of 128:
+// the next two steps are loaded meanwhile.  G = 2: two gangs of four wavefronts
+// take the steps of the same rows in turn, and their sums join at the end: what
+// the longest tile takes is halved, which is what a prompt takes that does not
+// fill the chip several times (2500 tokens, 16 + 8 heads: 69 us with one gang, 50
+// with two; 1000 tokens, 32 + 8: 32 and 26; but 7999, 64 + 8: 1127 and 1224).
+// 7999 tokens, 64 + 8 heads of 128:
 // 1149 us, 913 TFLOP/s, where a library product of 16384^3 reaches 1300.
-// Vector units 62% and matrix units 43% busy at 1.9 of 2.4 GHz: the clock gives
+// Vector units 64% and matrix units 45% busy at 1.9 of 2.4 GHz: the clock gives
 // way to the power they draw.  Variants with other orders of the same
 // instructions (products and weights interleaved one by one, operands read
 // ahead, loads one step ahead instead of two) differ by up to 6% in cycles and
@@ -806,8 +811,8 @@ __device__ __forceinline__ floatx16 mfma32x32x16(half8 a, half8 b, floatx16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
-template <typename T, int D>
-__global__ __launch_bounds__(kWaves* kWave)
+template <typename T, int D, int G>
+__global__ __launch_bounds__(G* kWaves* kWave)
 __attribute__((amdgpu_waves_per_eu(2))) void kv8_prefill_kernel(AttnArgs a) {
   constexpr int R = 32 * kWaves;
   constexpr int NG = D <= 128 ? 2 : 1;          // 32-token groups of a step
@@ -817,7 +822,9 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_prefill_kernel(AttnArgs a) {
   // (sized at the launch: with the size known here the register allocator
   // trades registers for it, and spills)
   extern __shared__ __align__(16) uint8_t lds[];
-  const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int tid = threadIdx.x, lane = tid % kWave, any_wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int wave = any_wave % kWaves, gang = any_wave / kWaves;
+  uint8_t* const bufs = lds + gang * 2 * kBuf;
   const int col = lane % 32, lh = lane / 32;
   const unsigned id = blockIdx.x, pair = id / (unsigned)a.hk;
   const int h = (int)(id - pair * a.hk), turn = (int)(pair / (unsigned)a.splits);
@@ -841,7 +848,7 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_prefill_kernel(AttnArgs a) {
   // Size 256: the sums take 128 registers, so the queries stay in LDS, where
   // each lane reads its own.
   half8 q[kQLds ? 1 : D / 16];
-  half8* q_lds = reinterpret_cast<half8*>(lds + 2 * kBuf) + wave * (D / 16) * kWave + lane;
+  half8* q_lds = reinterpret_cast<half8*>(lds + G * 2 * kBuf) + wave * (D / 16) * kWave + lane;
   const auto put_q = [&](int i, half8 v) {
     if constexpr (kQLds) q_lds[i * kWave] = v;
     else q[i] = v;
@@ -1057,13 +1064,16 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_prefill_kernel(AttnArgs a) {
 
   if (begin < end) {
     // (past the end the last group is loaded again, and masked)
+    constexpr int kStride = G * NG;
+    const int turns = (end - begin + kStride - 1) / kStride;
+    int g = begin + gang * NG;
     Ahead x0, x1;
-    look(begin);
+    look(g);
     load(x0);
-    look(begin + NG);
+    look(g + kStride);
     load(x1);
-    look(begin + 2 * NG);
-    stage(lds, x0);
+    look(g + 2 * kStride);
+    stage(bufs, x0);
     __syncthreads();
     const auto turn = [&](Ahead& now, Ahead& next, const uint8_t* in, uint8_t* out, int g) {
       uint32_t ks[NG], vs[NG];
@@ -1073,14 +1083,38 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_prefill_kernel(AttnArgs a) {
         vs[n] = now.vs[n];
       }
       load(now);
-      look(g + 3 * NG);
+      look(g + 3 * kStride);
       step(in, g, ks, vs, out, next);
       __syncthreads();
     };
-    for (int g = begin; g < end; g += 2 * NG) {
-      turn(x0, x1, lds, lds + kBuf, g);
-      if (g + NG < end) turn(x1, x0, lds + kBuf, lds, g + NG);
+    for (int i = 0; i < turns; i += 2, g += 2 * kStride) {
+      turn(x0, x1, bufs, bufs + kBuf, g);
+      if (i + 1 < turns) turn(x1, x0, bufs + kBuf, bufs, g + kStride);
     }
+  }
+
+  if constexpr (G == 2) {  // the second gang's sums join the first's, lane by lane
+    float* sums = reinterpret_cast<float*>(lds) + wave * (D / 2) * kWave + lane;
+    float* stats = reinterpret_cast<float*>(lds) + kWaves * (D / 2) * kWave + wave * 2 * kWave + lane;
+    if (gang == 1) {
+#pragma unroll
+      for (int i = 0; i < D / 2; ++i) sums[i * kWave] = acc[i / 16][i % 16] * as_float(top.bits);
+      stats[0] = run.m;
+      stats[kWave] = run.l;
+    }
+    __syncthreads();
+    if (gang == 0) {
+      const float om = stats[0], m = fmaxf(run.m, om);
+      const float f = exp2_fast(run.m - safe(m)), of = exp2_fast(om - safe(m));
+      const float fa = f * as_float(top.bits);
+#pragma unroll
+      for (int i = 0; i < D / 2; ++i) acc[i / 16][i % 16] = acc[i / 16][i % 16] * fa + sums[i * kWave] * of;
+      run.m = m;
+      run.l = run.l * f + stats[kWave] * of;
+      top.bits = kOneBits;
+    }
+    __syncthreads();  // the rows go out through the same memory
+    if (gang == 1) return;
   }
 
   // Rows go out through LDS (each wavefront its own part, free after the last
@@ -1161,9 +1195,13 @@ hipError_t launch_sized(const AttnArgs& a, const Kv8AttnPlan& p, hipStream_t str
   const unsigned grid = (unsigned)p.grid;
   constexpr size_t kLds = D == 64 ? kWaves * 32 * 68 * 4
                                   : 2 * (D <= 128 ? 2 : 1) * 32 * D * 2 * 2 + (D > 128 ? 128 * D * 2 : 0);
-  if (p.kernel == 1) kv8_prefill_kernel<T, D><<<grid, kThreads, kLds, stream>>>(a);
-  else if (p.rows == 16) kv8_decode_kernel<T, D, 1><<<grid, kThreads, 0, stream>>>(a);
-  else if constexpr (D <= 128) kv8_decode_kernel<T, D, 2><<<grid, kThreads, 0, stream>>>(a);
+  constexpr size_t kLds2 = 4 * 2 * 32 * D * 2 * 2;
+  if (p.kernel == 1 && p.gangs == 1) kv8_prefill_kernel<T, D, 1><<<grid, kThreads, kLds, stream>>>(a);
+  else if (p.kernel == 0 && p.rows == 16) kv8_decode_kernel<T, D, 1><<<grid, kThreads, 0, stream>>>(a);
+  else if constexpr (D <= 128) {
+    if (p.kernel == 1) kv8_prefill_kernel<T, D, 2><<<grid, 2 * kThreads, kLds2, stream>>>(a);
+    else kv8_decode_kernel<T, D, 2><<<grid, kThreads, 0, stream>>>(a);
+  }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || !a.merge) return e;
   kv8_merge_kernel<T, D>
@@ -1174,14 +1212,14 @@ hipError_t launch_sized(const AttnArgs& a, const Kv8AttnPlan& p, hipStream_t str
 }  // namespace
 
 // The launch: which kernel, and in how many splits each tile's tokens (batches
-// of unequal lengths cut them into equal shares, below).  Both
-// kernels' times follow from the number of workgroups W and the turns each makes
-// (decode: four 32-token groups, one per wavefront; prefill: one step), with the
+// of unequal lengths cut them into equal shares, below).  The kernels' times
+// follow from the number of workgroups and the turns each makes (decode: four
+// 32-token groups, one per wavefront; prefill: one step of each gang), with the
 // constants below fitted to 18 shapes at 1, 2, 4, 8 and 16 splits on either
-// kernel.  Small batches of a few hundred rows run on the decode kernel (4 x 50
-// queries, 32 + 8 heads, 1018 tokens: 13.9 us unsplit, the prefill kernel 25.6
-// at its best split), prompts that fill the chip on the prefill kernel (7999
-// tokens: 1.1 ms, the decode kernel's rate would be half).
+// kernel and to 19 prompts on one and two gangs.  Small batches of a few hundred
+// rows run on the decode kernel (4 x 50 queries, 32 + 8 heads, 1018 tokens: 14.3
+// us unsplit, the prefill kernel 19.1 at its best), prompts that fill the chip on
+// the prefill kernel (7999 tokens, 64 + 8 heads: 1.13 ms, the decode kernel 1.57).
 namespace {
 
 // Splits of a tile that join()'s LDS holds.
@@ -1195,14 +1233,14 @@ struct Estimate {
   bool merge;
 };
 
-Estimate estimate(bool prefill, int rows, double tiles, double groups, double tokens_heads, bool ragged,
+Estimate estimate(bool prefill, int gangs, int rows, double tiles, double groups, double longest, double tokens_heads, bool ragged,
                   double shared, int most_rows, int D, int hk, int cus) {
   // us of a turn at `per_cu` workgroups on each CU; slots: workgroups per CU
   const double base = prefill ? (D == 64 ? 1.1 : D == 128 ? 1.5 : 1.35)
                               : D == 256 ? 1.1 : (rows == 16 ? 0.55 : 0.85) * (D == 64 ? 0.75 : 1.0);
   const double more = prefill ? (D == 256 ? 0.6 : 0.4) : D == 256 ? 1.2 : (rows == 16 ? 0.25 : 0.58) * (D == 64 ? 0.6 : 1.0);
-  const int per_turn = prefill ? (D == 256 ? 1 : 2) : kWaves;
-  const double slots = cus * (prefill || D == 256 || rows > 16 ? 2.0 : 3.0);
+  const int per_turn = prefill ? (D == 256 ? 1 : 2 * gangs) : kWaves;
+  const double slots = cus * (gangs == 2 ? 1.0 : prefill || D == 256 || rows > 16 ? 2.0 : 3.0);
   const int held = rows < most_rows ? rows : most_rows;
   const int cap = most_splits(rows);
   Estimate best{1e30, 1, false};
@@ -1212,17 +1250,20 @@ Estimate estimate(bool prefill, int rows, double tiles, double groups, double to
     const auto round = [&](double n) {  // n workgroups at a time
       // the cache's bytes of a turn, at 6.5 TB/s, where they come from memory
       const double bytes = n * per_turn * 64.0 * D * shared / 6.5e6;
-      const double turn = base + more * (n / cus);
+      const double turn = base + more * (gangs * n / cus);
       return 2.5 + turns * (turn > bytes ? turn : bytes);
     };
     const double full = floor(w / slots), rest = w - full * slots;
-    double us = 3.0 + (prefill ? 1.0 : 0.0) + full * round(slots) + (rest >= 1 ? round(rest) : 0.0);
+    double us = full * round(slots) + (rest >= 1 ? round(rest) : 0.0);
+    // the last tile of a prompt sees the most, beside shorter ones
+    const double alone = 2.5 + ceil(ceil(longest / s) / per_turn) * (base + more * (gangs == 2 ? 1.75 : prefill ? 0.3 : 0.2));
+    us = 3.0 + (prefill ? 2 * gangs - 1 : 0) + (us > alone ? us : alone);
     if (ragged) us += 0.1 * round(w < slots ? w : slots);  // the longest request runs on
     bool merge = false;
     if (s > 1) {
       const double units = held * (D / 4), ways = units < kThreads ? kThreads / units : 1.0;
       const double join = 2.0 + 1.2 * ceil(units / kThreads) * ceil(s / (8.0 * ways));
-      const double second = 5.0 + tokens_heads * s * D * 8.0 / 3e6;
+      const double second = 4.5 + tokens_heads * s * D * 8.0 / 3e6;
       merge = prefill || second < join || tiles * hk > kMaxSplitCounters;
       us += merge ? second : join;
     }
@@ -1257,20 +1298,22 @@ Kv8AttnPlan plan_kv8_attention(const rf_kv8_attention_args& a, int cus) {
     const double n = most_kv - first;
     return (n < 1 ? 1 : n) / RF_KV8_GROUP + 0.5;
   };
-  const double tokens_heads = (double)a.tokens * a.q.heads;
+  const double tokens_heads = (double)a.tokens * a.q.heads, longest = most_kv / (double)RF_KV8_GROUP + 0.5;
   // (two tiles of 16 rows of size 256 would not fit the registers)
   const int few = most_rows <= 16 || D > 128 ? 16 : 32;
   const int most = (int)(most_rows < 1024 ? most_rows : 1024);
-  Estimate e = estimate(false, few, (double)useful(few), groups(few), tokens_heads, ragged,
+  Estimate e = estimate(false, 1, few, (double)useful(few), groups(few), longest, tokens_heads, ragged,
                         1.0 / ceil_div(most_rows, few), most, D, (int)hk, cus);
   p.kernel = 0;
   p.rows = few;
   if (most_rows > 16) {
-    const Estimate e1 = estimate(true, 128, (double)useful(128), groups(128), tokens_heads, ragged,
-                                 1.0 / ceil_div(most_rows, 128), most, D, (int)hk, cus);
-    if (e1.us < e.us) {
+    for (int gangs = 1; gangs <= (D == 256 ? 1 : 2); ++gangs) {
+      const Estimate e1 = estimate(true, gangs, 128, (double)useful(128), groups(128), longest, tokens_heads, ragged,
+                                   1.0 / ceil_div(most_rows, 128), most, D, (int)hk, cus);
+      if (e1.us >= e.us) continue;
       e = e1;
       p.kernel = 1;
+      p.gangs = gangs;
       p.rows = 128;
     }
   }

@@ -51,6 +51,7 @@ hipError_t launch_kv8_read(const rf_kv8_cache& c, const int32_t* slots, int64_t 
 // one tile, workgroups over the tokens of one tile, partial results.
 struct Kv8AttnPlan {
   int kernel;     // 0: tokens split over the wavefronts (few rows), 1: rows split over them
+  int gangs = 1;  // kernel 1: groups of four wavefronts that take a tile's tokens in turn
   int rows;       // rows of a tile
   int64_t tiles;  // upper bound of tiles per key/value head
   int splits;     // of a tile: all of them, or at most where `shares` is set

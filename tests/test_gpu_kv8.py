@@ -730,3 +730,51 @@ def test_read_of_whole_groups_and_of_others(d, hk, bs, dt):
                 if 0 <= sl < nb * bs:
                     want[i] = q[sl // bs, :, sl % bs].float() * s[sl // bs][:, None]
             assert torch.equal(got.cpu(), want.to(dt))
+
+
+# ---- prompts that fill the chip, or nearly: one gang of wavefronts a tile, or two,
+# ---- with and without splits
+
+PROMPTS = [
+    ([499], [499], 64, 4, 128, torch.float16, {}),
+    ([501], [501], 64, 4, 128, torch.bfloat16, {"causal": False}),
+    ([1799], [500], 64, 4, 128, torch.bfloat16, {"window": 300}),
+    ([1490, 203], [200, 100], 64, 4, 128, torch.float16, {}),
+    ([2497, 40, 170], [180, 30, 90], 64, 4, 128, torch.float16, {}),
+    ([2010], [400], 64, 8, 64, torch.bfloat16, {}),
+    ([6001], [250], 64, 8, 64, torch.float16, {}),
+    ([3170], [500], 32, 8, 128, torch.bfloat16, {}),
+    ([600], [600], 64, 2, 64, torch.float16, {}),
+    ([3000], [300], 64, 2, 64, torch.float16, {"window": 2000}),
+    ([300, 64, 0], [300, 0, 200], 64, 4, 128, torch.float16, {}),   # rows that see nothing
+]
+
+
+@pytest.mark.parametrize("case", range(len(PROMPTS)))
+def test_attention_of_prompts(case):
+    lens, news, hq, hk, d, dt, opt = PROMPTS[case]
+    _say("prompt", PROMPTS[case])
+    bs = 64
+    table, cu, nb, spare = _batch(lens, news, bs, case)
+    kq, ks, vq, vs = _filled(nb, hk, bs, d, 70 + case)
+    vs = vs * 2.0 ** torch.randint(-6, 3, vs.shape, generator=_rng(case))
+    for b in spare:
+        ks[b], vs[b] = float("nan"), float("nan")
+    cache = rf.KV8Cache.from_quantized(*(t.to(DEV) for t in (kq, ks, vq, vs)))
+    q = (torch.randn(int(cu[-1]), hq, d, generator=_rng(case)) * 2).to(dt)
+    args = (q.to(DEV), cache, torch.from_numpy(table).to(DEV),
+            torch.tensor(lens, dtype=torch.int32, device=DEV), torch.from_numpy(cu).to(DEV))
+    out, lse = rf.kv8_attention(*args, max_q_len=max(news), max_kv_len=max(lens), return_lse=True, **opt)
+    assert torch.equal(rf.kv8_attention(*args, max_q_len=max(news), max_kv_len=max(lens), **opt), out)
+    _check_attention(q, (kq.numpy(), ks.numpy(), vq.numpy(), vs.numpy()), table, lens, cu, out, lse, dt,
+                     scale=d ** -0.5, **opt)
+    # a block that is not finite reaches the queries that see it, and no others
+    if lens[0] > 320 and opt.get("causal", True) and not opt:
+        bad = ks.clone()
+        bad[int(table[0, (lens[0] - 1) // bs]), 0] = float("inf")
+        cache.k_scale.copy_(bad)
+        nan = torch.isnan(rf.kv8_attention(*args, max_q_len=max(news), max_kv_len=max(lens))).cpu()
+        first = (lens[0] - 1) // bs * bs - (lens[0] - news[0])   # the first query that sees it
+        want = torch.zeros_like(nan)
+        want[max(first, 0):news[0], :hq // hk] = True
+        assert torch.equal(nan, want)
