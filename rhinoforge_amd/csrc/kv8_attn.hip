@@ -1339,7 +1339,9 @@ Kv8AttnPlan plan_kv8_attention(const rf_kv8_attention_args& a, int cus) {
     // groups 11.5; 4 x 50 queries after 968 tokens, 32 rows: 14.0 and 20.9).
     int64_t shares = ceil_div(3 * useful(p.rows) * hk, 2 * cus) * cus / hk;
     if (shares < p.tiles) shares = p.tiles;
-    if (fits(shares * hk * p.rows, shares * hk)) {
+    // (16 workgroups a CU even out by themselves, and their partial results stay
+    // below 70 MB)
+    if (shares * hk <= 16 * cus && fits(shares * hk * p.rows, shares * hk)) {
       p.shares = (int)shares;
       p.splits = most_splits(p.rows);
       p.least = p.rows == 32 ? 32 : D == 256 ? 8 : 16;

@@ -747,6 +747,13 @@ PROMPTS = [
     ([600], [600], 64, 2, 64, torch.float16, {}),
     ([3000], [300], 64, 2, 64, torch.float16, {"window": 2000}),
     ([300, 64, 0], [300, 0, 200], 64, 4, 128, torch.float16, {}),   # rows that see nothing
+    # fewer rows, many splits: joined by the last workgroup or added by a second kernel
+    ([5000], [5], 16, 8, 128, torch.float16, {}),
+    ([1000], [20], 16, 8, 128, torch.bfloat16, {}),
+    ([5000], [60], 16, 8, 128, torch.float16, {}),
+    ([5003], [9], 8, 1, 256, torch.float16, {}),
+    ([3000], [40], 8, 1, 256, torch.bfloat16, {}),
+    ([700], [700], 8, 1, 256, torch.float16, {}),
 ]
 
 
