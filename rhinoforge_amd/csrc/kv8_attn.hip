@@ -797,10 +797,11 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_decode_kernel(AttnArgs a) {
 // the next two steps are loaded meanwhile.  G = 2: two gangs of four wavefronts
 // take the steps of the same rows in turn, and their sums join at the end: what
 // the longest tile takes is halved, which is what a prompt takes that does not
-// fill the chip several times (2500 tokens, 16 + 8 heads: 69 us with one gang, 50
+// fill the chip several times (2500 tokens, 16 + 8 heads: 69 us with one gang, 49
 // with two; 1000 tokens, 32 + 8: 32 and 26; but 7999, 64 + 8: 1127 and 1224).
 // 7999 tokens, 64 + 8 heads of 128:
-// 1149 us, 913 TFLOP/s, where a library product of 16384^3 reaches 1300.
+// 1102 to 1174 us on different cards, 952 to 893 TFLOP/s, where a library product
+// of 16384^3 reaches 1300.
 // Vector units 64% and matrix units 45% busy at 1.9 of 2.4 GHz: the clock gives
 // way to the power they draw.  Variants with other orders of the same
 // instructions (products and weights interleaved one by one, operands read
@@ -949,7 +950,10 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_prefill_kernel(AttnArgs a) {
   // One step of a wavefront: all of its scores, one look at their maximum, then
   // the weights.  The products of a group with V are issued among the weights of
   // the next group, the last ones among the conversion of the next step's bytes:
-  // those take the vector units, these the matrix units.
+  // those take the vector units, these the matrix units.  A wavefront's priority
+  // rises through the step, so that of two that share a SIMD the one ahead stays
+  // ahead and they are in different phases (five prompts with a window 151.9 ->
+  // 143.6 us, 2500 tokens 50.4 -> 48.6; on another card 155.0 -> 148.6).
   const auto step = [&](const uint8_t* buf, int g, const uint32_t (&kss)[NG], const uint32_t (&vss)[NG],
                         uint8_t* out, const Ahead& next) {
     const int t0 = opaque(g << 5);
@@ -960,6 +964,7 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_prefill_kernel(AttnArgs a) {
     floatx16 s[NG];
 #pragma unroll
     for (int n = 0; n < NG; ++n) s[n] = 0.0f;
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int i = 0; i < D / 16; ++i)
 #pragma unroll
@@ -967,6 +972,7 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_prefill_kernel(AttnArgs a) {
         const half8 k = *reinterpret_cast<const half8*>(buf + ((n * (D / 16) + i) * kWave + lane) * 16);
         s[n] = mfma32x32x16(k, get_q(i), s[n]);
       }
+    __builtin_amdgcn_s_setprio(2);
     uint32_t ks[NG], vs[NG], vmax = 0;
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
@@ -1052,6 +1058,7 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_prefill_kernel(AttnArgs a) {
           acc[i] = mfma32x32x16(v, p[u], acc[i]);
         }
     };
+    __builtin_amdgcn_s_setprio(3);
     weights(0);
     if constexpr (NG == 2) {
       const half8 p0[2] = {p[0], p[1]};
@@ -1059,6 +1066,7 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_prefill_kernel(AttnArgs a) {
       weights(1);
     }
     add(NG - 1, p);
+    __builtin_amdgcn_s_setprio(0);
     stage(out, next);
   };
 
