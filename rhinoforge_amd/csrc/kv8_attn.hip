@@ -3,9 +3,11 @@
 // For query row q (one query, one head) over its seen tokens j:
 //   x_j = (q . k_j) ks scale log2(e),  p_j = 2^(x_j - m),  o = vs sum p_j v_j / sum p_j
 // with integer k_j, v_j and the scales ks, vs of the token's block.  One pass
-// over the tokens with a running m: p only has to stay in fp16's range, so m
-// follows the largest x when that is 8 or more above it, not at every step;
-// results do not depend on how m is chosen beyond rounding.
+// over the tokens with two running references for each row: m follows its
+// largest x, m + d its largest x + log2 vs.  The sum l is kept relative to m, the
+// weights w_j = 2^(x_j + log2 vs_j - m - d) and o relative to m + d.  Both only
+// have to stay in range, so they move when something is 8 or more above them, not
+// at every step.
 //
 // Both products run on the matrix cores with the cache as the A operand and the
 // queries as columns: S^T = K Q^T leaves each lane with scores of one query row
@@ -13,12 +15,15 @@
 // stand (the v tiles hold tokens in that order).  int8 -> fp16 is exact.
 //   * Queries: fp16 as they are.  bf16 times a power of two per row, which
 //     brings the row's largest magnitude to [2^14, 2^15): exact in fp16 down to
-//     2^-38 of it; the power goes into that row's score factor.
-//   * p is rounded to fp16 (11 bits, round to nearest): 2^-12 relative, as much
-//     as the output's own rounding in fp16.  2^7 p is what is rounded, so that
-//     small weights stay normal.
-//   * vs goes into p as vs / max(vs so far): 2^log2 of it joins the exponent.
-//     The sum over p divides it out again.  m, the sums and o stay in fp32.
+//     2^-31 of it, within 2^-39 of it below; the power goes into that row's score
+//     factor.
+//   * w is rounded to fp16 (11 bits, round to nearest): 2^-11 relative, as much
+//     as the output's own rounding in fp16.  2^7 w is what is rounded: the row's
+//     largest lies in [2^7, 2^15), and a weight below fp16's normal range loses at
+//     most 2^-25, 2^-32 of the largest p vs that the row sees.  What other rows
+//     see, and blocks without weight, do not count.
+//   * A sum over w of one block, times 2^-(log2 vs - d), is its part of l.
+//     m, d, the sums and o stay in fp32.
 #include <math.h>
 
 #include "kv8_common.h"
@@ -328,29 +333,53 @@ __device__ __forceinline__ float pow2(int e) {  // |e| <= 126
   return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23);
 }
 
+// Inside a branch on a uniform condition: keeps the compiler from turning it
+// into a select per value that every group would pay for.
+__device__ __forceinline__ void keep_branch() { asm volatile(""); }
+
 // Running softmax of one query row, as the lanes of its column hold it: m and
-// svm agree over them, l is each lane's own share of the sum.
+// d agree over them, l is each lane's own share of the sum.
 struct Running {
-  float m;  // log2 units; -inf: nothing seen
-  float l;
+  float m = -__builtin_inff();  // log2 units; -inf: nothing seen
+  float l = 0.0f;
+  float d = 0.0f;               // the sums of p vs v are in units of 2^(m + d)
 };
 
 __device__ __forceinline__ float safe(float m) { return m == -__builtin_inff() ? 0.0f : m; }
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// The largest value scale so far, and log2 of it.
-struct Top {
-  uint32_t bits = 0;
-  float log = -__builtin_inff();
-};
 __device__ __forceinline__ float log2_fast(float x) { return __builtin_amdgcn_logf(x); }
 
-// log2(vs / top) for the exponent, not below -60: a block of zeros (whatever
-// its p are, they add nothing) or one that adds far less than one rounding of
-// the result.
-__device__ __forceinline__ float ratio_log2(uint32_t vs, const Top& t) {
-  return fmaxf(log2_fast(as_float(vs)) - t.log, -60.0f);
+// log2 of a value scale; of 0, so low that 2^ it is 0 and differences stay finite.
+__device__ __forceinline__ float scale_log2(uint32_t vs) {
+  float log = log2_fast(as_float(vs));
+  if (vs < 0x00800000u) {  // (the instruction takes denormals as 0)
+    keep_branch();
+    log = fmaxf(log2_fast(as_float(vs) * 0x1p64f) - 64.0f, -300.0f);
+  }
+  return log;
 }
+// log2 vs relative to the row's d, for the exponent, not below -60: 2^7 w is then
+// below 2^(15 - 60), which rounds to 0 in fp16.
+__device__ __forceinline__ float ratio_log2(float log_vs, const Running& r) {
+  return fmaxf(log_vs - r.d, -60.0f);
+}
+
+// A row's references after scores of at most x, and of at most xv with log2 vs;
+// by how much l and the sums of p vs v change.
+struct Change {
+  float l, o;
+};
+__device__ __forceinline__ Change raise_to(Running& r, float x, float xv) {
+  const float m = fmaxf(r.m, x), top = fmaxf(r.m + r.d, xv);
+  const float d = m == -__builtin_inff() ? 0.0f : top - m, fall = r.m - safe(m);
+  const Change c = {exp2_fast(fall), exp2_fast(fall + (r.d - d))};
+  r.m = m;
+  r.d = d;
+  return c;
+}
+// 2^(d / 2), to be applied twice: 2^d itself may leave fp32's normal range.
+__device__ __forceinline__ float half_unit(const Running& r) { return exp2_fast(0.5f * r.d); }
 
 // A group with a scale that is not finite (or negative): its scores become NaN
 // (those of tokens that a row does not see are overwritten after that) and the
@@ -359,9 +388,6 @@ __device__ __forceinline__ bool not_finite(uint32_t ks, uint32_t vs) {
   return (ks > vs ? ks : vs) >= kInfBits;
 }
 constexpr uint32_t kOneBits = 0x3f800000u;
-// Inside a branch on a uniform condition: keeps the compiler from turning it
-// into a select per value that every group would pay for.
-__device__ __forceinline__ void keep_branch() { asm volatile(""); }
 
 // ---------------------------------------------------------------------------
 // Splits of one tile.  Each workgroup stores its rows' sums and (m, l), waits
@@ -598,13 +624,10 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_decode_kernel(AttnArgs a) {
   }
   floatx4 acc[RT][D / 16];
   Running run[RT];
-  Top top;
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    run[r] = {-__builtin_inff(), 0.0f};
+  for (int r = 0; r < RT; ++r)
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) acc[r][i] = floatx4{0, 0, 0, 0};
-  }
 
   const auto step = [&](const Bytes<D>& b, int g) {
     floatx4 s[RT][2];
@@ -633,7 +656,8 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_decode_kernel(AttnArgs a) {
     }
     const int t0 = opaque(g << 5);
     const bool edge = t0 < lo_max || t0 + 32 > hi_min;
-    bool raise = vs > top.bits;
+    const float log_vs = scale_log2(vs);
+    bool raise = false;
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       const float c = as_float(ks) * factor[r];
@@ -655,43 +679,38 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_decode_kernel(AttnArgs a) {
       for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[r][tt][i]);
-      raise |= mx > run[r].m + (run[r].m == -__builtin_inff() ? 0.0f : kRaise);
+      raise |= mx + fmaxf(log_vs - run[r].d, 0.0f) > run[r].m + (run[r].m == -__builtin_inff() ? 0.0f : kRaise);
     }
     if (__ballot(raise)) {
-      float fv = 1.0f;
-      if (vs > top.bits) {
-        const float log = log2_fast(as_float(vs));
-        fv = exp2_fast(top.log - log);
-        top.bits = vs;
-        top.log = log;
-      }
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
-        float mx = run[r].m;
+        float mx = -__builtin_inff();
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
           for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[r][tt][i]);
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float f = exp2_fast(run[r].m - safe(mx));
-        run[r].m = mx;
-        run[r].l *= f;
-        const float fa = f * fv;
+        const Change f = raise_to(run[r], mx, mx + log_vs);
+        run[r].l *= f.l;
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) acc[r][i] *= fa;
+        for (int i = 0; i < D / 16; ++i) acc[r][i] *= f.o;
       }
     }
-    float lr = 0.0f;  // (see the prefill kernel)
-    if (vs != top.bits) {
-      lr = ratio_log2(vs, top);
-      asm volatile("" : "+v"(lr));
+    float lr[RT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) lr[r] = 0.0f;
+    if (opaque(t0) >= 0) {  // (always: see the prefill kernel)
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        lr[r] = ratio_log2(log_vs, run[r]);
+        asm volatile("" : "+v"(lr[r]));
+      }
     }
-    const float back = exp2_fast(-lr);
     half8 p[RT];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-      const float off = kShift + lr - safe(run[r].m);
+      const float off = kShift + lr[r] - safe(run[r].m);
       float sum = 0.0f;
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt)
@@ -701,7 +720,7 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_decode_kernel(AttnArgs a) {
           sum += e;
           p[r][tt * 4 + i] = (_Float16)e;
         }
-      run[r].l += sum * back;
+      run[r].l += sum * exp2_fast(-lr[r]);
     }
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) {
@@ -756,10 +775,10 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_decode_kernel(AttnArgs a) {
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) m = fmaxf(m, red_m[w][rr]);
     // nothing seen by this wavefront: its sums are 0 and their factor too
-    const float f = exp2_fast(run[r].m - safe(m)) * as_float(top.bits);
+    const float half = half_unit(run[r]), f = exp2_fast(run[r].m - safe(m)) * half;
 #pragma unroll
     for (int i = 0; i < D / 16; ++i)
-      *reinterpret_cast<floatx4*>(&red[wave][col][16 * i + 4 * lg]) = acc[r][i] * f;
+      *reinterpret_cast<floatx4*>(&red[wave][col][16 * i + 4 * lg]) = acc[r][i] * half * f;
     __syncthreads();
     for (int it = tid; it < 16 * (D / 4); it += kThreads) {
       const int c = it / (D / 4), d = it % (D / 4) * 4, rc = 16 * r + c;
@@ -895,8 +914,7 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_prefill_kernel(AttnArgs a) {
   my_hi_min = min(uniform(my_hi_min), end * 32), my_hi_max = min(uniform(my_hi_max), end * 32);
 
   floatx16 acc[D / 32];
-  Running run = {-__builtin_inff(), 0.0f};
-  Top top;
+  Running run;
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) acc[i] = 0.0f;
 
@@ -973,18 +991,19 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_prefill_kernel(AttnArgs a) {
         s[n] = mfma32x32x16(k, get_q(i), s[n]);
       }
     __builtin_amdgcn_s_setprio(2);
-    uint32_t ks[NG], vs[NG], vmax = 0;
+    uint32_t ks[NG];
+    float log_vs[NG];
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
       ks[n] = kss[n];
-      vs[n] = vss[n];
-      if (not_finite(ks[n], vs[n])) {
+      uint32_t vs = vss[n];
+      if (not_finite(ks[n], vs)) {
         keep_branch();
         ks[n] = kOneBits;
-        vs[n] = 0;
+        vs = 0;
         s[n] = __builtin_nanf("");
       }
-      vmax = vs[n] > vmax ? vs[n] : vmax;
+      log_vs[n] = scale_log2(vs);
     }
     if (t0 < my_lo_max || t0 + 32 * NG > my_hi_min) {
       keep_branch();
@@ -997,42 +1016,34 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_prefill_kernel(AttnArgs a) {
           s[n][i] = (tok < first) | (tok >= past) ? -__builtin_inff() : s[n][i];
         }
     }
-    float c[NG], mx = -__builtin_inff();
+    // the largest score, with log2 vs, and as much of that as is above d
+    float c[NG], mx = -__builtin_inff(), mv = mx, over = mx;
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
       c[n] = ks[n] == 0 ? 1.0f : as_float(ks[n]) * factor;  // (a block of zeros: every score is 0)
       float most = -__builtin_inff();
 #pragma unroll
       for (int i = 0; i < 16; ++i) most = fmaxf(most, s[n][i]);
-      mx = fmaxf(mx, most * c[n]);
+      most *= c[n];
+      mx = fmaxf(mx, most);
+      mv = fmaxf(mv, most + log_vs[n]);
+      over = fmaxf(over, most + fmaxf(log_vs[n] - run.d, 0.0f));
     }
-    const bool raise = vmax > top.bits || mx > run.m + (run.m == -__builtin_inff() ? 0.0f : kRaise);
-    if (__ballot(raise)) {
-      float fv = 1.0f;
-      if (vmax > top.bits) {
-        const float log = log2_fast(as_float(vmax));
-        fv = exp2_fast(top.log - log);
-        top.bits = vmax;
-        top.log = log;
-      }
-      mx = fmaxf(run.m, mx);
-      mx = fmaxf(mx, __shfl_xor(mx, 32));
-      const float f = exp2_fast(run.m - safe(mx));
-      run.m = mx;
-      run.l *= f;
-      const float fa = f * fv;
+    if (__ballot(over > run.m + (run.m == -__builtin_inff() ? 0.0f : kRaise))) {
+      const Change f = raise_to(run, fmaxf(mx, __shfl_xor(mx, 32)), fmaxf(mv, __shfl_xor(mv, 32)));
+      run.l *= f.l;
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) acc[i] *= fa;
+      for (int i = 0; i < D / 32; ++i) acc[i] *= f.o;
     }
     // (a branch the compiler cannot fold: in one block with the merge above it
-    // would keep the sums twice, 241 registers instead of 189, and spill at 256)
+    // would keep the sums twice, 256 registers instead of 211, and spill)
     float lr[NG];
 #pragma unroll
     for (int n = 0; n < NG; ++n) lr[n] = 0.0f;
-    if (NG == 1 ? vs[0] != top.bits : vs[0] != top.bits || vs[NG - 1] != top.bits) {
+    if (opaque(t0) >= 0) {  // (always: a block of its own)
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
-        lr[n] = ratio_log2(vs[n], top);
+        lr[n] = ratio_log2(log_vs[n], run);
         asm volatile("" : "+v"(lr[n]));
       }
     }
@@ -1104,9 +1115,10 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_prefill_kernel(AttnArgs a) {
   if constexpr (G == 2) {  // the second gang's sums join the first's, lane by lane
     float* sums = reinterpret_cast<float*>(lds) + wave * (D / 2) * kWave + lane;
     float* stats = reinterpret_cast<float*>(lds) + kWaves * (D / 2) * kWave + wave * 2 * kWave + lane;
+    const float half = half_unit(run);
     if (gang == 1) {
 #pragma unroll
-      for (int i = 0; i < D / 2; ++i) sums[i * kWave] = acc[i / 16][i % 16] * as_float(top.bits);
+      for (int i = 0; i < D / 2; ++i) sums[i * kWave] = acc[i / 16][i % 16] * half * half;
       stats[0] = run.m;
       stats[kWave] = run.l;
     }
@@ -1114,12 +1126,12 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_prefill_kernel(AttnArgs a) {
     if (gang == 0) {
       const float om = stats[0], m = fmaxf(run.m, om);
       const float f = exp2_fast(run.m - safe(m)), of = exp2_fast(om - safe(m));
-      const float fa = f * as_float(top.bits);
+      const float fa = f * half;
 #pragma unroll
-      for (int i = 0; i < D / 2; ++i) acc[i / 16][i % 16] = acc[i / 16][i % 16] * fa + sums[i * kWave] * of;
+      for (int i = 0; i < D / 2; ++i) acc[i / 16][i % 16] = acc[i / 16][i % 16] * half * fa + sums[i * kWave] * of;
       run.m = m;
       run.l = run.l * f + stats[kWave] * of;
-      top.bits = kOneBits;
+      run.d = 0.0f;
     }
     __syncthreads();  // the rows go out through the same memory
     if (gang == 1) return;
@@ -1133,14 +1145,14 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_prefill_kernel(AttnArgs a) {
   float l = run.l;
   l += __shfl_xor(l, 32);
   const int left = rows - wrow;  // rows of this wavefront's tile
-  const float f = partial ? as_float(top.bits) : l == 0.0f ? 0.0f : as_float(top.bits) / l;
+  const float half = half_unit(run), f = partial ? half : l == 0.0f ? 0.0f : half / l;
 #pragma unroll
   for (int i = 0; i < D / 32; i += 2) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       floatx4 o;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) o[c] = acc[i + j / 4][4 * (j % 4) + c] * f;
+      for (int c = 0; c < 4; ++c) o[c] = acc[i + j / 4][4 * (j % 4) + c] * half * f;
       *reinterpret_cast<floatx4*>(mine + col * kPitch + 8 * j + 4 * lh) = o;
     }
     const int d = lane % 8 * 8;
