@@ -1020,7 +1020,9 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_prefill_kernel(AttnArgs a) {
     float c[NG], mx = -__builtin_inff(), mv = mx, over = mx;
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
-      c[n] = ks[n] == 0 ? 1.0f : as_float(ks[n]) * factor;  // (a block of zeros: every score is 0)
+      // (not 0, also where ks is 0 or the product underflows: masked scores are
+      // -inf here already, and -inf * 0 is NaN; any score times 2^-126 is 0 to exp2)
+      c[n] = fmaxf(as_float(ks[n]) * factor, 0x1p-126f);
       float most = -__builtin_inff();
 #pragma unroll
       for (int i = 0; i < 16; ++i) most = fmaxf(most, s[n][i]);
