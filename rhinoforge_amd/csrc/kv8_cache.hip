@@ -47,7 +47,9 @@ __device__ __forceinline__ float sum_lanes(float v) {
   return v;
 }
 
-template <typename T, int LP, bool kInterleaved>
+// kPart: some dimensions are not rotated.  (A form of its own: where all are, the
+// selects that it takes would cost a wavefront per SIMD, 27.6 -> 29.3 us.)
+template <typename T, int LP, bool kInterleaved, bool kPart>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeArgs a) {
   constexpr int kHeads = kWave / LP, kAhead = 4;
   typedef T tx4 __attribute__((ext_vector_type(4)));
@@ -140,6 +142,10 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeArgs a) {
       } else {
         xo = x * ca - y * sa;
         yo = y * cb + x * sa;
+      }
+      if (kPart && !turned) {  // (0 times an infinity or NaN of another dimension is not 0)
+        xo = x * ca;
+        yo = y * cb;
       }
       if (mine && turn * kHeads + lane / LP < left) {
         uint8_t* out = dst + (int64_t)turn * kHeads * a.D * 2;
@@ -712,8 +718,11 @@ inline int log2i(int v) { return __builtin_ctz((unsigned)v); }
 
 template <typename T, int LP>
 hipError_t rope_sized(const RopeArgs& r, bool interleaved, unsigned grid, hipStream_t stream) {
-  if (interleaved) qk_norm_rope_kernel<T, LP, true><<<grid, 256, 0, stream>>>(r);
-  else qk_norm_rope_kernel<T, LP, false><<<grid, 256, 0, stream>>>(r);
+  const bool part = r.rot < r.D;
+  if (interleaved && part) qk_norm_rope_kernel<T, LP, true, true><<<grid, 256, 0, stream>>>(r);
+  else if (interleaved) qk_norm_rope_kernel<T, LP, true, false><<<grid, 256, 0, stream>>>(r);
+  else if (part) qk_norm_rope_kernel<T, LP, false, true><<<grid, 256, 0, stream>>>(r);
+  else qk_norm_rope_kernel<T, LP, false, false><<<grid, 256, 0, stream>>>(r);
   return hipGetLastError();
 }
 
