@@ -30,8 +30,13 @@ class PagedQwen3:
         self.device = model.model.norm.weight.device
         self.caches = [rf.KV8Cache(num_blocks, self.kv_heads, self.head_dim, block_size, device=self.device)
                        for _ in model.model.layers]
-        inv_freq = model.model.rotary_emb.inv_freq.to(self.device)
-        self.cos, self.sin = rf.rope_table(inv_freq, cfg.max_position_embeddings)
+        rope = model.model.rotary_emb
+        if getattr(rope, "rope_type", "default") == "longrope":
+            raise ValueError("longrope's frequencies depend on the length of the sequence: one table cannot hold them")
+        # (YaRN and its like also scale cos and sin; 1 elsewhere)
+        factor = getattr(rope, "attention_scaling", 1.0)
+        self.cos, self.sin = (t * factor for t in rf.rope_table(rope.inv_freq.to(self.device),
+                                                               cfg.max_position_embeddings))
         self.free = torch.arange(num_blocks, dtype=torch.int32, device=self.device)
 
     def logits(self, ids, table, cached, new, free_start, max_new: int, max_kv: int = 0):
