@@ -102,7 +102,8 @@ class KV8Cache:
         t = v.clamp(min=-127).view(torch.uint8).bitwise_xor_(0x80)
         t = t.view(nb, heads, bs // 32, 2, 4, 4, d // 32, 2, 16).permute(0, 1, 2, 6, 4, 8, 7, 3, 5)
         c.v = t.reshape(nb, heads, bs // 32, d // 32, 1024).contiguous()
-        c.k_scale, c.v_scale = k_scale.clone(), v_scale.clone()
+        # (a clone alone would keep a transposed tensor's strides)
+        c.k_scale, c.v_scale = (s.clone(memory_format=torch.contiguous_format) for s in (k_scale, v_scale))
         return c
 
     def to_quantized(self):
