@@ -1305,7 +1305,7 @@ Kv8AttnPlan plan_kv8_attention(const rf_kv8_attention_args& a, int cus) {
   const int64_t most_rows = most_q * group;
   int64_t most_kv = a.width * a.cache.block_size;
   if (a.max_kv_len > 0 && a.max_kv_len < most_kv) most_kv = a.max_kv_len;
-  if (a.window > 0 && a.window + most_q < most_kv) most_kv = a.window + most_q;
+  if (a.window > 0 && a.window < most_kv - most_q) most_kv = a.window + most_q;  // (a window may be any int64)
   const bool ragged = a.cu_q && a.requests > 1;
   // tiles that have work, and the upper bound that the grid covers
   const auto useful = [&](int rows) {

@@ -71,3 +71,20 @@ def test_norm_beside_values_that_are_not_finite():
     assert torch.equal(y[0, 0].isnan(), want.isnan()) and (y[0, 0].nan_to_num() == 0).all()
     assert y[1, 1].isnan().all()
     assert y[0, 1].isfinite().all() and y[1, 0].isfinite().all() and y[2].isfinite().all()
+
+
+# ---- windows of every size -----------------------------------------------------------
+
+@pytest.mark.parametrize("window", [2 ** 31, 2 ** 40, 2 ** 63 - 1])
+def test_a_window_past_every_length_launches_as_none(window):
+    """The same launch, so the same bits, for one token behind a long context."""
+    hk, d, n = 2, 128, 20000
+    cache = rf.KV8Cache(320, hk, d, 64)
+    kv = torch.randn(n, hk, d, generator=_rng(0)).half().to(DEV)
+    cache.append(kv, kv.flip(0), torch.arange(n, dtype=torch.int32, device=DEV))
+    q = torch.randn(1, 8, d, generator=_rng(1)).half().to(DEV)
+    table = torch.arange(320, dtype=torch.int32, device=DEV)[None]
+    lens = torch.tensor([n], dtype=torch.int32, device=DEV)
+    want = rf.kv8_attention(q, cache, table, lens, return_lse=True)
+    got = rf.kv8_attention(q, cache, table, lens, window=window, return_lse=True)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
