@@ -25,7 +25,9 @@ namespace rf_torch {
 //             the stream might find anything.
 //   partials  at least kMinPartials bytes, never cleared.  A buffer that has to
 //             grow, under capture too, is retired, never freed: a HIP graph
-//             captured earlier on that stream may still reference it.
+//             captured earlier on that stream may still reference it.  The next
+//             one is at least twice as large, so that needs which vary from call
+//             to call (the attention's) hold less than four times the largest.
 constexpr int64_t kMinPartials = 16 << 20;
 
 inline bool capturing(void* stream) {
@@ -60,8 +62,16 @@ struct ScratchCache {
       }
     }
     if (!s.partials || s.partial_bytes < bytes) {
-      const int64_t sz = (std::max<int64_t>((int64_t)bytes, kMinPartials) + (1 << 20) - 1) >> 20 << 20;
-      s.partials = keep(at::empty({sz}, opts));
+      const auto megabytes = [](int64_t n) { return (n + (1 << 20) - 1) >> 20 << 20; };
+      const int64_t need = std::max<int64_t>((int64_t)bytes, kMinPartials);
+      int64_t sz = megabytes(std::max<int64_t>(need, s.partials ? 2 * (int64_t)s.partial_bytes : 0));
+      try {
+        s.partials = keep(at::empty({sz}, opts));
+      } catch (const c10::OutOfMemoryError&) {  // what the call needs may fit still
+        if (sz == megabytes(need)) throw;
+        sz = megabytes(need);
+        s.partials = keep(at::empty({sz}, opts));
+      }
       s.partial_bytes = (size_t)sz;
     }
     return s;
