@@ -167,7 +167,8 @@ int rf_kv8_read(const rf_kv8_cache* cache, const int32_t* slots, int64_t n, int3
  *   Scores, sums and softmax statistics are fp32.  A token's weight times its
  *   block's v_scale is rounded to fp16, relative to the largest such product that
  *   the row sees: to 2^-11 of itself, or 2^-32 of that largest one.
- *   tokens * heads < 2^31 and width * block_size <= 2^30.
+ *   tokens * heads < 2^31, (requests + 1) * kv_heads + tokens * heads / 16 < 2^31
+ *   and width * block_size <= 2^30.
  *   max_q_len, max_kv_len  the largest of each, as far as the caller knows (0:
  *         not known).  They choose the launch; results are right without them.
  *   scratch  for calls whose tokens are split over workgroups: counters as

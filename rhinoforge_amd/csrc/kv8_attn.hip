@@ -52,6 +52,7 @@ struct AttnArgs {
   int tokens, requests, width, hq, hk, group, shift;
   int per_request;     // cu == nullptr: queries of a request
   int splits, least, tiles;
+  unsigned first;      // workgroup that the launch begins at
   int shares;          // find_share: of all tiles together (0: not used)
   bool merge;          // partial results are added by kv8_merge_kernel, else by join()
   int causal, window;  // window 0: none
@@ -564,7 +565,7 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_decode_kernel(AttnArgs a) {
   __shared__ float red_m[kWaves][R], red_l[kWaves][R];
   const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int col = lane % 16, lg = lane / 16;
-  const unsigned id = blockIdx.x, pair = id / (unsigned)a.hk;
+  const unsigned id = a.first + blockIdx.x, pair = id / (unsigned)a.hk;
   const int h = (int)(id - pair * a.hk);
   int split, splits;
   Tile t;
@@ -846,7 +847,7 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_prefill_kernel(AttnArgs a) {
   const int wave = any_wave % kWaves, gang = any_wave / kWaves;
   uint8_t* const bufs = lds + gang * 2 * kBuf;
   const int col = lane % 32, lh = lane / 32;
-  const unsigned id = blockIdx.x, pair = id / (unsigned)a.hk;
+  const unsigned id = a.first + blockIdx.x, pair = id / (unsigned)a.hk;
   const int h = (int)(id - pair * a.hk), turn = (int)(pair / (unsigned)a.splits);
   const int split = (int)(pair - (unsigned)turn * a.splits);
   // the last tiles of a request see the most tokens: they begin first
@@ -1213,19 +1214,25 @@ __global__ __launch_bounds__(kThreads) void kv8_merge_kernel(AttnArgs a) {
 }
 
 template <typename T, int D>
-hipError_t launch_sized(const AttnArgs& a, const Kv8AttnPlan& p, hipStream_t stream) {
-  const unsigned grid = (unsigned)p.grid;
+hipError_t launch_sized(AttnArgs a, const Kv8AttnPlan& p, hipStream_t stream) {
   constexpr size_t kLds = D == 64 ? kWaves * 32 * 68 * 4
                                   : 2 * (D <= 128 ? 2 : 1) * 32 * D * 2 * 2 + (D > 128 ? 128 * D * 2 : 0);
   constexpr size_t kLds2 = 4 * 2 * 32 * D * 2 * 2;
-  if (p.kernel == 1 && p.gangs == 1) kv8_prefill_kernel<T, D, 1><<<grid, kThreads, kLds, stream>>>(a);
-  else if (p.kernel == 0 && p.rows == 16) kv8_decode_kernel<T, D, 1><<<grid, kThreads, 0, stream>>>(a);
-  else if constexpr (D <= 128) {
-    if (p.kernel == 1) kv8_prefill_kernel<T, D, 2><<<grid, 2 * kThreads, kLds2, stream>>>(a);
-    else kv8_decode_kernel<T, D, 2><<<grid, kThreads, 0, stream>>>(a);
+  // (no workgroup waits for another, so those of one tile may be in two launches)
+  const int64_t most = kMaxThreads / (p.gangs * kThreads);
+  for (int64_t i = 0; i < p.grid; i += most) {
+    a.first = (unsigned)i;
+    const unsigned grid = (unsigned)(p.grid - i < most ? p.grid - i : most);
+    if (p.kernel == 1 && p.gangs == 1) kv8_prefill_kernel<T, D, 1><<<grid, kThreads, kLds, stream>>>(a);
+    else if (p.kernel == 0 && p.rows == 16) kv8_decode_kernel<T, D, 1><<<grid, kThreads, 0, stream>>>(a);
+    else if constexpr (D <= 128) {
+      if (p.kernel == 1) kv8_prefill_kernel<T, D, 2><<<grid, 2 * kThreads, kLds2, stream>>>(a);
+      else kv8_decode_kernel<T, D, 2><<<grid, kThreads, 0, stream>>>(a);
+    }
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
   }
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || !a.merge) return e;
+  if (!a.merge) return hipSuccess;
   kv8_merge_kernel<T, D>
       <<<(unsigned)ceil_div((int64_t)a.tokens * a.hq * (D / 4), kThreads), kThreads, 0, stream>>>(a);
   return hipGetLastError();
@@ -1348,7 +1355,7 @@ Kv8AttnPlan plan_kv8_attention(const rf_kv8_attention_args& a, int cus) {
   const auto fits = [&](int64_t rows, int64_t grid) {
     p.partials = rows;
     p.workspace = (size_t)rows * (D + 2) * 4;
-    return p.workspace <= 0x7fffffff && (p.merge || grid <= kMaxSplitCounters);
+    return p.workspace <= 0x7fffffff && grid <= (p.merge ? 0x7fffffff : kMaxSplitCounters);
   };
   // (the sums of tiles times groups fit, whatever the offsets say)
   if (p.kernel == 0 && !p.merge && a.requests > 1 && a.requests < kShareRequests &&

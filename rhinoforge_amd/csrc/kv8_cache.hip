@@ -279,6 +279,7 @@ struct AppendArgs {
   int64_t tokens, num_blocks;
   int heads, shift;        // log2(block size)
   int chunk;               // long runs: consecutive tokens whose runs a workgroup begins
+  int64_t first;           // token that the launch begins at
 };
 
 constexpr float kLeastAmax = 0x1p-100f;
@@ -414,7 +415,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
   const unsigned both = 2u * (unsigned)a.heads, part = blockIdx.x / both, which = blockIdx.x - part * both;
   const int side = which >= (unsigned)a.heads, h = (int)which - (side ? a.heads : 0);
   constexpr int bs = BS;
-  const int64_t t0 = (int64_t)part * a.chunk;
+  const int64_t t0 = a.first + (int64_t)part * a.chunk;
   {  // token t0 - 1 + tid (chunk + 128 < 256)
     const int64_t at = t0 - 1 + tid;
     near_slots[tid] = at >= 0 && at < a.tokens ? a.slots[at] : -1;
@@ -735,13 +736,19 @@ hipError_t rope_typed(const RopeArgs& r, bool interleaved, unsigned grid, hipStr
 }
 
 template <typename T, int D>
-hipError_t append_sized(const AppendArgs& a, hipStream_t stream) {
-  const unsigned grid = (unsigned)(ceil_div(a.tokens, a.chunk) * a.heads * 2);
+hipError_t append_sized(AppendArgs a, hipStream_t stream) {
   const size_t lds = (size_t)(D + 16) << a.shift;
-  if (a.shift == 5) kv8_append_kernel<T, D, 32><<<grid, 256, lds, stream>>>(a);
-  else if (a.shift == 6) kv8_append_kernel<T, D, 64><<<grid, 256, lds, stream>>>(a);
-  else kv8_append_kernel<T, D, 128><<<grid, 256, lds, stream>>>(a);
-  return hipGetLastError();
+  const int64_t parts = ceil_div(a.tokens, a.chunk), most = kMaxThreads / 256 / (2 * a.heads);
+  for (int64_t i = 0; i < parts; i += most) {
+    a.first = i * a.chunk;
+    const unsigned grid = (unsigned)((parts - i < most ? parts - i : most) * 2 * a.heads);
+    if (a.shift == 5) kv8_append_kernel<T, D, 32><<<grid, 256, lds, stream>>>(a);
+    else if (a.shift == 6) kv8_append_kernel<T, D, 64><<<grid, 256, lds, stream>>>(a);
+    else kv8_append_kernel<T, D, 128><<<grid, 256, lds, stream>>>(a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 template <typename T>
@@ -752,22 +759,28 @@ hipError_t append_typed(const AppendArgs& a, int D, hipStream_t stream) {
 }
 
 template <typename T>
-hipError_t read_typed(const ReadArgs& a, int D, hipStream_t stream) {
-  const unsigned grid = (unsigned)(ceil_div(a.n, 32) * a.heads);
-  if (D == 64) kv8_read_kernel<T, 64><<<grid, 256, 0, stream>>>(a);
-  else if (D == 128) kv8_read_kernel<T, 128><<<grid, 256, 0, stream>>>(a);
-  else kv8_read_kernel<T, 256><<<grid, 256, 0, stream>>>(a);
-  return hipGetLastError();
+hipError_t read_typed(ReadArgs a, int D, hipStream_t stream) {
+  const int64_t most = kMaxThreads / 256 / a.heads * 32;  // entries of a launch
+  for (int64_t left = a.n; left > 0; left -= most) {
+    a.n = left < most ? left : most;
+    const unsigned grid = (unsigned)(ceil_div(a.n, 32) * a.heads);
+    if (D == 64) kv8_read_kernel<T, 64><<<grid, 256, 0, stream>>>(a);
+    else if (D == 128) kv8_read_kernel<T, 128><<<grid, 256, 0, stream>>>(a);
+    else kv8_read_kernel<T, 256><<<grid, 256, 0, stream>>>(a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    const int64_t bytes = a.n * a.heads * D * (int64_t)sizeof(T);
+    a.slots += a.n;
+    a.k_out += bytes;
+    a.v_out += bytes;
+  }
+  return hipSuccess;
 }
 
 }  // namespace
 
 hipError_t launch_qk_norm_rope(const rf_kv8_rope_args& a, hipStream_t stream) {
   RopeArgs r;
-  r.q = (const uint8_t*)a.q.data;
-  r.k = (const uint8_t*)a.k.data;
-  r.q_out = (uint8_t*)a.q_out;
-  r.k_out = (uint8_t*)a.k_out;
   r.q_ts = a.q.token_stride * 2;
   r.q_hs = a.q.head_stride * 2;
   r.k_ts = a.k.token_stride * 2;
@@ -777,7 +790,6 @@ hipError_t launch_qk_norm_rope(const rf_kv8_rope_args& a, hipStream_t stream) {
   r.cos = a.cos;
   r.sin = a.sin;
   r.pos = a.positions;
-  r.tokens = (int)a.tokens;
   r.table_rows = a.table_rows;
   r.pos64 = a.positions64;
   r.hq = a.q.heads;
@@ -789,15 +801,32 @@ hipError_t launch_qk_norm_rope(const rf_kv8_rope_args& a, hipStream_t stream) {
   // Few tokens: a wavefront per kHeads heads.  Many: as many heads per wavefront
   // as leave about 16 wavefronts for each CU.
   const int64_t at_once = kWave / lanes, q_turns = ceil_div(r.hq, at_once), k_turns = ceil_div(r.hk, at_once);
-  int64_t each = r.tokens * (q_turns + k_turns) / 4096;
+  int64_t each = a.tokens * (q_turns + k_turns) / 4096;
   each = each < 1 ? 1 : each > q_turns ? q_turns : each;
   r.turns = (int)each;
   r.q_parts = (int)ceil_div(q_turns, each);
   r.parts = r.q_parts + (int)ceil_div(k_turns, each);
-  const int64_t grid = ceil_div((int64_t)r.tokens * r.parts, 256 / kWave);
-  return a.dtype == RF_W8A16_DTYPE_F16
-             ? rope_typed<_Float16>(r, a.interleaved, (unsigned)grid, stream)
-             : rope_typed<__bf16>(r, a.interleaved, (unsigned)grid, stream);
+  // (a wavefront counts the wavefronts before it in 32 bits, fewer than threads)
+  const int64_t most = kMaxThreads / 256 * (256 / kWave) / r.parts;  // tokens of a launch
+  for (int64_t t = 0; t < a.tokens; t += most) {
+    r.tokens = (int)(a.tokens - t < most ? a.tokens - t : most);
+    r.q = (const uint8_t*)a.q.data + t * r.q_ts;
+    r.k = (const uint8_t*)a.k.data + t * r.k_ts;
+    r.q_out = (uint8_t*)a.q_out + t * r.hq * r.D * 2;
+    r.k_out = (uint8_t*)a.k_out + t * r.hk * r.D * 2;
+    if (a.positions) {
+      r.pos = (const uint8_t*)a.positions + t * (a.positions64 ? 8 : 4);
+    } else if (r.rot > 0) {  // token t has row t
+      r.cos = a.cos + t * (r.rot / 2);
+      r.sin = a.sin + t * (r.rot / 2);
+      r.table_rows = a.table_rows - t;
+    }
+    const unsigned grid = (unsigned)ceil_div((int64_t)r.tokens * r.parts, 256 / kWave);
+    const hipError_t e = a.dtype == RF_W8A16_DTYPE_F16 ? rope_typed<_Float16>(r, a.interleaved, grid, stream)
+                                                       : rope_typed<__bf16>(r, a.interleaved, grid, stream);
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 hipError_t launch_kv8_plan(const rf_kv8_plan_args& a, hipStream_t stream) {
@@ -810,7 +839,7 @@ hipError_t launch_kv8_plan(const rf_kv8_plan_args& a, hipStream_t stream) {
 
 hipError_t launch_kv8_append(const rf_kv8_cache& c, const rf_kv8_heads& k, const rf_kv8_heads& v,
                              int dtype, const int32_t* slots, int64_t tokens, hipStream_t stream) {
-  AppendArgs a;
+  AppendArgs a{};
   a.x[0] = (const uint8_t*)k.data;
   a.x[1] = (const uint8_t*)v.data;
   a.ts[0] = k.token_stride * 2;

@@ -138,8 +138,6 @@ int rf_kv8_read(const rf_kv8_cache* cache, const int32_t* slots, int64_t n, int3
   if ((!half_dtype(dtype) && dtype != RF_W8A16_DTYPE_F32) || n < 0 || n > kMaxSize ||
       (n > 0 && (!slots || !k_out || !v_out)))
     return RF_W8A16_EINVAL;
-  // one thread per eight values: the launch's workgroups are counted in 31 bits
-  if (n * cache->kv_heads > (int64_t)0x7fffffff * 256 / (cache->head_dim / 8)) return RF_W8A16_EINVAL;
   const size_t out = dtype == RF_W8A16_DTYPE_F32 ? 32 : 16;
   if (!aligned(slots, 4) || !aligned(k_out, out) || !aligned(v_out, out)) return RF_W8A16_EALIGN;
   if (n == 0) return RF_W8A16_OK;

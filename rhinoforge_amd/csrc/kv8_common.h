@@ -39,6 +39,10 @@ struct Eight<float> {
   }
 };
 
+// A launch holds fewer than 2^32 threads along x: with more it runs those modulo
+// 2^32, without an error.  What needs more workgroups runs in several launches.
+constexpr int64_t kMaxThreads = ((int64_t)1 << 32) - 1;
+
 // Validated arguments, as the C ABI passes them on (kv8_capi.hip).
 hipError_t launch_qk_norm_rope(const rf_kv8_rope_args& a, hipStream_t stream);
 hipError_t launch_kv8_plan(const rf_kv8_plan_args& a, hipStream_t stream);
