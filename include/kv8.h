@@ -112,7 +112,10 @@ int rf_kv8_qk_norm_rope(const rf_kv8_rope_args* args, void* stream);
  *   *free_next   *free_start + blocks needed; above num_free they ran out (the
  *                entries of blocks that were not there are -1)
  * All arrays int32.  requests <= RF_KV8_MAX_REQUESTS, tokens (the length of
- * slots and positions) >= 0. */
+ * slots and positions) >= 0.  Every workgroup reads all lengths and *free_start
+ * while others write, so slots, positions, cu, kv_lens and free_next may not
+ * overlap cached, fresh, free_blocks or free_start (RF_W8A16_EINVAL): the next
+ * call's lengths are another array, or a copy made after this call. */
 typedef struct rf_kv8_plan_args {
   int32_t* block_table;
   const int32_t* cached;

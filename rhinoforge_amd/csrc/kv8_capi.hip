@@ -57,6 +57,11 @@ int check_attention(const rf_kv8_attention_args* a) {
   return RF_W8A16_OK;
 }
 
+struct Ints {
+  const int32_t* p;
+  int64_t n;
+};
+
 int status_of(hipError_t e) { return e == hipSuccess ? RF_W8A16_OK : RF_W8A16_EHIP; }
 
 }  // namespace
@@ -105,6 +110,12 @@ int rf_kv8_plan(const rf_kv8_plan_args* a, void* stream) {
                         (const void*)a->slots, (const void*)a->positions, (const void*)a->cu,
                         (const void*)a->kv_lens, (const void*)a->free_next})
     if (!aligned(p, 4)) return RF_W8A16_EALIGN;
+  const Ints in[] = {{a->cached, a->requests}, {a->fresh, a->requests}, {a->free_blocks, a->num_free}, {a->free_start, 1}};
+  const Ints out[] = {{a->slots, a->tokens}, {a->positions, a->tokens}, {a->cu, a->requests + 1},
+                      {a->kv_lens, a->requests}, {a->free_next, 1}};
+  for (const Ints& o : out)
+    for (const Ints& i : in)
+      if (o.n > 0 && i.n > 0 && o.p < i.p + i.n && i.p < o.p + o.n) return RF_W8A16_EINVAL;
   DeviceInfo dev;
   const int st = check_device(&dev);
   if (st != RF_W8A16_OK) return st;

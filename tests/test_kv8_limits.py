@@ -1,11 +1,14 @@
-"""CPU tests of the int8 paged cache: layouts that KV8Cache takes, and sizes that the
-C ABI takes or refuses."""
+"""CPU tests of the int8 paged cache: layouts that KV8Cache takes, and operands that
+the C ABI refuses."""
 from __future__ import annotations
+
+import ctypes
 
 import pytest
 import torch
 
 import rhinoforge_amd as rf
+from rhinoforge_amd import capi
 
 
 @pytest.mark.parametrize("form", ["transposed", "strided", "broadcast"])
@@ -31,3 +34,40 @@ def test_from_quantized_of_scales_that_are_not_contiguous(form):
         rf.kv8_append(c, torch.zeros(1, hk, 64).half(), torch.zeros(1, hk, 64).half(), slots)
     # and its own way back
     assert all(torch.equal(a, b) for a, b in zip(c.to_quantized(), (k, s, v, s)))
+
+
+# ---- the C ABI: rf_kv8_plan's outputs apart from its inputs ---------------------------
+
+IN = {"cached": 5, "fresh": 5, "free_blocks": 9, "free_start": 1}    # elements, for 5 requests
+OUT = {"slots": 40, "positions": 40, "cu": 6, "kv_lens": 5, "free_next": 1}
+
+
+def _plan(**at):
+    """The status of a call whose arrays are at made-up addresses, 4 KB apart."""
+    names = ["block_table", *IN, *OUT]
+    where = {n: (1 << 20) + 4096 * i for i, n in enumerate(names)}
+    a = capi.KV8PlanArgs(**{**where, **at}, requests=5, width=3, table_stride=3, num_free=9, tokens=40,
+                         block_size=32)
+    if at == {}:
+        return where
+    return capi.load().rf_kv8_plan(ctypes.byref(a), None)
+
+
+@pytest.mark.parametrize("out", sorted(OUT))
+@pytest.mark.parametrize("inp", sorted(IN))
+def test_plan_refuses_outputs_over_its_inputs(out, inp):
+    """A workgroup may read an input after another has written its outputs."""
+    where = _plan()
+    assert _plan(**{out: where[inp]}) == capi.EINVAL
+    assert _plan(**{out: where[inp] + 4 * (IN[inp] - 1)}) == capi.EINVAL
+    assert _plan(**{out: where[inp] - 4 * (OUT[out] - 1)}) == capi.EINVAL
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses are made up: nothing may run on them")
+@pytest.mark.parametrize("out", sorted(OUT))
+@pytest.mark.parametrize("inp", sorted(IN))
+def test_plan_takes_outputs_right_beside_its_inputs(out, inp):
+    """Refused later, for want of a device."""
+    where = _plan()
+    assert _plan(**{out: where[inp] + 4 * IN[inp]}) not in (capi.OK, capi.EINVAL)
+    assert _plan(**{out: where[inp] - 4 * OUT[out]}) not in (capi.OK, capi.EINVAL)
