@@ -47,11 +47,13 @@ __device__ __forceinline__ float sum_lanes(float v) {
   return v;
 }
 
-// kPart: some dimensions are not rotated.  (A form of its own: where all are, the
-// selects that it takes would cost a wavefront per SIMD, 27.6 -> 29.3 us.)
+// kPart: some dimensions are not rotated.  A form of its own: where all are, the
+// selects that it takes would cost a wavefront per SIMD (27.8 -> 29.3 us), and here
+// fewer loads ahead pay for them (half of 128 rotated, 4001 tokens, 64 + 8 heads:
+// 31.5 us with four, 30.0 with two; interleaved 31.7, 30.8 with three).
 template <typename T, int LP, bool kInterleaved, bool kPart>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeArgs a) {
-  constexpr int kHeads = kWave / LP, kAhead = 4;
+  constexpr int kHeads = kWave / LP, kAhead = !kPart ? 4 : kInterleaved ? 3 : 2;
   typedef T tx4 __attribute__((ext_vector_type(4)));
   const int lane = threadIdx.x % kWave, sub = lane % LP;
   const unsigned w = blockIdx.x * (256 / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
