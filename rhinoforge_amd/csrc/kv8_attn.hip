@@ -530,7 +530,7 @@ __device__ __forceinline__ void join(const AttnArgs& a, const Tile& t, int h, in
 // cache straight into MFMA operands (no LDS), one turn ahead of the products.  At
 // the end the wavefronts' sums meet in LDS.  Bound by the cache's bytes: 130999
 // tokens, 32 + 8 heads of 128, in 47.1 us, 5.7 TB/s (a plain read of as many bytes
-// reaches 6.7); short contexts by their round trips: 777 tokens 8.0 us, of which
+// reaches 6.7); short contexts by their round trips: 777 tokens 8.4 us, of which
 // 4.4 remain for 64 tokens.  Eight wavefronts a workgroup gave the same times:
 // one CU takes in about 64 GB/s however many of them ask.
 // ---------------------------------------------------------------------------
@@ -820,9 +820,9 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_decode_kernel(AttnArgs a) {
 // fill the chip several times (2500 tokens, 16 + 8 heads: 69 us with one gang, 49
 // with two; 1000 tokens, 32 + 8: 32 and 26; but 7999, 64 + 8: 1127 and 1224).
 // 7999 tokens, 64 + 8 heads of 128:
-// 1102 to 1174 us on different cards, 952 to 893 TFLOP/s, where a library product
+// 1089 to 1174 us on different cards, 963 to 893 TFLOP/s, where a library product
 // of 16384^3 reaches 1300.
-// Vector units 64% and matrix units 45% busy at 1.9 of 2.4 GHz: the clock gives
+// Vector units 63% and matrix units 45% busy at 1.9 of 2.4 GHz: the clock gives
 // way to the power they draw.  Variants with other orders of the same
 // instructions (products and weights interleaved one by one, operands read
 // ahead, loads one step ahead instead of two) differ by up to 6% in cycles and
@@ -1264,7 +1264,8 @@ struct Estimate {
 
 Estimate estimate(bool prefill, int gangs, int rows, double tiles, double groups, double longest, double tokens_heads, bool ragged,
                   double shared, int most_rows, int D, int hk, int cus) {
-  // us of a turn at `per_cu` workgroups on each CU; slots: workgroups per CU
+  // us of a turn; slots: workgroups that run at a time (prompts of size 256: LDS
+  // holds one on each CU, the fitted constants go with two)
   const double base = prefill ? (D == 64 ? 1.1 : D == 128 ? 1.5 : 1.35)
                               : D == 256 ? 1.1 : (rows == 16 ? 0.55 : 0.85) * (D == 64 ? 0.75 : 1.0);
   const double more = prefill ? (D == 256 ? 0.6 : 0.4) : D == 256 ? 1.2 : (rows == 16 ? 0.25 : 0.58) * (D == 64 ? 0.6 : 1.0);

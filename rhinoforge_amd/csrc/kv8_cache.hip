@@ -15,7 +15,7 @@ namespace {
 // with that token's cos and sin and the weight in registers and the next heads'
 // loads in flight; heads advance a scalar base, so they cost no address math
 // (4001 tokens of 64 + 8 heads: 46 us with per-lane addresses and IEEE square
-// root and division, 28.7 so).
+// root and division, 27.8 so).
 // ---------------------------------------------------------------------------
 struct RopeArgs {
   const uint8_t *q, *k;
