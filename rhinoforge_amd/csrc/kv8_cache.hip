@@ -398,10 +398,11 @@ __device__ __forceinline__ void requantize(uint8_t* dst, int side, int o0, float
 // trips slots, values and scales, stores, whatever their number.  Longer ones
 // come one after the other: the values are read once, stay in registers until
 // the scale is known and go out through LDS in 16-byte chunks.  Bound by those
-// round trips for few tokens (48 single ones: 5.3 us, 256: 5.3), by the bytes for
-// many (6874 tokens in prompts, 8 heads of 128: 14.9 us, 2.8 TB/s).  A wavefront
-// for each run, which single tokens alone would like (4.7 us for 256), needs 127 us
-// for a prompt of 1024 tokens, where this takes 6.0.
+// round trips for few tokens (48 single ones: 5.3 us, 256: 5.6), by the bytes for
+// many (6874 tokens in prompts, 8 heads of 128: 14.8 us, 2.9 TB/s).  A wavefront
+// for each run, which single tokens alone would like (3.7 us for 48, 4.7 for 256),
+// needs 127 us for a prompt of 1024 tokens, where this takes 6.0.  256 runs of 8
+// tokens take 13.0 us, of 9, one after the other, 21.0.
 constexpr int kShort = 8;
 
 template <typename T, int D, int BS>
@@ -619,7 +620,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
 // Where they are one 32-token group of a block its bytes are read in memory
 // order and turned in LDS into rows of tokens; any other 32 are gathered, eight
 // dimensions of one token per thread.  Bound by the values it writes: 6874
-// tokens, 8 heads of 128: 13.1 us, 3.2 TB/s (gathering all of them: 19).
+// tokens, 8 heads of 128: 12.6 us, 3.4 TB/s (gathering all of them: 19).
 // ---------------------------------------------------------------------------
 struct ReadArgs {
   const uint8_t *k, *v;
