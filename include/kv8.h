@@ -98,6 +98,27 @@ typedef struct rf_kv8_rope_args {
 } rf_kv8_rope_args;
 int rf_kv8_qk_norm_rope(const rf_kv8_rope_args* args, void* stream);
 
+/* The same with positions of several axes (images and video: time, height,
+ * width).  Pair i turns by row positions[axis(i) * axis_stride + t], column i.
+ *   axes       1 .. RF_KV8_MAX_AXES
+ *   sections   pairs of each axis (0 or more), rot / 2 together
+ *   mixed 0    the axes' pairs one after the other: sections[0] of axis 0, then
+ *              sections[1] of axis 1, ..
+ *   mixed 1    in turn: pair i belongs to axis i % axes while i / axes is below
+ *              that axis' section, to axis 0 from there on; sections have to be
+ *              such that all pairs of the axes above 0 are there
+ * positions are needed, and rot > 0.  A position of any axis outside the table
+ * gives a token of NaN.  axis_stride: elements between axes, at least tokens. */
+#define RF_KV8_MAX_AXES 4
+typedef struct rf_kv8_mrope_args {
+  rf_kv8_rope_args rope;
+  int64_t axis_stride;
+  int32_t axes;
+  int32_t mixed;
+  int32_t sections[RF_KV8_MAX_AXES];
+} rf_kv8_mrope_args;
+int rf_kv8_qk_norm_mrope(const rf_kv8_mrope_args* args, void* stream);
+
 /* Block tables and slots of a batch, from its lengths (negative: taken as 0).
  * Request i holds cached[i] tokens and gets fresh[i] new ones; its blocks
  * [ceil(cached / bs), ceil((cached + fresh) / bs)) are taken from `free_blocks`

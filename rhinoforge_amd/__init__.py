@@ -53,10 +53,12 @@ from .quant import (dequantize_int4_group_wise, dequantize_linear_per_channel,  
                     quantize_int4_group_wise, quantize_int4_per_channel,
                     quantize_linear_per_channel)
 from .kv8 import (KV8Cache, KV8Plan, kv8_append, kv8_attention, kv8_plan, kv8_read,  # noqa: E402
-                  qk_norm_rope, rope_table)
+                  qk_norm_mrope, qk_norm_rope, rope_table)
+from .kv4 import KV4Cache, kv4_append, kv4_attention, kv4_read  # noqa: E402
 from .nn import W4A16Linear, W8A16Embedding, W8A16Linear  # noqa: E402
 
 __all__ = [
+    "KV4Cache",
     "KV8Cache",
     "KV8Plan",
     "LAYOUT_ROWMAJOR",
@@ -70,6 +72,9 @@ __all__ = [
     "W8A16Linear",
     "dequantize_int4_group_wise",
     "dequantize_linear_per_channel",
+    "kv4_append",
+    "kv4_attention",
+    "kv4_read",
     "kv8_append",
     "kv8_attention",
     "kv8_plan",
@@ -84,6 +89,7 @@ __all__ = [
     "pack_weight_int4",
     "packed_shape",
     "packed_shape_int4",
+    "qk_norm_mrope",
     "qk_norm_rope",
     "quantize_int4_group_wise",
     "quantize_int4_per_channel",

@@ -26,8 +26,9 @@ LIBDIR = PKG / "lib"
 INCLUDE = ROOT / "include"
 
 CAPI_SOURCES = ["w8a16_capi.hip", "w8a16_gemv.hip", "w8a16_gemm.hip", "w8a16_quant.hip",
-                "kv8_capi.hip", "kv8_cache.hip", "kv8_attn.hip"]
-TORCH_SOURCES = ["w8a16_torch.cpp", "kv8_torch.cpp"]
+                "kv8_capi.hip", "kv8_cache.hip", "kv8_attn.hip",
+                "kv4_capi.hip", "kv4_cache.hip", "kv4_attn.hip"]
+TORCH_SOURCES = ["w8a16_torch.cpp", "kv8_torch.cpp", "kv4_torch.cpp"]
 CAPI_LIB = LIBDIR / "librf_w8a16.so"
 TORCH_LIB = LIBDIR / "librf_w8a16_torch.so"
 BENCH_LIB = LIBDIR / "librf_bench.so"

@@ -1,4 +1,4 @@
-"""ctypes binding of the C ABI in include/w8a16.h and include/kv8.h.
+"""ctypes binding of the C ABI in include/w8a16.h, include/kv8.h and include/kv4.h.
 
 This is the binding a Python host (such as the reference's runtime) would add
 to call the library without the torch op.  It loads ``lib/librf_w8a16.so``;
@@ -171,9 +171,34 @@ class KV8AttentionArgs(ctypes.Structure):
                 ("scale", _c.c_float)]
 
 
+class KV8MropeArgs(ctypes.Structure):
+    """struct rf_kv8_mrope_args."""
+    _fields_ = [("rope", KV8RopeArgs), ("axis_stride", _c.c_int64), ("axes", _c.c_int32),
+                ("mixed", _c.c_int32), ("sections", _c.c_int32 * 4)]
+
+
+class KV4Cache(ctypes.Structure):
+    """struct rf_kv4_cache (include/kv4.h)."""
+    _fields_ = [("k", _c.c_void_p), ("v", _c.c_void_p), ("rows", _c.c_void_p),
+                ("num_blocks", _c.c_int64), ("kv_heads", _c.c_int32), ("head_dim", _c.c_int32),
+                ("block_size", _c.c_int32)]
+
+
+class KV4AttentionArgs(ctypes.Structure):
+    """struct rf_kv4_attention_args."""
+    _fields_ = [("cache", KV4Cache), ("q", KV8Heads), ("cu_q", _c.c_void_p),
+                ("kv_lens", _c.c_void_p), ("block_table", _c.c_void_p), ("out", _c.c_void_p),
+                ("lse", _c.c_void_p), ("scratch", _c.POINTER(Scratch)),
+                ("tokens", _c.c_int64), ("requests", _c.c_int64), ("width", _c.c_int64),
+                ("table_stride", _c.c_int64), ("max_q_len", _c.c_int64), ("max_kv_len", _c.c_int64),
+                ("dtype", _c.c_int32), ("causal", _c.c_int32), ("window", _c.c_int64),
+                ("scale", _c.c_float)]
+
+
 # name -> (restype, argtypes): every entry point declared in include/kv8.h
 KV8_SIGNATURES = {
     "rf_kv8_qk_norm_rope": (_c.c_int, [_c.POINTER(KV8RopeArgs), _c.c_void_p]),
+    "rf_kv8_qk_norm_mrope": (_c.c_int, [_c.POINTER(KV8MropeArgs), _c.c_void_p]),
     "rf_kv8_plan": (_c.c_int, [_c.POINTER(KV8PlanArgs), _c.c_void_p]),
     "rf_kv8_append": (_c.c_int, [_c.POINTER(KV8Cache), _c.POINTER(KV8Heads), _c.POINTER(KV8Heads),
                                  _c.c_int32, _c.c_void_p, _c.c_int64, _c.c_void_p]),
@@ -181,6 +206,16 @@ KV8_SIGNATURES = {
                                _c.c_void_p, _c.c_void_p, _c.c_void_p]),
     "rf_kv8_attention_workspace": (_c.c_size_t, [_c.POINTER(KV8AttentionArgs)]),
     "rf_kv8_attention": (_c.c_int, [_c.POINTER(KV8AttentionArgs), _c.c_void_p]),
+}
+
+# ... in include/kv4.h
+KV4_SIGNATURES = {
+    "rf_kv4_append": (_c.c_int, [_c.POINTER(KV4Cache), _c.POINTER(KV8Heads), _c.POINTER(KV8Heads),
+                                 _c.c_int32, _c.c_void_p, _c.c_int64, _c.c_void_p]),
+    "rf_kv4_read": (_c.c_int, [_c.POINTER(KV4Cache), _c.c_void_p, _c.c_int64, _c.c_int32,
+                               _c.c_void_p, _c.c_void_p, _c.c_void_p]),
+    "rf_kv4_attention_workspace": (_c.c_size_t, [_c.POINTER(KV4AttentionArgs)]),
+    "rf_kv4_attention": (_c.c_int, [_c.POINTER(KV4AttentionArgs), _c.c_void_p]),
 }
 
 _lib = None
@@ -193,7 +228,7 @@ def load() -> ctypes.CDLL:
         if not LIB_PATH.is_file():
             raise OSError(f"{LIB_PATH} not built; run `python rhinoforge_amd/_build.py`")
         lib = ctypes.CDLL(str(LIB_PATH))
-        for name, (res, args) in {**SIGNATURES, **KV8_SIGNATURES}.items():
+        for name, (res, args) in {**SIGNATURES, **KV8_SIGNATURES, **KV4_SIGNATURES}.items():
             fn = getattr(lib, name)
             fn.restype = res
             fn.argtypes = args

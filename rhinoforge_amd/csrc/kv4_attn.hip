@@ -1,0 +1,778 @@
+// Attention over the 4-bit paged cache (kv4.h), gfx950.
+//
+// For query row q (one query, one head) over its seen tokens j, which hold whole
+// numbers k_j, v_j, steps a_j, b_j and zero points y_j, z_j:
+//   x_j = (q . k_j - y_j sum(q)) a_j scale log2(e),  p_j = 2^(x_j - m)
+//   o   = sum p_j b_j (v_j - z_j) / sum p_j
+// in one pass over the tokens with a running reference m.
+//
+// Both products run on the matrix cores with the cache as the A operand and the
+// queries as columns, as over the int8 cache (kv8_attn.hip): scores leave the first
+// product as the second one takes its operand.
+//
+// Few rows: a token's numbers meet one tile of rows or two, so as little as
+// possible is done to them.  Keys: k - 8, exact in fp16 (without the 8 the products
+// would have one sign, and the matrix cores' sums lose two bits more: an lse off by
+// 6e-7 instead of 1e-7); what the zero point differs from 8, and the step, go into
+// the scores, of which there is one for 64 or more numbers.  Values: v - z, exact
+// in fp16; the step goes into the weight.
+// Many rows: every number is turned into the fp16 value that it stands for (exact),
+// once for 128 rows, and what is left is attention over fp16.
+//
+//   * Queries: fp16 as they are.  bf16 times a power of two per row, which
+//     brings the row's largest magnitude to [2^14, 2^15): exact in fp16 down to
+//     2^-31 of it, within 2^-39 of it below; the power goes into that row's score
+//     factor.
+//   * Weights p b (or p) are rounded to fp16 (11 bits, to nearest): 2^-11
+//     relative, as much as the output's own rounding in fp16.  2^7 times the weight
+//     is what is rounded, the row's largest so far lies in [2^7, 2^15), and what is
+//     below fp16's normal range loses at most 2^-25: 2^-32 of the largest weight.
+//   * m, the sums and o stay in fp32.
+#include "kv4_common.h"
+#include "paged_attn.h"
+
+namespace rf {
+namespace {
+
+struct AttnArgs : PagedArgs {
+  const uint16_t* rows;
+};
+
+// Nothing seen yet.  (Finite: differences from scores of -inf are not NaN.)
+constexpr float kNothing = -1e30f;
+// Score factors stay finite and above 0: a masked score is -inf whatever it is
+// multiplied by, and scores beyond these ranges are 0 or infinite to exp2.
+__device__ __forceinline__ float in_range(float factor) { return fminf(fmaxf(factor, 0x1p-126f), 0x1p127f); }
+
+// (n - z) of a token pair's numbers: base - (base + z), exact in fp16.
+__device__ __forceinline__ half2v less(uint32_t v, uint32_t z) { return as_half2(v) - as_half2(z); }
+
+// ---------------------------------------------------------------------------
+// Few rows (single tokens, a few drafted ones): RT tiles of 16 rows, held by
+// all four wavefronts; the wavefronts take 32-token groups in turn and read the
+// cache straight into MFMA operands (no LDS), kAhead turns ahead of the products.
+// At the end the wavefronts' sums meet in LDS.
+// ---------------------------------------------------------------------------
+template <int D>
+struct Bytes {
+  uint4 k[D / 64], v[D / 64];
+  uint4 kw, vw;  // words of this lane's eight tokens
+};
+
+template <int D>
+__device__ __forceinline__ void fetch(const AttnArgs& a, const Group& g, int lane, Bytes<D>& b) {
+  const int64_t group = (g.at << (a.shift - 5)) + g.sub;
+  const uint8_t* kp = a.k + group * (16 * D);
+  const uint8_t* vp = a.v + group * (16 * D);
+  const uint16_t* rp = a.rows + group * 64;
+  b.kw = load_u4(rp + lane / 16 * 8);
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) b.k[i] = load_u4_stream(kp + i * kTileBytes + lane * 16);
+  b.vw = load_u4(rp + 32 + lane / 16 * 8);
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) b.v[i] = load_u4_stream(vp + i * kTileBytes + lane * 16);
+}
+
+// Eight numbers less 8, in the order of their dimensions.
+__device__ __forceinline__ half8 centred8(uint32_t d) {
+  constexpr uint32_t k8 = 0x64086408u, k84 = 0x54805480u;  // 1024 + 8, 64 + 8
+  const uint32_t d8 = d >> 8;
+  return join8(less(and_or(d, kNibbles, kBase), k8), less(and_or(d, kNibbles4, kBase4), k84),
+               less(and_or(d8, kNibbles, kBase), k8), less(and_or(d8, kNibbles4, kBase4), k84));
+}
+
+template <typename T, int D, int RT>
+__global__ __launch_bounds__(kWaves* kWave)
+__attribute__((amdgpu_waves_per_eu(2))) void kv4_decode_kernel(AttnArgs a) {
+  constexpr int R = 16 * RT, A = D / 64;
+  __shared__ __align__(16) float red[kWaves][16][D + 4];
+  __shared__ float red_m[kWaves][R], red_l[kWaves][R];
+  const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int col = lane % 16, lg = lane / 16;
+  const unsigned id = a.first + blockIdx.x, pair = id / (unsigned)a.hk;
+  const int h = (int)(id - pair * a.hk);
+  int split, splits;
+  Tile t;
+  if (a.shares) {
+    if (!find_share<R>(a, (int)pair, &t, &split, &splits)) return;
+  } else {
+    const int x = (int)(pair / (unsigned)a.splits);
+    if (!find_tile<R>(a, x, &t)) return;
+    splits = a.splits;
+    split = (int)(pair - (unsigned)x * splits);
+  }
+  const int rows = min(t.queries * a.group - t.row0, R);  // of this tile
+  // its first and last rows bound what any row sees
+  int lo_min, lo_max, hi_min, hi_max;
+  seen(a, t, t.row0, &lo_min, &hi_min);
+  seen(a, t, t.row0 + rows - 1, &lo_max, &hi_max);
+  lo_max = uniform(lo_max), hi_min = uniform(hi_min);
+  const Share share = share_of(a, lo_min >> 5, (hi_max + 31) >> 5, split, splits);
+  if (split >= share.splits) {
+    if (a.merge) no_share(a, t, h, rows, split);
+    return;
+  }
+  const int begin = uniform(share.begin), end = uniform(share.end);
+  const bool partial = share.splits > 1 || a.merge;
+
+  // ---- queries, as B operands: column = row, dimensions 64 i + 16 lg + 8 j + ..
+  half8 q[RT][2 * A];
+  float factor[RT], qsum[RT];  // qsum: -sum(q)
+  int lo[RT], hi[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    const int row = t.row0 + min(16 * r + col, rows - 1);
+    const int qi = (int)((unsigned)row / (unsigned)a.group);
+    const uint8_t* p = a.q + (int64_t)(t.first_token + qi) * a.q_ts +
+                       (int64_t)(h * a.group + (row - qi * a.group)) * a.q_hs + lg * 32;
+    uint4 raw[2 * A];
+#pragma unroll
+    for (int i = 0; i < 2 * A; ++i) raw[i] = load_u4(p + (i / 2) * 128 + (i % 2) * 16);
+    factor[r] = a.scale_log2e;
+    if constexpr (!__is_same(T, _Float16)) {
+      float m = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 2 * A; ++i) m = load_amax<T>(raw[i], m);
+      m = fmaxf(m, __shfl_xor(m, 16));
+      m = fmaxf(m, __shfl_xor(m, 32));
+      const int e = row_exponent(m), e1 = e / 2, e2 = e - e1;
+      const float f1 = pow2(-e1), f2 = pow2(-e2);
+#pragma unroll
+      for (int i = 0; i < 2 * A; ++i)
+        q[r][i] = __builtin_convertvector(Eight<T>::load(&raw[i]) * f1 * f2, half8);
+      factor[r] = a.scale_log2e * pow2(e1) * pow2(e2);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2 * A; ++i) q[r][i] = as_half8(raw[i]);
+    }
+    factor[r] = in_range(factor[r]);
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 2 * A; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum += (float)q[r][i][j];
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    qsum[r] = -sum;
+    seen(a, t, row, &lo[r], &hi[r]);
+  }
+  floatx4 acc[RT][4 * A];
+  float m[RT], l[RT];  // l: each lane's own share of the sum
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    m[r] = kNothing;
+    l[r] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4 * A; ++i) acc[r][i] = floatx4{0, 0, 0, 0};
+  }
+
+  const auto step = [&](const Bytes<D>& b, int g, bool ok) {
+    floatx4 s[RT][2];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) s[r][0] = s[r][1] = floatx4{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < A; ++i) {
+      const uint32_t d[4] = {b.k[i].x, b.k[i].y, b.k[i].z, b.k[i].w};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const half8 k = centred8(d[w]);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) s[r][w / 2] = mfma16x16x32(k, q[r][2 * i + w % 2], s[r][w / 2]);
+      }
+    }
+    const uint32_t kw[4] = {b.kw.x, b.kw.y, b.kw.z, b.kw.w}, vw[4] = {b.vw.x, b.vw.y, b.vw.z, b.vw.w};
+    half2v ks[4], kz[4], vs[4];  // tokens 2 i and 2 i + 1 of the lane's eight
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      ks[i] = as_half2(kw[i] & kStepBits);
+      kz[i] = less(and_or(kw[i], kNibbles, kBase), 0x64086408u);  // less 8
+      vs[i] = as_half2(vw[i] & kStepBits);
+    }
+    const int t0 = opaque(g << 5);
+    const bool edge = t0 < lo_max || t0 + 32 > hi_min;
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = __builtin_fmaf((float)kz[i / 2][i % 2], qsum[r], s[r][i / 4][i % 4]);
+        s[r][i / 4][i % 4] = __builtin_fmaf((float)ks[i / 2][i % 2], x, 0.0f);
+      }
+      if (!ok) {
+        keep_branch();
+        s[r][0] = s[r][1] = __builtin_nanf("");
+      }
+      if (edge) {
+        keep_branch();
+        const int first = lo[r] - t0 - 8 * lg, past = hi[r] - t0 - 8 * lg;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          s[r][i / 4][i % 4] = ((i < first) | (i >= past)) ? -__builtin_inff() : s[r][i / 4][i % 4];
+      }
+    }
+    half8 p[RT];
+    float sum[RT];
+    bool raise = false;
+    const auto weights = [&](int r) {  // the largest of them
+      const float off = kShift - m[r];
+      float most = 0.0f;
+      sum[r] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float e = exp2_fast(__builtin_fmaf(s[r][i / 4][i % 4], factor[r], off));
+        const float w = __builtin_fmaf((float)vs[i / 2][i % 2], e, 0.0f);
+        sum[r] += e;
+        most = fmaxf(most, w);
+        p[r][i] = (_Float16)w;
+      }
+      return most;
+    };
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const float most = weights(r);
+      raise |= most > 32768.0f || sum[r] == __builtin_inff();
+    }
+    if (__ballot(raise)) {
+      keep_branch();
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        float top = m[r];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          top = fmaxf(top, s[r][i / 4][i % 4] * factor[r] + log2_fast(fmaxf((float)vs[i / 2][i % 2], 0x1p-24f)));
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float f = exp2_fast(m[r] - top);
+        m[r] = top;
+        l[r] *= f;
+#pragma unroll
+        for (int i = 0; i < 4 * A; ++i) acc[r][i] *= f;
+        weights(r);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < RT; ++r) l[r] += sum[r];
+    uint32_t z[4], z4[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      z[i] = and_or(vw[i], kNibbles, kBase);
+      z4[i] = and_or(vw[i] << 4, kNibbles4, kBase4);
+    }
+#pragma unroll
+    for (int i = 0; i < A; ++i) {
+      const uint32_t d[4] = {b.v[i].x, b.v[i].y, b.v[i].z, b.v[i].w};
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        half2v v[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t x = n < 2 ? d[w] : d[w] >> 8;
+          v[w] = n % 2 ? less(and_or(x, kNibbles4, kBase4), z4[w]) : less(and_or(x, kNibbles, kBase), z[w]);
+        }
+        const half8 v8 = join8(v[0], v[1], v[2], v[3]);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) acc[r][4 * i + n] = mfma16x16x32(v8, p[r], acc[r][4 * i + n]);
+      }
+    }
+  };
+
+  if (begin + wave < end) {
+    // group g's bytes are loaded while group g - kWaves is worked on, and its
+    // block id one turn before that.
+    const auto id_of = [&](int g) { return group_of(a, t, h, min(g, end - 1)); };
+    int g = begin + wave;
+    Bytes<D> b0, b1;
+    Group now = id_of(g), next = id_of(g + kWaves);
+    fetch<D>(a, now, lane, b0);
+    while (true) {
+      fetch<D>(a, next, lane, b1);
+      bool ok = now.ok;
+      now = next;
+      next = id_of(g + 2 * kWaves);
+      step(b0, g, ok);
+      g += kWaves;
+      if (g >= end) break;
+      fetch<D>(a, next, lane, b0);
+      ok = now.ok;
+      now = next;
+      next = id_of(g + 2 * kWaves);
+      step(b1, g, ok);
+      g += kWaves;
+      if (g >= end) break;
+    }
+  }
+
+  // ---- the four wavefronts' results
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    l[r] += __shfl_xor(l[r], 16);
+    l[r] += __shfl_xor(l[r], 32);
+    if (lg == 0) {
+      red_m[wave][16 * r + col] = m[r];
+      red_l[wave][16 * r + col] = l[r];
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    __syncthreads();
+    const int rr = 16 * r + col;
+    float top = red_m[0][rr];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, red_m[w][rr]);
+    const float f = exp2_fast(m[r] - top);
+#pragma unroll
+    for (int i = 0; i < A; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        floatx4 o;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) o[n] = acc[r][4 * i + n][j] * f;
+        *reinterpret_cast<floatx4*>(&red[wave][col][64 * i + 16 * lg + 4 * j]) = o;
+      }
+    __syncthreads();
+    for (int it = tid; it < 16 * (D / 4); it += kThreads) {
+      const int c = it / (D / 4), d = it % (D / 4) * 4, rc = 16 * r + c;
+      if (rc >= rows) continue;
+      float mm = red_m[0][rc];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) mm = fmaxf(mm, red_m[w][rc]);
+      float ll = 0.0f;
+      floatx4 o = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        ll += red_l[w][rc] * exp2_fast(red_m[w][rc] - mm);
+        o += *reinterpret_cast<const floatx4*>(&red[w][c][d]);
+      }
+      const int64_t to = out_row(a, t, h, rc);
+      if (partial) {
+        const Partials parts(a);
+        const int i = a.merge ? (int)to * a.splits + split : (int)id * R + rc;
+        parts.store(i * D + d, o);
+        if (d == 0) parts.store_stat(i, mm, ll);
+      } else {
+        finish<T>(a, to, D, d, o, mm, ll);
+      }
+    }
+  }
+  if (partial && !a.merge)
+    join<T, D>(a, t, h, rows, share.splits, ((int)id - split * a.hk) * R, a.hk * R,
+               a.counters + (id - (unsigned)(split * a.hk)), &red[0][0][0]);
+}
+
+// ---------------------------------------------------------------------------
+// Many rows (prompts): four wavefronts of 32 rows each.  A step's numbers are
+// loaded once per workgroup, turned into the fp16 values that they stand for on
+// their way into LDS, in operand order (a wavefront reads 1 KB in lane order per
+// MFMA), and those of the next two steps are loaded meanwhile.  G = 2: two gangs
+// of four wavefronts take the steps of the same rows in turn, and their sums join
+// at the end: what the longest tile takes is halved, which is what a prompt takes
+// that does not fill the chip several times.
+// ---------------------------------------------------------------------------
+template <typename T, int D, int G>
+__global__ __launch_bounds__(G* kWaves* kWave)
+__attribute__((amdgpu_waves_per_eu(2))) void kv4_prefill_kernel(AttnArgs a) {
+  constexpr int R = 32 * kWaves, A = D / 64;
+  constexpr int NG = D <= 128 ? 2 : 1;          // 32-token groups of a step
+  constexpr int kBuf = NG * 32 * D * 2 * 2;     // bytes of a step's K and V in fp16
+  // A step has NG * A tiles of keys and as many of values: one of each per
+  // wavefront, or, of size 64, one of either.
+  constexpr bool kBoth = NG * A == kWaves;
+  constexpr bool kQLds = D > 128;               // see below
+  // (sized at the launch: with the size known here the register allocator
+  // trades registers for it, and spills)
+  extern __shared__ __align__(16) uint8_t lds[];
+  const int tid = threadIdx.x, lane = tid % kWave, any_wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int wave = any_wave % kWaves, gang = any_wave / kWaves;
+  uint8_t* const bufs = lds + gang * 2 * kBuf;
+  const int col = lane % 32, lh = lane / 32;
+  const unsigned id = a.first + blockIdx.x, pair = id / (unsigned)a.hk;
+  const int h = (int)(id - pair * a.hk), turn = (int)(pair / (unsigned)a.splits);
+  const int split = (int)(pair - (unsigned)turn * a.splits);
+  // the last tiles of a request see the most tokens: they begin first
+  const int x = a.tiles - 1 - turn;
+  Tile t;
+  if (!find_tile<R>(a, x, &t)) return;
+  const int rows = min(t.queries * a.group - t.row0, R);  // of this tile
+  int lo_min, hi_max, unused;
+  seen(a, t, t.row0, &lo_min, &unused);
+  seen(a, t, t.row0 + rows - 1, &unused, &hi_max);
+  const Share share = share_of(a, lo_min >> 5, (hi_max + 31) >> 5, split, a.splits);
+  if (split >= share.splits) {
+    no_share(a, t, h, rows, split);
+    return;
+  }
+  const int begin = uniform(share.begin), end = uniform(share.end);
+  const bool partial = a.splits > 1;  // merge_splits_kernel adds them
+
+  // Size 256: the sums take 128 registers, so the queries stay in LDS, where
+  // each lane reads its own.
+  half8 q[kQLds ? 1 : D / 16];
+  half8* q_lds = reinterpret_cast<half8*>(lds + G * 2 * kBuf) + wave * (D / 16) * kWave + lane;
+  const auto put_q = [&](int i, half8 v) {
+    if constexpr (kQLds) q_lds[i * kWave] = v;
+    else q[i] = v;
+  };
+  const auto get_q = [&](int i) {
+    if constexpr (kQLds) return q_lds[i * kWave];
+    else return q[i];
+  };
+  float factor = a.scale_log2e;
+  int lo, hi;
+  const int wrow = wave * 32;  // this wavefront's first row of the tile
+  {
+    const int row = t.row0 + min(wrow + col, rows - 1);
+    const int qi = (int)((unsigned)row / (unsigned)a.group);
+    const uint8_t* p = a.q + (int64_t)(t.first_token + qi) * a.q_ts +
+                       (int64_t)(h * a.group + (row - qi * a.group)) * a.q_hs + lh * 16;
+    uint4 raw[D / 16];
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) raw[i] = load_u4(p + i * 32);
+    if constexpr (!__is_same(T, _Float16)) {
+      float m = 0.0f;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) m = load_amax<T>(raw[i], m);
+      m = fmaxf(m, __shfl_xor(m, 32));
+      const int e = row_exponent(m), e1 = e / 2, e2 = e - e1;
+      const float f1 = pow2(-e1), f2 = pow2(-e2);
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+        put_q(i, __builtin_convertvector(Eight<T>::load(&raw[i]) * f1 * f2, half8));
+      factor = a.scale_log2e * pow2(e1) * pow2(e2);
+    } else {
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) put_q(i, as_half8(raw[i]));
+    }
+    factor = in_range(factor);
+    seen(a, t, row, &lo, &hi);
+    hi = min(hi, end * 32);
+  }
+  const bool idle = wrow >= rows;
+  int my_lo_min, my_lo_max, my_hi_min, my_hi_max;
+  seen(a, t, t.row0 + min(wrow, rows - 1), &my_lo_min, &my_hi_min);
+  seen(a, t, t.row0 + min(wrow + 32, rows) - 1, &my_lo_max, &my_hi_max);
+  my_lo_min = uniform(my_lo_min), my_lo_max = uniform(my_lo_max);
+  my_hi_min = min(uniform(my_hi_min), end * 32), my_hi_max = min(uniform(my_hi_max), end * 32);
+
+  floatx16 acc[D / 32];
+  float m = kNothing, l = 0.0f;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) acc[i] = 0.0f;
+
+  // A step's bytes and words are loaded two steps ahead (a short share is bound
+  // by their round trip), its block ids three.
+  const int g16 = lane / 16, l16 = lane % 16;
+  const int tile = kBoth ? wave : wave % (kWaves / 2), my_group = tile / A, my_tile = tile % A;
+  const bool my_k = kBoth || wave < kWaves / 2, my_v = kBoth || wave >= kWaves / 2;
+  struct Ahead {
+    uint4 k, v, vw;
+    uint32_t kw;  // words of the lane's two tokens
+    bool ok[NG];
+  };
+  Group ids[NG];
+  const auto look = [&](int g) {
+#pragma unroll
+    for (int n = 0; n < NG; ++n) ids[n] = group_of(a, t, h, min(g + n, end - 1));
+  };
+  const auto load = [&](Ahead& x) {
+    const Group& gr = NG == 1 || my_group == 0 ? ids[0] : ids[NG - 1];
+    const int64_t group = (gr.at << (a.shift - 5)) + gr.sub;
+    const int64_t at = group * (16 * D) + my_tile * kTileBytes + lane * 16;
+    const uint16_t* rp = a.rows + group * 64;
+    if (my_k) {
+      const int token = l16 / 4 * 8 + l16 % 4;
+      x.k = load_u4(a.k + at);
+      x.kw = rp[token] | (uint32_t)rp[token + 4] << 16;
+    }
+    if (my_v) {
+      x.v = load_u4(a.v + at);
+      x.vw = load_u4(rp + 32 + g16 * 8);
+    }
+#pragma unroll
+    for (int n = 0; n < NG; ++n) x.ok[n] = ids[n].ok;
+  };
+  // Element e of a value operand is token 16 u + 8 lh + e, so the first product's
+  // rows are in the order 16 u + 8 x + 4 lh + c for token 16 u + 8 lh + 4 x + c.  A
+  // 32-dimension tile of values holds dimension 4 c + b in row 8 b + c.
+  const auto stage = [&](uint8_t* buf, const Ahead& x) {
+    if (my_k) {
+      const uint32_t d[4] = {x.k.x, x.k.y, x.k.z, x.k.w};
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt) {
+        const uint32_t w = __builtin_amdgcn_perm(x.kw, x.kw, tt ? 0x03020302u : 0x01000100u);
+        const half2v s = as_half2(w & kStepBits);
+        const uint32_t z = and_or(w, kNibbles, kBase), z4 = and_or(w << 4, kNibbles4, kBase4);
+        const int row = 16 * (l16 / 8) + 8 * tt + 4 * (l16 / 4 % 2) + l16 % 4;
+        uint8_t* p = buf + ((my_group * (D / 16) + my_tile * 4 + g16) * kWave + row) * 16;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t u = d[2 * tt + j], u8 = u >> 8;
+          *reinterpret_cast<half8*>(p + j * 32 * 16) =
+              join8(less(and_or(u, kNibbles, kBase), z) * s, less(and_or(u, kNibbles4, kBase4), z4) * s,
+                    less(and_or(u8, kNibbles, kBase), z) * s, less(and_or(u8, kNibbles4, kBase4), z4) * s);
+        }
+      }
+    }
+    if (my_v) {
+      const uint32_t d[4] = {x.v.x, x.v.y, x.v.z, x.v.w}, w[4] = {x.vw.x, x.vw.y, x.vw.z, x.vw.w};
+      uint8_t* p = buf + kBuf / 2 + (((my_group * (D / 32) + my_tile * 2 + l16 / 8) * 2 + g16 / 2) * kWave +
+                                     (g16 % 2) * 32 + l16 % 8) * 16;
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        half2v v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t u = n < 2 ? d[i] : d[i] >> 8;
+          const half2v s = as_half2(w[i] & kStepBits);
+          v[i] = n % 2 ? less(and_or(u, kNibbles4, kBase4), and_or(w[i] << 4, kNibbles4, kBase4)) * s
+                       : less(and_or(u, kNibbles, kBase), and_or(w[i], kNibbles, kBase)) * s;
+        }
+        *reinterpret_cast<half8*>(p + n * 8 * 16) = join8(v[0], v[1], v[2], v[3]);
+      }
+    }
+  };
+  // One step of a wavefront: all of its scores, one look at their maximum, then
+  // the weights.  The products of a group with V are issued among the weights of
+  // the next group, the last ones among the conversion of the next step's bytes:
+  // those take the vector units, these the matrix units.  A wavefront's priority
+  // rises through the step, so that of two that share a SIMD the one ahead stays
+  // ahead and they are in different phases.
+  const auto step = [&](const uint8_t* buf, int g, const bool (&ok)[NG], uint8_t* out, const Ahead& next) {
+    const int t0 = opaque(g << 5);
+    if (idle || t0 >= my_hi_max || t0 + 32 * NG <= my_lo_min) {
+      stage(out, next);
+      return;
+    }
+    floatx16 s[NG];
+#pragma unroll
+    for (int n = 0; n < NG; ++n) s[n] = 0.0f;
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+      for (int n = 0; n < NG; ++n) {
+        const half8 k = *reinterpret_cast<const half8*>(buf + ((n * (D / 16) + i) * kWave + lane) * 16);
+        s[n] = mfma32x32x16(k, get_q(i), s[n]);
+      }
+    __builtin_amdgcn_s_setprio(2);
+#pragma unroll
+    for (int n = 0; n < NG; ++n)
+      if (!ok[n]) {
+        keep_branch();
+        s[n] = __builtin_nanf("");
+      }
+    if (t0 < my_lo_max || t0 + 32 * NG > my_hi_min) {
+      keep_branch();
+      const int first = lo - t0 - 8 * lh, past = hi - t0 - 8 * lh;
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int tok = 32 * n + 16 * (i / 8) + i % 8;  // past t0 + 8 lh
+          s[n][i] = ((tok < first) | (tok >= past)) ? -__builtin_inff() : s[n][i];
+        }
+    }
+    float mx = -__builtin_inff();
+#pragma unroll
+    for (int n = 0; n < NG; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[n][i]);
+    mx *= factor;
+    if (__ballot(mx > m + kRaise)) {
+      const float top = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32))), f = exp2_fast(m - top);
+      m = top;
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) acc[i] *= f;
+    }
+    // (a value the compiler cannot fold into the branch above: merged with it, it
+    // would keep the sums twice, and spill)
+    float off = 0.0f;
+    if (opaque(t0) >= 0) {  // (always: a block of its own)
+      off = kShift - m;
+      asm volatile("" : "+v"(off));
+    }
+    half8 p[2];
+    const auto weights = [&](int n) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float e = exp2_fast(__builtin_fmaf(s[n][i], factor, off));
+        sum += e;
+        p[i / 8][i % 8] = (_Float16)e;
+      }
+      l += sum;
+    };
+    const auto add = [&](int n, const half8 (&p)[2]) {
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const half8 v = *reinterpret_cast<const half8*>(
+              buf + kBuf / 2 + (((n * (D / 32) + i) * 2 + u) * kWave + lane) * 16);
+          acc[i] = mfma32x32x16(v, p[u], acc[i]);
+        }
+    };
+    __builtin_amdgcn_s_setprio(3);
+    weights(0);
+    if constexpr (NG == 2) {
+      const half8 p0[2] = {p[0], p[1]};
+      add(0, p0);
+      weights(1);
+    }
+    add(NG - 1, p);
+    __builtin_amdgcn_s_setprio(0);
+    stage(out, next);
+  };
+
+  if (begin < end) {
+    // (past the end the last group is loaded again, and masked)
+    constexpr int kStride = G * NG;
+    const int turns = (end - begin + kStride - 1) / kStride;
+    int g = begin + gang * NG;
+    Ahead x0, x1;
+    look(g);
+    load(x0);
+    look(g + kStride);
+    load(x1);
+    look(g + 2 * kStride);
+    stage(bufs, x0);
+    __syncthreads();
+    const auto turn = [&](Ahead& now, Ahead& next, const uint8_t* in, uint8_t* out, int g) {
+      bool ok[NG];
+#pragma unroll
+      for (int n = 0; n < NG; ++n) ok[n] = now.ok[n];
+      load(now);
+      look(g + 3 * kStride);
+      step(in, g, ok, out, next);
+      __syncthreads();
+    };
+    for (int i = 0; i < turns; i += 2, g += 2 * kStride) {
+      turn(x0, x1, bufs, bufs + kBuf, g);
+      if (i + 1 < turns) turn(x1, x0, bufs + kBuf, bufs, g + kStride);
+    }
+  }
+
+  if constexpr (G == 2) {  // the second gang's sums join the first's, lane by lane
+    float* sums = reinterpret_cast<float*>(lds) + wave * (D / 2) * kWave + lane;
+    float* stats = reinterpret_cast<float*>(lds) + kWaves * (D / 2) * kWave + wave * 2 * kWave + lane;
+    if (gang == 1) {
+#pragma unroll
+      for (int i = 0; i < D / 2; ++i) sums[i * kWave] = acc[i / 16][i % 16];
+      stats[0] = m;
+      stats[kWave] = l;
+    }
+    __syncthreads();
+    if (gang == 0) {
+      const float om = stats[0], top = fmaxf(m, om), f = exp2_fast(m - top), of = exp2_fast(om - top);
+#pragma unroll
+      for (int i = 0; i < D / 2; ++i) acc[i / 16][i % 16] = acc[i / 16][i % 16] * f + sums[i * kWave] * of;
+      m = top;
+      l = l * f + stats[kWave] * of;
+    }
+    __syncthreads();  // the rows go out through the same memory
+    if (gang == 1) return;
+  }
+
+  // Rows go out through LDS (each wavefront its own part, free after the last
+  // barrier), 64 dimensions at a time: straight from the registers every lane
+  // would store four values of another row.
+  constexpr int kPitch = 64 + 4;
+  float* mine = reinterpret_cast<float*>(lds) + wave * 32 * kPitch;
+  l += __shfl_xor(l, 32);
+  const int left = rows - wrow;  // rows of this wavefront's tile
+  const float f = partial ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+  for (int i = 0; i < D / 32; i += 2) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {  // dimensions 32 (j / 4) + 16 lh + 4 (j % 4) + ..
+      floatx4 o;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) o[b] = acc[i + j / 4][4 * b + j % 4] * f;
+      *reinterpret_cast<floatx4*>(mine + col * kPitch + 32 * (j / 4) + 16 * lh + 4 * (j % 4)) = o;
+    }
+    const int d = lane % 8 * 8;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int rr = 8 * n + lane / 8;
+      if (rr >= left) continue;
+      const float* src = mine + rr * kPitch + d;
+      const floatx4 x = *reinterpret_cast<const floatx4*>(src);
+      const floatx4 y = *reinterpret_cast<const floatx4*>(src + 4);
+      const int64_t to = out_row(a, t, h, wrow + rr);
+      if (partial) {
+        float* part = a.part + (to * a.splits + split) * D + 32 * i + d;
+        *reinterpret_cast<floatx4*>(part) = x;
+        *reinterpret_cast<floatx4*>(part + 4) = y;
+      } else {
+        Eight<T>::store(a.out + (to * D + 32 * i + d) * 2,
+                        __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+      }
+    }
+  }
+  if (lh == 0 && col < left) {
+    const int64_t to = out_row(a, t, h, wrow + col);
+    if (partial) Partials(a).store_stat((int)to * a.splits + split, m, l);
+    else if (a.lse)
+      a.lse[to] = l == 0.0f ? -__builtin_inff() : (m - kShift + log2_fast(l)) * kLn2;
+  }
+}
+
+template <typename T, int D>
+hipError_t launch_sized(AttnArgs a, const PagedPlan& p, hipStream_t stream) {
+  constexpr size_t kLds = D == 64 ? kWaves * 32 * 68 * 4
+                                  : 2 * (D <= 128 ? 2 : 1) * 32 * D * 2 * 2 + (D > 128 ? 128 * D * 2 : 0);
+  constexpr size_t kLds2 = 4 * 2 * 32 * D * 2 * 2;
+  // (no workgroup waits for another, so those of one tile may be in two launches)
+  const int64_t most = kMaxThreads / (p.gangs * kThreads);
+  for (int64_t i = 0; i < p.grid; i += most) {
+    a.first = (unsigned)i;
+    const unsigned grid = (unsigned)(p.grid - i < most ? p.grid - i : most);
+    if (p.kernel == 1 && p.gangs == 1) kv4_prefill_kernel<T, D, 1><<<grid, kThreads, kLds, stream>>>(a);
+    else if (p.kernel == 0 && p.rows == 16) kv4_decode_kernel<T, D, 1><<<grid, kThreads, 0, stream>>>(a);
+    else if constexpr (D <= 128) {
+      if (p.kernel == 1) kv4_prefill_kernel<T, D, 2><<<grid, 2 * kThreads, kLds2, stream>>>(a);
+      else kv4_decode_kernel<T, D, 2><<<grid, kThreads, 0, stream>>>(a);
+    }
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  if (!a.merge) return hipSuccess;
+  merge_splits_kernel<T, D>
+      <<<(unsigned)ceil_div((int64_t)a.tokens * a.hq * (D / 4), kThreads), kThreads, 0, stream>>>(a);
+  return hipGetLastError();
+}
+
+struct Kv4Costs {
+  static double base(bool prefill, int rows, int D) {
+    return prefill ? (D == 64 ? 1.1 : D == 128 ? 1.5 : 1.35)
+                   : D == 256 ? 1.1 : (rows == 16 ? 0.55 : 0.85) * (D == 64 ? 0.75 : 1.0);
+  }
+  static double more(bool prefill, int rows, int D) {
+    return prefill ? (D == 256 ? 0.6 : 0.4) : D == 256 ? 1.2 : (rows == 16 ? 0.25 : 0.58) * (D == 64 ? 0.6 : 1.0);
+  }
+  static double slots(bool prefill, int gangs, int rows, int D) {
+    return gangs == 2 ? 1.0 : prefill || D == 256 || rows > 16 ? 2.0 : 3.0;
+  }
+  static double token_bytes(int D) { return D + 4.0; }
+  static int share_least(int rows, int D) { return rows == 32 ? 32 : D == 256 ? 8 : 16; }
+};
+
+}  // namespace
+
+PagedPlan plan_kv4_attention(const rf_kv4_attention_args& a, int cus) {
+  return plan_paged_attention<Kv4Costs>(shape_of(a), cus);
+}
+
+hipError_t launch_kv4_attention(const rf_kv4_attention_args& in, const PagedPlan& p, hipStream_t stream) {
+  AttnArgs a;
+  fill_paged(a, in, p);
+  a.rows = in.cache.rows;
+  const int D = in.cache.head_dim;
+  const bool f16 = in.dtype == RF_W8A16_DTYPE_F16;
+  if (D == 64)
+    return f16 ? launch_sized<_Float16, 64>(a, p, stream) : launch_sized<__bf16, 64>(a, p, stream);
+  if (D == 128)
+    return f16 ? launch_sized<_Float16, 128>(a, p, stream) : launch_sized<__bf16, 128>(a, p, stream);
+  return f16 ? launch_sized<_Float16, 256>(a, p, stream) : launch_sized<__bf16, 256>(a, p, stream);
+}
+
+}  // namespace rf

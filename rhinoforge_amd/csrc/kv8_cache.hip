@@ -29,6 +29,9 @@ struct RopeArgs {
   int turns;           // of kHeads heads each, per wavefront
   int q_parts, parts;  // wavefronts of one token: for q, for both
   float eps;
+  int64_t pos_stride;  // several axes: positions between axes
+  int axes, mixed;
+  int upto[RF_KV8_MAX_AXES];  // mixed: pairs below which i % axes is the axis; else the axis' end
 };
 
 // Sum over the LP lanes of a head, in all of them.
@@ -51,7 +54,8 @@ __device__ __forceinline__ float sum_lanes(float v) {
 // selects that it takes would cost a wavefront per SIMD (27.8 -> 29.3 us), and here
 // fewer loads ahead pay for them (half of 128 rotated, 4001 tokens, 64 + 8 heads:
 // 31.5 us with four, 30.0 with two; interleaved 31.7, 30.8 with three).
-template <typename T, int LP, bool kInterleaved, bool kPart>
+// kAxes: positions of several axes, one of which turns each pair.
+template <typename T, int LP, bool kInterleaved, bool kPart, bool kAxes>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeArgs a) {
   constexpr int kHeads = kWave / LP, kAhead = !kPart ? 4 : kInterleaved ? 3 : 2;
   typedef T tx4 __attribute__((ext_vector_type(4)));
@@ -88,7 +92,43 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeArgs a) {
   }
 
   floatx4 ca = 1.0f, sa = 0.0f, cb = 1.0f, sb = 0.0f;  // (halves as pairs: ca and sa only)
-  if (a.rot > 0) {
+  if constexpr (kAxes) {
+    bool ok = true;
+    int64_t rows[RF_KV8_MAX_AXES];
+#pragma unroll
+    for (int x = 0; x < RF_KV8_MAX_AXES; ++x) {
+      const int64_t at = (x < a.axes ? x : 0) * a.pos_stride + t;
+      const int64_t row = a.pos64 ? reinterpret_cast<const int64_t*>(a.pos)[at]
+                                  : reinterpret_cast<const int32_t*>(a.pos)[at];
+      const bool in = row >= 0 && row < a.table_rows;
+      ok = ok && in;
+      rows[x] = (in ? row : 0) * (a.rot / 2);
+    }
+    const auto at = [&](int pair) {
+      const int turn = (int)((unsigned)pair % (unsigned)a.axes);
+      int64_t row = rows[0];
+#pragma unroll
+      for (int x = 1; x < RF_KV8_MAX_AXES; ++x)
+        if (a.mixed ? turn == x && pair < a.upto[x] : x < a.axes && pair >= a.upto[x - 1]) row = rows[x];
+      return row + pair;
+    };
+    if (turned) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (kInterleaved && i % 2) {
+          ca[i] = ca[i - 1], sa[i] = sa[i - 1], cb[i] = cb[i - 1], sb[i] = sb[i - 1];
+          continue;
+        }
+        const int64_t p = at(kInterleaved ? a0 / 2 + i / 2 : a0 + i);
+        ca[i] = a.cos[p], sa[i] = a.sin[p];
+        if (kInterleaved) {
+          const int64_t r = at(b0 / 2 + i / 2);
+          cb[i] = a.cos[r], sb[i] = a.sin[r];
+        }
+      }
+    }
+    if (!ok) ca = cb = __builtin_nanf("");
+  } else if (a.rot > 0) {
     const int64_t row = a.pos == nullptr ? t
                         : a.pos64        ? reinterpret_cast<const int64_t*>(a.pos)[t]
                                          : reinterpret_cast<const int32_t*>(a.pos)[t];
@@ -720,22 +760,22 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(ReadArgs a) {
 
 inline int log2i(int v) { return __builtin_ctz((unsigned)v); }
 
-template <typename T, int LP>
+template <typename T, int LP, bool kAxes>
 hipError_t rope_sized(const RopeArgs& r, bool interleaved, unsigned grid, hipStream_t stream) {
   const bool part = r.rot < r.D;
-  if (interleaved && part) qk_norm_rope_kernel<T, LP, true, true><<<grid, 256, 0, stream>>>(r);
-  else if (interleaved) qk_norm_rope_kernel<T, LP, true, false><<<grid, 256, 0, stream>>>(r);
-  else if (part) qk_norm_rope_kernel<T, LP, false, true><<<grid, 256, 0, stream>>>(r);
-  else qk_norm_rope_kernel<T, LP, false, false><<<grid, 256, 0, stream>>>(r);
+  if (interleaved && part) qk_norm_rope_kernel<T, LP, true, true, kAxes><<<grid, 256, 0, stream>>>(r);
+  else if (interleaved) qk_norm_rope_kernel<T, LP, true, false, kAxes><<<grid, 256, 0, stream>>>(r);
+  else if (part) qk_norm_rope_kernel<T, LP, false, true, kAxes><<<grid, 256, 0, stream>>>(r);
+  else qk_norm_rope_kernel<T, LP, false, false, kAxes><<<grid, 256, 0, stream>>>(r);
   return hipGetLastError();
 }
 
-template <typename T>
+template <typename T, bool kAxes>
 hipError_t rope_typed(const RopeArgs& r, bool interleaved, unsigned grid, hipStream_t stream) {
-  return r.D <= 64    ? rope_sized<T, 8>(r, interleaved, grid, stream)
-         : r.D <= 128 ? rope_sized<T, 16>(r, interleaved, grid, stream)
-         : r.D <= 256 ? rope_sized<T, 32>(r, interleaved, grid, stream)
-                      : rope_sized<T, 64>(r, interleaved, grid, stream);
+  return r.D <= 64    ? rope_sized<T, 8, kAxes>(r, interleaved, grid, stream)
+         : r.D <= 128 ? rope_sized<T, 16, kAxes>(r, interleaved, grid, stream)
+         : r.D <= 256 ? rope_sized<T, 32, kAxes>(r, interleaved, grid, stream)
+                      : rope_sized<T, 64, kAxes>(r, interleaved, grid, stream);
 }
 
 template <typename T, int D>
@@ -782,8 +822,18 @@ hipError_t read_typed(ReadArgs a, int D, hipStream_t stream) {
 
 }  // namespace
 
-hipError_t launch_qk_norm_rope(const rf_kv8_rope_args& a, hipStream_t stream) {
-  RopeArgs r;
+hipError_t launch_qk_norm_rope(const rf_kv8_rope_args& a, const rf_kv8_mrope_args* m, hipStream_t stream) {
+  RopeArgs r{};
+  if (m) {
+    r.pos_stride = m->axis_stride;
+    r.axes = m->axes;
+    r.mixed = m->mixed;
+    for (int i = 0, end = 0; i < m->axes; ++i) {
+      end += m->sections[i];
+      r.upto[i] = m->mixed ? m->axes * m->sections[i] : end;
+    }
+  }
+  const bool f16 = a.dtype == RF_W8A16_DTYPE_F16;
   r.q_ts = a.q.token_stride * 2;
   r.q_hs = a.q.head_stride * 2;
   r.k_ts = a.k.token_stride * 2;
@@ -825,8 +875,10 @@ hipError_t launch_qk_norm_rope(const rf_kv8_rope_args& a, hipStream_t stream) {
       r.table_rows = a.table_rows - t;
     }
     const unsigned grid = (unsigned)ceil_div((int64_t)r.tokens * r.parts, 256 / kWave);
-    const hipError_t e = a.dtype == RF_W8A16_DTYPE_F16 ? rope_typed<_Float16>(r, a.interleaved, grid, stream)
-                                                       : rope_typed<__bf16>(r, a.interleaved, grid, stream);
+    const hipError_t e = m && f16 ? rope_typed<_Float16, true>(r, a.interleaved, grid, stream)
+                         : m      ? rope_typed<__bf16, true>(r, a.interleaved, grid, stream)
+                         : f16    ? rope_typed<_Float16, false>(r, a.interleaved, grid, stream)
+                                  : rope_typed<__bf16, false>(r, a.interleaved, grid, stream);
     if (e != hipSuccess) return e;
   }
   return hipSuccess;

@@ -1,77 +1,23 @@
 // C-ABI layer of the int8 paged cache (kv8.h): every refusal happens here,
 // before any launch.
-#include "kv8_common.h"
+#include "paged_check.h"
 
 namespace rf {
 namespace {
 
-constexpr int64_t kMaxSize = (int64_t)1 << 30;  // tokens, requests, slots of one call
-
-bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
-
-int check_device(DeviceInfo* dev) {
-  const int st = device_info(dev);
-  if (st != RF_W8A16_OK) return st;
-  return dev->gfx950 ? RF_W8A16_OK : RF_W8A16_EDEVICE;
-}
-
-bool half_dtype(int dtype) { return dtype == RF_W8A16_DTYPE_F16 || dtype == RF_W8A16_DTYPE_BF16; }
-
-int check_heads(const rf_kv8_heads& h) {
-  if (!h.data || h.heads < 1 || h.heads > 4096) return RF_W8A16_EINVAL;
-  if (!aligned(h.data, 16) || h.token_stride % 8 || h.head_stride % 8) return RF_W8A16_EALIGN;
-  return RF_W8A16_OK;
-}
-
 int check_cache(const rf_kv8_cache& c) {
   if (!c.k || !c.v || !c.k_scale || !c.v_scale) return RF_W8A16_EINVAL;
-  if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256) return RF_W8A16_EINVAL;
-  if (c.block_size != 32 && c.block_size != 64 && c.block_size != 128) return RF_W8A16_EINVAL;
-  if (c.kv_heads < 1 || c.kv_heads > 4096 || c.num_blocks < 1) return RF_W8A16_EINVAL;
-  // slots are int32
-  if (c.num_blocks > 0x7fffffff / c.block_size) return RF_W8A16_EINVAL;
+  if (!sizes_fit(c)) return RF_W8A16_EINVAL;
   if (!aligned(c.k, 16) || !aligned(c.v, 16) || !aligned(c.k_scale, 4) || !aligned(c.v_scale, 4))
     return RF_W8A16_EALIGN;
   return RF_W8A16_OK;
 }
 
 int check_attention(const rf_kv8_attention_args* a) {
-  if (!a) return RF_W8A16_EINVAL;
-  int st = check_cache(a->cache);
-  if (st == RF_W8A16_OK) st = check_heads(a->q);
-  if (st != RF_W8A16_OK) return st;
-  if (!half_dtype(a->dtype) || !a->kv_lens || !a->block_table || !a->out) return RF_W8A16_EINVAL;
-  if (a->q.heads % a->cache.kv_heads) return RF_W8A16_EINVAL;
-  if (a->tokens < 0 || a->tokens > kMaxSize || a->requests < 1 || a->requests > kMaxSize)
-    return RF_W8A16_EINVAL;
-  if (a->tokens * a->q.heads > 0x7fffffff) return RF_W8A16_EINVAL;
-  if (!a->cu_q && a->tokens % a->requests) return RF_W8A16_EINVAL;
-  if (a->width < 1 || a->table_stride < a->width || a->width > kMaxSize / a->cache.block_size)
-    return RF_W8A16_EINVAL;
-  if (!(a->scale > 0.0f) || !(a->scale < __builtin_inff())) return RF_W8A16_EINVAL;
-  if (a->window < 0 || (a->window > 0 && !a->causal)) return RF_W8A16_EINVAL;
-  if (a->max_q_len < 0 || a->max_kv_len < 0) return RF_W8A16_EINVAL;
-  if (!aligned(a->out, 16) || !aligned(a->lse, 4) || !aligned(a->cu_q, 4) ||
-      !aligned(a->kv_lens, 4) || !aligned(a->block_table, 4))
-    return RF_W8A16_EALIGN;
-  return RF_W8A16_OK;
+  return a ? check_paged_attention(a, check_cache(a->cache)) : RF_W8A16_EINVAL;
 }
 
-struct Ints {
-  const int32_t* p;
-  int64_t n;
-};
-
-int status_of(hipError_t e) { return e == hipSuccess ? RF_W8A16_OK : RF_W8A16_EHIP; }
-
-}  // namespace
-}  // namespace rf
-
-using namespace rf;
-
-extern "C" {
-
-int rf_kv8_qk_norm_rope(const rf_kv8_rope_args* a, void* stream) {
+int check_rope(const rf_kv8_rope_args* a) {
   if (!a) return RF_W8A16_EINVAL;
   int st = check_heads(a->q);
   if (st == RF_W8A16_OK) st = check_heads(a->k);
@@ -88,11 +34,50 @@ int rf_kv8_qk_norm_rope(const rf_kv8_rope_args* a, void* stream) {
   if (!aligned(a->q_out, 16) || !aligned(a->k_out, 16) || !aligned(a->q_weight, 16) ||
       !aligned(a->k_weight, 16) || !aligned(a->positions, a->positions64 ? 8 : 4))
     return RF_W8A16_EALIGN;
-  if (a->tokens == 0) return RF_W8A16_OK;
+  return RF_W8A16_OK;
+}
+
+struct Ints {
+  const int32_t* p;
+  int64_t n;
+};
+
+}  // namespace
+}  // namespace rf
+
+using namespace rf;
+
+extern "C" {
+
+int rf_kv8_qk_norm_rope(const rf_kv8_rope_args* a, void* stream) {
+  int st = check_rope(a);
+  if (st != RF_W8A16_OK || a->tokens == 0) return st;
   DeviceInfo dev;
   st = check_device(&dev);
   if (st != RF_W8A16_OK) return st;
-  return status_of(launch_qk_norm_rope(*a, static_cast<hipStream_t>(stream)));
+  return status_of(launch_qk_norm_rope(*a, nullptr, static_cast<hipStream_t>(stream)));
+}
+
+int rf_kv8_qk_norm_mrope(const rf_kv8_mrope_args* a, void* stream) {
+  if (!a) return RF_W8A16_EINVAL;
+  int st = check_rope(&a->rope);
+  if (st != RF_W8A16_OK) return st;
+  if (a->rope.rot < 1 || !a->rope.positions || a->axes < 1 || a->axes > RF_KV8_MAX_AXES) return RF_W8A16_EINVAL;
+  if (a->axis_stride < a->rope.tokens) return RF_W8A16_EINVAL;
+  int64_t pairs = 0;
+  for (int i = 0; i < a->axes; ++i) {
+    if (a->sections[i] < 0 || a->sections[i] > a->rope.rot / 2) return RF_W8A16_EINVAL;
+    pairs += a->sections[i];
+    // (mixed: the last pair of axis i is axes * (section - 1) + i)
+    if (a->mixed && i > 0 && a->sections[i] > 0 && a->axes * (a->sections[i] - 1) + i >= a->rope.rot / 2)
+      return RF_W8A16_EINVAL;
+  }
+  if (pairs != a->rope.rot / 2) return RF_W8A16_EINVAL;
+  if (a->rope.tokens == 0) return RF_W8A16_OK;
+  DeviceInfo dev;
+  st = check_device(&dev);
+  if (st != RF_W8A16_OK) return st;
+  return status_of(launch_qk_norm_rope(a->rope, a, static_cast<hipStream_t>(stream)));
 }
 
 int rf_kv8_plan(const rf_kv8_plan_args* a, void* stream) {
@@ -172,7 +157,7 @@ int rf_kv8_attention(const rf_kv8_attention_args* a, void* stream) {
   DeviceInfo dev;
   st = check_device(&dev);
   if (st != RF_W8A16_OK) return st;
-  const Kv8AttnPlan p = plan_kv8_attention(*a, dev.cus);
+  const PagedPlan p = plan_kv8_attention(*a, dev.cus);
   if (p.workspace > 0) {
     const rf_w8a16_scratch* w = a->scratch;
     if (!w || !w->counters || !w->partials || w->partial_bytes < p.workspace) return RF_W8A16_EWORKSPACE;

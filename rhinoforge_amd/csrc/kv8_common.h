@@ -44,7 +44,8 @@ struct Eight<float> {
 constexpr int64_t kMaxThreads = ((int64_t)1 << 32) - 1;
 
 // Validated arguments, as the C ABI passes them on (kv8_capi.hip).
-hipError_t launch_qk_norm_rope(const rf_kv8_rope_args& a, hipStream_t stream);
+// (m: the same call's axes, or null: one axis)
+hipError_t launch_qk_norm_rope(const rf_kv8_rope_args& a, const rf_kv8_mrope_args* m, hipStream_t stream);
 hipError_t launch_kv8_plan(const rf_kv8_plan_args& a, hipStream_t stream);
 hipError_t launch_kv8_append(const rf_kv8_cache& c, const rf_kv8_heads& k, const rf_kv8_heads& v,
                              int dtype, const int32_t* slots, int64_t tokens, hipStream_t stream);
@@ -53,7 +54,7 @@ hipError_t launch_kv8_read(const rf_kv8_cache& c, const int32_t* slots, int64_t 
 
 // How a call of the attention is launched: rows (query, head of the group) of
 // one tile, workgroups over the tokens of one tile, partial results.
-struct Kv8AttnPlan {
+struct PagedPlan {
   int kernel;     // 0: tokens split over the wavefronts (few rows), 1: rows split over them
   int gangs = 1;  // kernel 1: groups of four wavefronts that take a tile's tokens in turn
   int rows;       // rows of a tile
@@ -66,8 +67,8 @@ struct Kv8AttnPlan {
   int64_t partials;  // rows of partial results
   size_t workspace;  // their bytes
 };
-Kv8AttnPlan plan_kv8_attention(const rf_kv8_attention_args& a, int cus);
-hipError_t launch_kv8_attention(const rf_kv8_attention_args& a, const Kv8AttnPlan& p,
+PagedPlan plan_kv8_attention(const rf_kv8_attention_args& a, int cus);
+hipError_t launch_kv8_attention(const rf_kv8_attention_args& a, const PagedPlan& p,
                                 hipStream_t stream);
 
 }  // namespace rf

@@ -11,91 +11,24 @@
 //   attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale,
 //             Tensor block_table, Tensor kv_lens, Tensor? cu_q, int max_q_len, int max_kv_len,
 //             bool causal, int window, float scale, bool return_lse) -> (Tensor, Tensor)
+// and of namespace `rope`, the same norms and rotation by positions of several axes:
+//   qk_norm_mrope(Tensor q, Tensor k, Tensor? q_weight, Tensor? k_weight, Tensor cos, Tensor sin,
+//                 Tensor positions, int[] sections, bool mixed, float eps, bool interleaved)
+//                 -> (Tensor, Tensor)
 // They are what the reference's decoders run between the W8A16 projections
 // (src/fused/rpu_qwen3_model.h: head norms, RoPE, KV insert, SDPA).  Checks in
 // the manner of w8a16_torch.cpp: dtype and shape first (shared with the Meta
 // kernels), then devices; invalid input raises, there is no CPU computation.
-#include <ATen/ATen.h>
-#include <ATen/hip/EmptyTensor.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
-#include <torch/library.h>
-
-#include <vector>
-
-#include "../../include/kv8.h"
-#include "torch_scratch.h"
+#include "paged_torch.h"
 
 namespace {
 
-using OptTensor = c10::optional<at::Tensor>;
-
-bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
-
-void check_status(int st, const char* op) {
-  TORCH_CHECK(st == RF_W8A16_OK, op, ": ", rf_w8a16_status_str(st), " (status ", st, ")");
-}
-
-int32_t dtype_code(at::ScalarType t) {
-  return t == at::kHalf ? RF_W8A16_DTYPE_F16 : t == at::kBFloat16 ? RF_W8A16_DTYPE_BF16 : RF_W8A16_DTYPE_F32;
-}
-
-void check_half(const at::Tensor& t, const char* op, const char* name) {
-  TORCH_CHECK(t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16, op, ": ", name,
-              " must be float16 or bfloat16, got ", t.scalar_type());
-}
-
-void check_ints(const at::Tensor& t, int64_t dim, const char* op, const char* name) {
-  TORCH_CHECK(t.scalar_type() == at::kInt, op, ": ", name, " must be int32, got ", t.scalar_type());
-  TORCH_CHECK(t.dim() == dim, op, ": ", name, " must have ", dim, " dimension(s), got shape ",
-              t.sym_sizes());
-  TORCH_CHECK(dim != 1 || t.is_contiguous(), op, ": ", name, " must be contiguous");
-}
-
-void check_same_device(const at::Tensor& t, const at::Tensor& first, const char* op,
-                       const char* name) {
-  TORCH_CHECK(t.is_cuda(), op, ": ", name,
-              " must be on a HIP device (there is no CPU implementation)");
-  TORCH_CHECK(t.device() == first.device(), op, ": ", name, " must be on ", first.device(), ", got ",
-              t.device());
-}
-
-[[noreturn]] void no_cpu(const char* op) {
-  TORCH_CHECK(false, op, ": tensors are on the CPU; the kernels run on a HIP device (gfx950) only "
-              "and there is no CPU implementation");
-}
-
-void* stream_of(const at::Tensor& t) {
-  return c10::hip::getCurrentHIPStream(t.device().index()).stream();
-}
-
-// A new contiguous tensor, straight from the caching allocator (at::empty's way
-// there through the dispatcher is a third of what a single-token call costs).
-at::Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType dtype, const at::Tensor& like) {
-  return at::detail::empty_cuda(sizes, dtype, like.device(), c10::nullopt);
-}
-
-bool aligned16(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
-
-// A [tokens, heads, D] operand as the C ABI takes it; one of another layout is
-// copied (kept alive in *keep).
-rf_kv8_heads heads_of(const at::Tensor& t, at::Tensor* keep) {
-  const auto fits = [](const at::Tensor& x) {
-    return x.stride(2) == 1 && (x.size(0) <= 1 || x.stride(0) % 8 == 0) &&
-           (x.size(1) <= 1 || x.stride(1) % 8 == 0) && aligned16(x);
-  };
-  *keep = fits(t) ? t : t.is_contiguous() ? t.clone() : t.contiguous();
-  const at::Tensor& x = *keep;
-  return {x.data_ptr(), x.size(0) <= 1 ? x.size(1) * x.size(2) : x.stride(0),
-          x.size(1) <= 1 ? x.size(2) : x.stride(1), (int32_t)x.size(1)};
-}
-
-at::Tensor aligned_copy(const at::Tensor& t) { return aligned16(t) ? t : t.clone(); }
+using namespace rf_torch;
 
 // ---- norms and rotation ----------------------------------------------------------
-void check_rope(const at::Tensor& q, const at::Tensor& k, const OptTensor& qw, const OptTensor& kw,
-                const OptTensor& cos, const OptTensor& sin, const OptTensor& pos) {
-  const char* op = "kv8::qk_norm_rope";
+// All of a call but its positions.
+void check_rope_operands(const char* op, const at::Tensor& q, const at::Tensor& k, const OptTensor& qw,
+                         const OptTensor& kw, const OptTensor& cos, const OptTensor& sin) {
   check_half(q, op, "q");
   TORCH_CHECK(k.scalar_type() == q.scalar_type(), op, ": k must be ", q.scalar_type(), " as q, got ",
               k.scalar_type());
@@ -124,41 +57,44 @@ void check_rope(const at::Tensor& q, const at::Tensor& k, const OptTensor& qw, c
     TORCH_CHECK(rot >= 16 && rot % 16 == 0 && rot <= D, op, ": rotated dimensions ", rot,
                 " must be a multiple of 16 up to head_dim ", D);
     TORCH_CHECK(cos->sym_size(0) >= 1, op, ": cos and sin have no rows");
-    if (given(pos)) {
-      TORCH_CHECK((pos->scalar_type() == at::kInt || pos->scalar_type() == at::kLong) &&
-                      pos->dim() == 1 && pos->sym_size(0) == q.sym_size(0) && pos->is_contiguous(),
-                  op, ": positions must be a contiguous int32 or int64 [tokens]");
-    } else {
-      TORCH_CHECK(cos->sym_size(0) >= q.sym_size(0), op,
-                  ": without positions cos and sin need a row for each token");
-    }
   }
 }
 
-using Two = std::tuple<at::Tensor, at::Tensor>;
-
-Two rope_hip(const at::Tensor& q, const at::Tensor& k, const OptTensor& qw, const OptTensor& kw,
-             const OptTensor& cos, const OptTensor& sin, const OptTensor& pos, double eps,
-             bool interleaved) {
-  RECORD_FUNCTION("kv8::qk_norm_rope", {});
+void check_rope(const at::Tensor& q, const at::Tensor& k, const OptTensor& qw, const OptTensor& kw,
+                const OptTensor& cos, const OptTensor& sin, const OptTensor& pos) {
   const char* op = "kv8::qk_norm_rope";
-  check_rope(q, k, qw, kw, cos, sin, pos);
-  check_same_device(k, q, op, "k");
-  for (const OptTensor* t : {&qw, &kw, &cos, &sin, &pos})
-    if (given(*t)) check_same_device(**t, q, op, "an argument");
-  c10::DeviceGuard dev_guard(q.device());
+  check_rope_operands(op, q, k, qw, kw, cos, sin);
+  if (!given(cos)) return;
+  if (given(pos)) {
+    TORCH_CHECK((pos->scalar_type() == at::kInt || pos->scalar_type() == at::kLong) &&
+                    pos->dim() == 1 && pos->sym_size(0) == q.sym_size(0) && pos->is_contiguous(),
+                op, ": positions must be a contiguous int32 or int64 [tokens]");
+  } else {
+    TORCH_CHECK(cos->sym_size(0) >= q.sym_size(0), op,
+                ": without positions cos and sin need a row for each token");
+  }
+}
+
+// The operands as the C ABI takes them, checked for their devices, and the outputs.
+struct RopeCall {
+  at::Tensor q, k;
   at::Tensor keep[6];
-  rf_kv8_rope_args a{};
-  a.q = heads_of(q, &keep[0]);
-  a.k = heads_of(k, &keep[1]);
-  at::Tensor qo = new_tensor(q.sizes(), q.scalar_type(), q), ko = new_tensor(k.sizes(), k.scalar_type(), k);
-  a.q_out = qo.data_ptr();
-  a.k_out = ko.data_ptr();
-  if (given(qw)) a.q_weight = (keep[2] = aligned_copy(*qw)).data_ptr();
-  if (given(kw)) a.k_weight = (keep[3] = aligned_copy(*kw)).data_ptr();
+};
+
+void fill_rope(RopeCall& c, rf_kv8_rope_args& a, const char* op, const at::Tensor& q, const at::Tensor& k,
+               const OptTensor& qw, const OptTensor& kw, const OptTensor& cos, const OptTensor& sin,
+               const OptTensor& pos, double eps, bool interleaved) {
+  a.q = heads_of(q, &c.keep[0]);
+  a.k = heads_of(k, &c.keep[1]);
+  c.q = new_tensor(q.sizes(), q.scalar_type(), q);
+  c.k = new_tensor(k.sizes(), k.scalar_type(), k);
+  a.q_out = c.q.data_ptr();
+  a.k_out = c.k.data_ptr();
+  if (given(qw)) a.q_weight = (c.keep[2] = aligned_copy(*qw)).data_ptr();
+  if (given(kw)) a.k_weight = (c.keep[3] = aligned_copy(*kw)).data_ptr();
   if (given(cos)) {
-    a.cos = (keep[4] = aligned_copy(*cos)).data_ptr<float>();
-    a.sin = (keep[5] = aligned_copy(*sin)).data_ptr<float>();
+    a.cos = (c.keep[4] = aligned_copy(*cos)).data_ptr<float>();
+    a.sin = (c.keep[5] = aligned_copy(*sin)).data_ptr<float>();
     a.rot = (int32_t)cos->size(1) * 2;
     a.table_rows = cos->size(0);
     if (given(pos)) {
@@ -171,8 +107,23 @@ Two rope_hip(const at::Tensor& q, const at::Tensor& k, const OptTensor& qw, cons
   a.dtype = dtype_code(q.scalar_type());
   a.interleaved = interleaved;
   a.eps = (float)eps;
+}
+
+Two rope_hip(const at::Tensor& q, const at::Tensor& k, const OptTensor& qw, const OptTensor& kw,
+             const OptTensor& cos, const OptTensor& sin, const OptTensor& pos, double eps,
+             bool interleaved) {
+  RECORD_FUNCTION("kv8::qk_norm_rope", {});
+  const char* op = "kv8::qk_norm_rope";
+  check_rope(q, k, qw, kw, cos, sin, pos);
+  check_same_device(k, q, op, "k");
+  for (const OptTensor* t : {&qw, &kw, &cos, &sin, &pos})
+    if (given(*t)) check_same_device(**t, q, op, "an argument");
+  c10::DeviceGuard dev_guard(q.device());
+  RopeCall c;
+  rf_kv8_rope_args a{};
+  fill_rope(c, a, op, q, k, qw, kw, cos, sin, pos, eps, interleaved);
   if (a.tokens > 0) check_status(rf_kv8_qk_norm_rope(&a, stream_of(q)), op);
-  return {qo, ko};
+  return {c.q, c.k};
 }
 
 Two rope_meta(const at::Tensor& q, const at::Tensor& k, const OptTensor& qw, const OptTensor& kw,
@@ -185,6 +136,71 @@ Two rope_cpu(const at::Tensor& q, const at::Tensor& k, const OptTensor& qw, cons
              const OptTensor& cos, const OptTensor& sin, const OptTensor& pos, double, bool) {
   check_rope(q, k, qw, kw, cos, sin, pos);
   no_cpu("kv8::qk_norm_rope");
+}
+
+// Several axes: positions [axes, tokens]; sections: pairs of each.
+void check_mrope(const at::Tensor& q, const at::Tensor& k, const OptTensor& qw, const OptTensor& kw,
+                 const at::Tensor& cos, const at::Tensor& sin, const at::Tensor& pos,
+                 at::IntArrayRef sections, bool mixed) {
+  const char* op = "rope::qk_norm_mrope";
+  check_rope_operands(op, q, k, qw, kw, cos, sin);
+  const int64_t axes = (int64_t)sections.size();
+  TORCH_CHECK(axes >= 1 && axes <= RF_KV8_MAX_AXES, op, ": between 1 and ", RF_KV8_MAX_AXES,
+              " sections, got ", axes);
+  TORCH_CHECK((pos.scalar_type() == at::kInt || pos.scalar_type() == at::kLong) && pos.dim() == 2 &&
+                  pos.sym_size(0) == axes && pos.sym_size(1) == q.sym_size(0),
+              op, ": positions must be int32 or int64 [", axes, " axes, ", q.sym_size(0), " tokens], got ",
+              pos.scalar_type(), " ", pos.sym_sizes());
+  const c10::SymInt pairs = cos.sym_size(1);
+  c10::SymInt sum = 0;
+  for (const int64_t n : sections) TORCH_CHECK(n >= 0, op, ": sections must not be negative, got ", sections);
+  for (int64_t i = 0; i < axes; ++i) {
+    TORCH_CHECK(pairs >= sections[i], op, ": sections ", sections, " must add up to the ", pairs,
+                " pairs of cos and sin");
+    sum += sections[i];
+  }
+  TORCH_CHECK(sum == pairs, op, ": sections ", sections, " must add up to the ", pairs, " pairs of cos and sin");
+  for (int64_t i = 1; i < axes; ++i)
+    TORCH_CHECK(!mixed || sections[i] == 0 || pairs > axes * (sections[i] - 1) + i, op, ": sections ", sections,
+                " cannot be mixed, axis ", i, " has more pairs than places");
+}
+
+Two mrope_hip(const at::Tensor& q, const at::Tensor& k, const OptTensor& qw, const OptTensor& kw,
+              const at::Tensor& cos, const at::Tensor& sin, const at::Tensor& pos,
+              at::IntArrayRef sections, bool mixed, double eps, bool interleaved) {
+  RECORD_FUNCTION("rope::qk_norm_mrope", {});
+  const char* op = "rope::qk_norm_mrope";
+  check_mrope(q, k, qw, kw, cos, sin, pos, sections, mixed);
+  check_same_device(k, q, op, "k");
+  for (const OptTensor* t : {&qw, &kw})
+    if (given(*t)) check_same_device(**t, q, op, "a norm weight");
+  for (const at::Tensor* t : {&cos, &sin, &pos}) check_same_device(*t, q, op, "an argument");
+  c10::DeviceGuard dev_guard(q.device());
+  const bool rows = (pos.size(1) <= 1 || pos.stride(1) == 1) && (pos.size(0) <= 1 || pos.stride(0) >= pos.size(1));
+  const at::Tensor p = rows ? pos : pos.contiguous();
+  RopeCall c;
+  rf_kv8_mrope_args a{};
+  fill_rope(c, a.rope, op, q, k, qw, kw, cos, sin, p, eps, interleaved);
+  a.axes = (int32_t)sections.size();
+  a.axis_stride = a.axes == 1 ? a.rope.tokens : p.stride(0);
+  a.mixed = mixed;
+  for (int i = 0; i < a.axes; ++i) a.sections[i] = (int32_t)sections[i];
+  if (a.rope.tokens > 0) check_status(rf_kv8_qk_norm_mrope(&a, stream_of(q)), op);
+  return {c.q, c.k};
+}
+
+Two mrope_meta(const at::Tensor& q, const at::Tensor& k, const OptTensor& qw, const OptTensor& kw,
+               const at::Tensor& cos, const at::Tensor& sin, const at::Tensor& pos,
+               at::IntArrayRef sections, bool mixed, double, bool) {
+  check_mrope(q, k, qw, kw, cos, sin, pos, sections, mixed);
+  return {at::empty_symint(q.sym_sizes(), q.options()), at::empty_symint(k.sym_sizes(), k.options())};
+}
+
+Two mrope_cpu(const at::Tensor& q, const at::Tensor& k, const OptTensor& qw, const OptTensor& kw,
+              const at::Tensor& cos, const at::Tensor& sin, const at::Tensor& pos,
+              at::IntArrayRef sections, bool mixed, double, bool) {
+  check_mrope(q, k, qw, kw, cos, sin, pos, sections, mixed);
+  no_cpu("rope::qk_norm_mrope");
 }
 
 // ---- block tables and slots ------------------------------------------------------
@@ -388,30 +404,8 @@ void check_attention(const at::Tensor& q, const at::Tensor& kc, const at::Tensor
   const char* op = "kv8::attention";
   check_half(q, op, "q");
   check_cache(kc, vc, ks, vs, op);
-  check_ints(table, 2, op, "block_table");
-  check_ints(lens, 1, op, "kv_lens");
-  TORCH_CHECK(q.dim() == 3 && q.sym_size(2) == kc.sym_size(3) * 32, op,
-              ": q must be [tokens, heads, ", kc.sym_size(3) * 32, "], got ", q.sym_sizes());
-  TORCH_CHECK(q.sym_size(1) >= 1 && q.sym_size(1) % kc.sym_size(1) == 0, op, ": q's heads ",
-              q.sym_size(1), " must be a multiple of the cache's ", kc.sym_size(1));
-  const c10::SymInt B = lens.sym_size(0);
-  TORCH_CHECK(B >= 1 && table.sym_size(0) == B, op, ": block_table and kv_lens differ in requests");
-  TORCH_CHECK(table.sym_size(1) >= 1 && table.sym_stride(1) == 1 &&
-                  (B <= 1 || table.sym_stride(0) >= table.sym_size(1)),
-              op, ": block_table must have rows of unit stride, one after the other");
-  if (given(cu)) {
-    check_ints(*cu, 1, op, "cu_q");
-    TORCH_CHECK(cu->sym_size(0) == B + 1, op, ": cu_q must have ", B + 1, " elements, got ",
-                cu->sym_size(0));
-  } else {
-    TORCH_CHECK(q.sym_size(0) % B == 0, op, ": without cu_q the tokens (", q.sym_size(0),
-                ") must be a multiple of the requests (", B, ")");
-  }
-  TORCH_CHECK(scale > 0 && (float)scale < std::numeric_limits<float>::infinity() && (float)scale > 0,
-              op, ": scale must be positive and finite, got ", scale);
-  TORCH_CHECK(window >= 0 && (window == 0 || causal), op,
-              ": window must be 0 (none), or positive with causal");
-  TORCH_CHECK(max_q >= 0 && max_kv >= 0, op, ": max_q_len and max_kv_len must not be negative");
+  rf_torch::check_attention(op, q, kc.sym_size(1), kc.sym_size(3) * 32, table, lens, cu, max_q, max_kv, causal,
+                            window, scale);
 }
 
 Two attention_hip(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc,
@@ -425,40 +419,8 @@ Two attention_hip(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& v
   rf_kv8_attention_args a{};
   a.cache = cache_of(kc, vc, ks, vs, op);
   check_same_device(kc, q, op, "k_cache");
-  check_same_device(table, q, op, "block_table");
-  check_same_device(lens, q, op, "kv_lens");
-  if (given(cu)) check_same_device(*cu, q, op, "cu_q");
-  c10::DeviceGuard dev_guard(q.device());
-  at::Tensor out = new_tensor(q.sizes(), q.scalar_type(), q);
-  at::Tensor lse = return_lse ? new_tensor({q.size(0), q.size(1)}, at::kFloat, q) : new_tensor({0}, at::kFloat, q);
-  if (q.size(0) == 0) return {out, lse};
-  at::Tensor keep;
-  a.q = heads_of(q, &keep);
-  if (given(cu)) a.cu_q = cu->data_ptr<int32_t>();
-  a.kv_lens = lens.data_ptr<int32_t>();
-  a.block_table = table.data_ptr<int32_t>();
-  a.out = out.data_ptr();
-  a.lse = return_lse ? lse.data_ptr<float>() : nullptr;
-  a.tokens = q.size(0);
-  a.requests = lens.size(0);
-  a.width = table.size(1);
-  a.table_stride = a.requests <= 1 ? a.width : table.stride(0);
-  a.max_q_len = max_q;
-  a.max_kv_len = max_kv;
-  a.dtype = dtype_code(q.scalar_type());
-  a.causal = causal;
-  a.window = window;
-  a.scale = (float)scale;
-  void* stream = stream_of(q);
-  const int st = rf_torch::with_scratch(
-      q.device(), stream, op,
-      [&](const rf_w8a16_scratch* scratch) {
-        a.scratch = scratch;
-        return rf_kv8_attention(&a, stream);
-      },
-      [&] { return rf_kv8_attention_workspace(&a) + RF_W8A16_WS_COUNTER_BYTES; });
-  check_status(st, op);
-  return {out, lse};
+  return run_attention(op, a, rf_kv8_attention, rf_kv8_attention_workspace, q, table, lens, cu, max_q, max_kv,
+                       causal, window, scale, return_lse);
 }
 
 Two attention_meta(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc,
@@ -466,9 +428,7 @@ Two attention_meta(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& 
                    const at::Tensor& lens, const OptTensor& cu, int64_t max_q, int64_t max_kv,
                    bool causal, int64_t window, double scale, bool return_lse) {
   check_attention(q, kc, vc, ks, vs, table, lens, cu, max_q, max_kv, causal, window, scale);
-  const auto o = q.options().dtype(at::kFloat);
-  return {at::empty_symint(q.sym_sizes(), q.options()),
-          return_lse ? at::empty_symint({q.sym_size(0), q.sym_size(1)}, o) : at::empty({0}, o)};
+  return attention_outputs(q, return_lse);
 }
 
 Two attention_cpu(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc,
@@ -522,3 +482,15 @@ TORCH_LIBRARY_IMPL(kv8, Autograd, m) {
   for (const char* op : {"qk_norm_rope", "plan", "append", "read", "attention"})
     m.impl(op, torch::CppFunction::makeFallthrough());
 }
+
+// Norms and rotation do not depend on the cache: the forms for several axes have a
+// namespace of their own.
+TORCH_LIBRARY(rope, m) {
+  m.def("qk_norm_mrope(Tensor q, Tensor k, Tensor? q_weight, Tensor? k_weight, Tensor cos, "
+        "Tensor sin, Tensor positions, int[] sections, bool mixed, float eps, bool interleaved) "
+        "-> (Tensor, Tensor)");
+}
+TORCH_LIBRARY_IMPL(rope, CUDA, m) { m.impl("qk_norm_mrope", TORCH_FN(mrope_hip)); }
+TORCH_LIBRARY_IMPL(rope, Meta, m) { m.impl("qk_norm_mrope", TORCH_FN(mrope_meta)); }
+TORCH_LIBRARY_IMPL(rope, CPU, m) { m.impl("qk_norm_mrope", TORCH_FN(mrope_cpu)); }
+TORCH_LIBRARY_IMPL(rope, Autograd, m) { m.impl("qk_norm_mrope", torch::CppFunction::makeFallthrough()); }

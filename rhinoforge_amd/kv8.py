@@ -1,11 +1,13 @@
 """Attention over an int8 paged cache: what a decoder layer does between its
-q/k/v projections and its o projection (``torch.ops.kv8``, csrc/kv8_*).
+q/k/v projections and its o projection (``torch.ops.kv8``, ``torch.ops.rope``,
+csrc/kv8_*).
 
 The reference runs these steps inside its fused decoder (head norms, RoPE, KV
 insert, SDPA: src/fused/rpu_qwen3_model.h:3310-3517).  Here they are five ops
 that share one cache:
 
-* :func:`qk_norm_rope`   head norms and position rotation of q and k, one launch;
+* :func:`qk_norm_rope`   head norms and position rotation of q and k, one launch
+  (:func:`qk_norm_mrope`: by positions of several axes);
 * :func:`kv8_plan`       block tables, slots and positions from request lengths;
 * :func:`kv8_append`     quantizes new keys and values into the cache;
 * :func:`kv8_attention`  ragged batches of single tokens, drafted tokens or prompts;
@@ -16,13 +18,14 @@ captured into a graph.
 """
 from __future__ import annotations
 
-from typing import NamedTuple
+from typing import NamedTuple, Sequence
 
 import torch
 
 # (resolved once: single-token calls are bound by the host)
 _ops = torch.ops.kv8
-_qk_norm_rope, _plan, _append = _ops.qk_norm_rope.default, _ops.plan.default, _ops.append.default
+_qk_norm_rope, _qk_norm_mrope = _ops.qk_norm_rope.default, torch.ops.rope.qk_norm_mrope.default
+_plan, _append = _ops.plan.default, _ops.append.default
 _read, _attention = _ops.read.default, _ops.attention.default
 
 GROUP = 32          # tokens of one group of tiles
@@ -125,6 +128,11 @@ class KV8Cache:
         """:func:`kv8_read` from this cache."""
         return kv8_read(self, slots, dtype)
 
+    def attention(self, q: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor,
+                  cu_q: torch.Tensor | None = None, **kw):
+        """:func:`kv8_attention` over this cache."""
+        return kv8_attention(q, self, block_table, kv_lens, cu_q, **kw)
+
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None,
                  k_weight: torch.Tensor | None, cos: torch.Tensor | None, sin: torch.Tensor | None,
@@ -142,6 +150,23 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
     fp32 throughout, one rounding.  Returns new contiguous (q, k).
     """
     return _qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+
+
+def qk_norm_mrope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None,
+                  k_weight: torch.Tensor | None, cos: torch.Tensor, sin: torch.Tensor,
+                  positions: torch.Tensor, sections: Sequence[int], *, mixed: bool = False,
+                  eps: float = 1e-6, interleaved: bool = False):
+    """:func:`qk_norm_rope` with positions of several axes (images and video: time,
+    height, width).
+
+    positions [axes, tokens], int32 or int64, up to four axes; sections: how many of
+    the rot / 2 pairs each axis turns.  Pair i of token t uses column i of row
+    ``positions[axis(i), t]``: without ``mixed`` the axes' pairs follow each other,
+    with it they take turns (pair i belongs to axis i % axes while i // axes is below
+    that axis' section, and to axis 0 from there on).  A position of any axis outside
+    the table gives NaN.
+    """
+    return _qk_norm_mrope(q, k, q_weight, k_weight, cos, sin, positions, sections, mixed, eps, interleaved)
 
 
 def rope_table(inv_freq: torch.Tensor, rows: int):
