@@ -50,45 +50,158 @@ __device__ __forceinline__ half2v less(uint32_t v, uint32_t z) { return as_half2
 // ---------------------------------------------------------------------------
 // Few rows (single tokens, a few drafted ones): RT tiles of 16 rows, held by
 // all four wavefronts; the wavefronts take 32-token groups in turn and read the
-// cache straight into MFMA operands (no LDS), kAhead turns ahead of the products.
-// At the end the wavefronts' sums meet in LDS.
+// cache straight into MFMA operands (no LDS), one turn ahead of the products.  At
+// the end the wavefronts' sums meet in LDS.
+//
+// A product has 16 columns, and a single token of a model with four query heads to
+// a key head fills four of them.  W = 2, 4: tiles of 16 / W rows, each of which has
+// W columns; of the eight scores that a lane has of its row it takes N = 8 / W on,
+// and the weights meet in the first of the columns.
 // ---------------------------------------------------------------------------
-template <int D>
-struct Bytes {
-  uint4 k[D / 64], v[D / 64];
-  uint4 kw, vw;  // words of this lane's eight tokens
+// Loads of one group: its place in scalar registers, 32 bits of each lane.  (As
+// plain pointers the addresses were summed in vector registers that loads under way
+// may be writing, and waited for them.)
+struct Base {
+  static constexpr int kStream = 2;  // nt: read once
+  __amdgpu_buffer_rsrc_t p;
+  __device__ __forceinline__ Base(const void* q, int bytes)
+      : p(__builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(q), 0, bytes, 0x00027000)) {}
+  __device__ __forceinline__ uint4 stream16(int at, int more) const {
+    return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(p, at, more, kStream));
+  }
+  template <int kBytes>
+  __device__ __forceinline__ auto load(int at, int more) const {
+    if constexpr (kBytes == 4) return __builtin_amdgcn_raw_buffer_load_b32(p, at, more, 0);
+    else if constexpr (kBytes == 8) return __builtin_amdgcn_raw_buffer_load_b64(p, at, more, 0);
+    else return __builtin_amdgcn_raw_buffer_load_b128(p, at, more, 0);
+  }
 };
 
-template <int D>
-__device__ __forceinline__ void fetch(const AttnArgs& a, const Group& g, int lane, Bytes<D>& b) {
+template <int N>
+struct Words {  // of N tokens, two of 16 bits each
+  typedef uint32_t vec __attribute__((ext_vector_type(N / 2)));
+  vec w;
+  __device__ __forceinline__ void load(const Base& b, int at, int more) {
+    w = __builtin_bit_cast(vec, b.load<2 * N>(at, more));
+  }
+  __device__ __forceinline__ uint32_t at(int i) const { return w[i]; }
+};
+
+template <int D, int N>
+struct Bytes {
+  uint4 k[D / 64], v[D / 64];
+  Words<N> kw, vs;  // of the tokens whose scores the lane takes on
+  Words<8> vw;      // of its eight tokens
+};
+
+template <int D, int N>
+__device__ __forceinline__ void fetch(const AttnArgs& a, const Group& g, int lane, Bytes<D, N>& b) {
   const int64_t group = (g.at << (a.shift - 5)) + g.sub;
-  const uint8_t* kp = a.k + group * (16 * D);
-  const uint8_t* vp = a.v + group * (16 * D);
-  const uint16_t* rp = a.rows + group * 64;
-  b.kw = load_u4(rp + lane / 16 * 8);
+  const Base k(a.k + group * (16 * D), 16 * D), v(a.v + group * (16 * D), 16 * D), rows(a.rows + group * 64, 128);
+  const int first = lane / 16 * 16, mine = first + lane % 16 / (2 * N) * (2 * N);
+  b.kw.load(rows, mine, 0);
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i) b.k[i] = load_u4_stream(kp + i * kTileBytes + lane * 16);
-  b.vw = load_u4(rp + 32 + lane / 16 * 8);
+  for (int i = 0; i < D / 64; ++i) b.k[i] = k.stream16(lane * 16, i * kTileBytes);
+  b.vs.load(rows, mine, 64);
+  b.vw.load(rows, first, 64);
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i) b.v[i] = load_u4_stream(vp + i * kTileBytes + lane * 16);
+  for (int i = 0; i < D / 64; ++i) b.v[i] = v.stream16(lane * 16, i * kTileBytes);
+}
+
+// What lane n + N of a row of 16 lanes holds (0 past the row).
+template <int N>
+__device__ __forceinline__ uint32_t from_above(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x100 + N, 0xf, 0xf, true);
 }
 
 // Eight numbers less 8, in the order of their dimensions.
 __device__ __forceinline__ half8 centred8(uint32_t d) {
   constexpr uint32_t k8 = 0x64086408u, k84 = 0x54805480u;  // 1024 + 8, 64 + 8
   const uint32_t d8 = d >> 8;
-  return join8(less(and_or(d, kNibbles, kBase), k8), less(and_or(d, kNibbles4, kBase4), k84),
-               less(and_or(d8, kNibbles, kBase), k8), less(and_or(d8, kNibbles4, kBase4), k84));
+  return join8(less(mask_or(d, kNibbles, kBase), k8), less(mask_or(d, kNibbles4, kBase4), k84),
+               less(mask_or(d8, kNibbles, kBase), k8), less(mask_or(d8, kNibbles4, kBase4), k84));
 }
 
-template <typename T, int D, int RT>
+// The wavefronts' sums meet in LDS, and go out or wait for those of other splits.
+// (Lane numbers are made anew here: kept through the loop, what follows from them
+// would take registers there.)
+template <typename T, int D, int RT, int W>
+__device__ __forceinline__ void finish_tile(const AttnArgs& a, const Tile& t, int h, int rows, int split, int splits,
+                                            bool partial, unsigned id, const float (&m)[RT], float (&l)[RT],
+                                            const floatx4 (&acc)[RT][D / 16], float (&red)[kWaves][16][D + 4],
+                                            float (&red_m)[kWaves][16 / W * RT], float (&red_l)[kWaves][16 / W * RT]) {
+  constexpr int C = 16 / W, R = C * RT, A = D / 64;
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
+  const int lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int lg = lane / 16, col = lane % C, part = lane % 16 / C;
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+#pragma unroll
+    for (int n = C; n < kWave; n *= 2) l[r] += __shfl_xor(l[r], n);
+    if (lane < C) {
+      red_m[wave][C * r + col] = m[r];
+      red_l[wave][C * r + col] = l[r];
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    __syncthreads();
+    const int rr = C * r + col;
+    float top = red_m[0][rr];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, red_m[w][rr]);
+    const float f = exp2_fast(m[r] - top);
+    if (part == 0) {
+#pragma unroll
+      for (int i = 0; i < A; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          floatx4 o;
+#pragma unroll
+          for (int n = 0; n < 4; ++n) o[n] = acc[r][4 * i + n][j] * f;
+          *reinterpret_cast<floatx4*>(&red[wave][col][64 * i + 16 * lg + 4 * j]) = o;
+        }
+    }
+    __syncthreads();
+    for (int it = tid; it < C * (D / 4); it += kThreads) {
+      const int c = it / (D / 4), d = it % (D / 4) * 4, rc = C * r + c;
+      if (rc >= rows) continue;
+      float mm = red_m[0][rc];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) mm = fmaxf(mm, red_m[w][rc]);
+      float ll = 0.0f;
+      floatx4 o = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        ll += red_l[w][rc] * exp2_fast(red_m[w][rc] - mm);
+        o += *reinterpret_cast<const floatx4*>(&red[w][c][d]);
+      }
+      const int64_t to = out_row(a, t, h, rc);
+      if (partial) {
+        const Partials parts(a);
+        const int i = a.merge ? (int)to * a.splits + split : (int)id * R + rc;
+        parts.store(i * D + d, o);
+        if (d == 0) parts.store_stat(i, mm, ll);
+      } else {
+        finish<T>(a, to, D, d, o, mm, ll);
+      }
+    }
+  }
+  if (partial && !a.merge)
+    join<T, D>(a, t, h, rows, splits, ((int)id - split * a.hk) * R, a.hk * R,
+               a.counters + (id - (unsigned)(split * a.hk)), &red[0][0][0]);
+}
+
+template <typename T, int D, int RT, int W>
 __global__ __launch_bounds__(kWaves* kWave)
-__attribute__((amdgpu_waves_per_eu(2))) void kv4_decode_kernel(AttnArgs a) {
-  constexpr int R = 16 * RT, A = D / 64;
+__attribute__((amdgpu_waves_per_eu(D <= 128 && RT == 1 ? 3 : 2))) void kv4_decode_kernel(AttnArgs a) {
+  static_assert(RT == 1 || W == 1);
+  constexpr int C = 16 / W, N = 8 / W, R = C * RT, A = D / 64, kAhead = 1;
   __shared__ __align__(16) float red[kWaves][16][D + 4];
   __shared__ float red_m[kWaves][R], red_l[kWaves][R];
   const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  const int col = lane % 16, lg = lane / 16;
+  const int lg = lane / 16, col = lane % C, part = lane % 16 / C;
   const unsigned id = a.first + blockIdx.x, pair = id / (unsigned)a.hk;
   const int h = (int)(id - pair * a.hk);
   int split, splits;
@@ -116,34 +229,57 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv4_decode_kernel(AttnArgs a) {
   const bool partial = share.splits > 1 || a.merge;
 
   // ---- queries, as B operands: column = row, dimensions 64 i + 16 lg + 8 j + ..
-  half8 q[RT][2 * A];
-  float factor[RT], qsum[RT];  // qsum: -sum(q)
-  int lo[RT], hi[RT];
+  uint4 raw[RT][2 * A];
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
-    const int row = t.row0 + min(16 * r + col, rows - 1);
+    const int row = t.row0 + min(C * r + col, rows - 1);
     const int qi = (int)((unsigned)row / (unsigned)a.group);
     const uint8_t* p = a.q + (int64_t)(t.first_token + qi) * a.q_ts +
                        (int64_t)(h * a.group + (row - qi * a.group)) * a.q_hs + lg * 32;
-    uint4 raw[2 * A];
 #pragma unroll
-    for (int i = 0; i < 2 * A; ++i) raw[i] = load_u4(p + (i / 2) * 128 + (i % 2) * 16);
+    for (int i = 0; i < 2 * A; ++i) raw[r][i] = load_u4(p + (i / 2) * 128 + (i % 2) * 16);
+  }
+
+  // The bytes of kAhead turns are under way while one is worked on, and the block
+  // ids of the turn after them.  The first go out before the queries are looked at.
+  const auto id_of = [&](int g) { return group_of(a, t, h, min(g, end - 1)); };
+  constexpr int kBufs = kAhead + 1;
+  int g = begin + wave, to = g + kAhead * kWaves;
+  Bytes<D, N> b[kBufs];
+  bool ok[kBufs];
+  Group next;
+  if (g < end) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const Group x = id_of(g + i * kWaves);
+      ok[i] = x.ok;
+      fetch(a, x, lane, b[i]);
+      __builtin_amdgcn_sched_barrier(0);  // (in this order: what is waited for is counted back)
+    }
+    next = id_of(to);
+  }
+
+  half8 q[RT][2 * A];
+  float factor[RT], qsum[RT];  // qsum: -sum(q)
+  int pos[RT];                 // of the row's query
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
     factor[r] = a.scale_log2e;
     if constexpr (!__is_same(T, _Float16)) {
       float m = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 2 * A; ++i) m = load_amax<T>(raw[i], m);
+      for (int i = 0; i < 2 * A; ++i) m = load_amax<T>(raw[r][i], m);
       m = fmaxf(m, __shfl_xor(m, 16));
       m = fmaxf(m, __shfl_xor(m, 32));
       const int e = row_exponent(m), e1 = e / 2, e2 = e - e1;
       const float f1 = pow2(-e1), f2 = pow2(-e2);
 #pragma unroll
       for (int i = 0; i < 2 * A; ++i)
-        q[r][i] = __builtin_convertvector(Eight<T>::load(&raw[i]) * f1 * f2, half8);
+        q[r][i] = __builtin_convertvector(Eight<T>::load(&raw[r][i]) * f1 * f2, half8);
       factor[r] = a.scale_log2e * pow2(e1) * pow2(e2);
     } else {
 #pragma unroll
-      for (int i = 0; i < 2 * A; ++i) q[r][i] = as_half8(raw[i]);
+      for (int i = 0; i < 2 * A; ++i) q[r][i] = as_half8(raw[r][i]);
     }
     factor[r] = in_range(factor[r]);
     float sum = 0.0f;
@@ -154,7 +290,7 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv4_decode_kernel(AttnArgs a) {
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
     qsum[r] = -sum;
-    seen(a, t, row, &lo[r], &hi[r]);
+    pos[r] = t.kv_len - t.queries + (int)((unsigned)(t.row0 + min(C * r + col, rows - 1)) / (unsigned)a.group);
   }
   floatx4 acc[RT][4 * A];
   float m[RT], l[RT];  // l: each lane's own share of the sum
@@ -166,10 +302,10 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv4_decode_kernel(AttnArgs a) {
     for (int i = 0; i < 4 * A; ++i) acc[r][i] = floatx4{0, 0, 0, 0};
   }
 
-  const auto step = [&](const Bytes<D>& b, int g, bool ok) {
-    floatx4 s[RT][2];
+  const auto step = [&](const Bytes<D, N>& b, int g, bool ok) {
+    floatx4 all[RT][2];
 #pragma unroll
-    for (int r = 0; r < RT; ++r) s[r][0] = s[r][1] = floatx4{0, 0, 0, 0};
+    for (int r = 0; r < RT; ++r) all[r][0] = all[r][1] = floatx4{0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < A; ++i) {
       const uint32_t d[4] = {b.k[i].x, b.k[i].y, b.k[i].z, b.k[i].w};
@@ -177,39 +313,44 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv4_decode_kernel(AttnArgs a) {
       for (int w = 0; w < 4; ++w) {
         const half8 k = centred8(d[w]);
 #pragma unroll
-        for (int r = 0; r < RT; ++r) s[r][w / 2] = mfma16x16x32(k, q[r][2 * i + w % 2], s[r][w / 2]);
+        for (int r = 0; r < RT; ++r) all[r][w / 2] = mfma16x16x32(k, q[r][2 * i + w % 2], all[r][w / 2]);
       }
     }
-    const uint32_t kw[4] = {b.kw.x, b.kw.y, b.kw.z, b.kw.w}, vw[4] = {b.vw.x, b.vw.y, b.vw.z, b.vw.w};
-    half2v ks[4], kz[4], vs[4];  // tokens 2 i and 2 i + 1 of the lane's eight
+    half2v ks[(N + 1) / 2], kz[(N + 1) / 2], vs[(N + 1) / 2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      ks[i] = as_half2(kw[i] & kStepBits);
-      kz[i] = less(and_or(kw[i], kNibbles, kBase), 0x64086408u);  // less 8
-      vs[i] = as_half2(vw[i] & kStepBits);
+    for (int i = 0; i < N / 2; ++i) {
+      ks[i] = as_half2(b.kw.at(i) & kStepBits);
+      kz[i] = less(mask_or(b.kw.at(i), kNibbles, kBase), 0x64086408u);  // less 8
+      vs[i] = as_half2(b.vs.at(i) & kStepBits);
     }
     const int t0 = opaque(g << 5);
     const bool edge = t0 < lo_max || t0 + 32 > hi_min;
+    float s[RT][N];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float x = __builtin_fmaf((float)kz[i / 2][i % 2], qsum[r], s[r][i / 4][i % 4]);
-        s[r][i / 4][i % 4] = __builtin_fmaf((float)ks[i / 2][i % 2], x, 0.0f);
+      for (int i = 0; i < N; ++i) {
+        float x = all[r][i / 4][i % 4];
+#pragma unroll
+        for (int n = 1; n < W; ++n) x = part == n ? all[r][(n * N + i) / 4][(n * N + i) % 4] : x;
+        x = __builtin_fmaf((float)kz[i / 2][i % 2], qsum[r], x);
+        s[r][i] = __builtin_fmaf((float)ks[i / 2][i % 2], x, 0.0f);
       }
       if (!ok) {
         keep_branch();
-        s[r][0] = s[r][1] = __builtin_nanf("");
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[r][i] = __builtin_nanf("");
       }
       if (edge) {
         keep_branch();
-        const int first = lo[r] - t0 - 8 * lg, past = hi[r] - t0 - 8 * lg;
+        const int at = t0 + 8 * lg + N * part;
+        const int first = a.window > 0 ? pos[r] - a.window + 1 - at : -at, past = (a.causal ? pos[r] + 1 : t.kv_len) - at;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          s[r][i / 4][i % 4] = ((i < first) | (i >= past)) ? -__builtin_inff() : s[r][i / 4][i % 4];
+        for (int i = 0; i < N; ++i) s[r][i] = ((i < first) | (i >= past)) ? -__builtin_inff() : s[r][i];
       }
     }
-    half8 p[RT];
+    typedef _Float16 halfN __attribute__((ext_vector_type(N)));
+    halfN mine[RT];
     float sum[RT];
     bool raise = false;
     const auto weights = [&](int r) {  // the largest of them
@@ -217,12 +358,12 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv4_decode_kernel(AttnArgs a) {
       float most = 0.0f;
       sum[r] = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float e = exp2_fast(__builtin_fmaf(s[r][i / 4][i % 4], factor[r], off));
+      for (int i = 0; i < N; ++i) {
+        const float e = exp2_fast(__builtin_fmaf(s[r][i], factor[r], off));
         const float w = __builtin_fmaf((float)vs[i / 2][i % 2], e, 0.0f);
         sum[r] += e;
         most = fmaxf(most, w);
-        p[r][i] = (_Float16)w;
+        mine[r][i] = (_Float16)w;
       }
       return most;
     };
@@ -237,10 +378,10 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv4_decode_kernel(AttnArgs a) {
       for (int r = 0; r < RT; ++r) {
         float top = m[r];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          top = fmaxf(top, s[r][i / 4][i % 4] * factor[r] + log2_fast(fmaxf((float)vs[i / 2][i % 2], 0x1p-24f)));
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
+        for (int i = 0; i < N; ++i)
+          top = fmaxf(top, s[r][i] * factor[r] + log2_fast(fmaxf((float)vs[i / 2][i % 2], 0x1p-24f)));
+#pragma unroll
+        for (int n = C; n < kWave; n *= 2) top = fmaxf(top, __shfl_xor(top, n));
         const float f = exp2_fast(m[r] - top);
         m[r] = top;
         l[r] *= f;
@@ -249,13 +390,26 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv4_decode_kernel(AttnArgs a) {
         weights(r);
       }
     }
+    half8 p[RT];
 #pragma unroll
-    for (int r = 0; r < RT; ++r) l[r] += sum[r];
+    for (int r = 0; r < RT; ++r) {
+      l[r] += sum[r];
+      if constexpr (W == 1) {
+        p[r] = mine[r];
+      } else if constexpr (W == 2) {
+        const uint2 u = __builtin_bit_cast(uint2, mine[r]);
+        p[r] = as_half8(make_uint4(u.x, u.y, from_above<C>(u.x), from_above<C>(u.y)));
+      } else {
+        const uint32_t u = __builtin_bit_cast(uint32_t, mine[r]);
+        p[r] = as_half8(make_uint4(u, from_above<C>(u), from_above<2 * C>(u), from_above<3 * C>(u)));
+      }
+    }
+    const uint32_t vw[4] = {b.vw.at(0), b.vw.at(1), b.vw.at(2), b.vw.at(3)};
     uint32_t z[4], z4[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      z[i] = and_or(vw[i], kNibbles, kBase);
-      z4[i] = and_or(vw[i] << 4, kNibbles4, kBase4);
+      z[i] = mask_or(vw[i], kNibbles, kBase);
+      z4[i] = mask_or(vw[i] << 4, kNibbles4, kBase4);
     }
 #pragma unroll
     for (int i = 0; i < A; ++i) {
@@ -266,7 +420,7 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv4_decode_kernel(AttnArgs a) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const uint32_t x = n < 2 ? d[w] : d[w] >> 8;
-          v[w] = n % 2 ? less(and_or(x, kNibbles4, kBase4), z4[w]) : less(and_or(x, kNibbles, kBase), z[w]);
+          v[w] = n % 2 ? less(mask_or(x, kNibbles4, kBase4), z4[w]) : less(mask_or(x, kNibbles, kBase), z[w]);
         }
         const half8 v8 = join8(v[0], v[1], v[2], v[3]);
 #pragma unroll
@@ -275,87 +429,24 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv4_decode_kernel(AttnArgs a) {
     }
   };
 
-  if (begin + wave < end) {
-    // group g's bytes are loaded while group g - kWaves is worked on, and its
-    // block id one turn before that.
-    const auto id_of = [&](int g) { return group_of(a, t, h, min(g, end - 1)); };
-    int g = begin + wave;
-    Bytes<D> b0, b1;
-    Group now = id_of(g), next = id_of(g + kWaves);
-    fetch<D>(a, now, lane, b0);
-    while (true) {
-      fetch<D>(a, next, lane, b1);
-      bool ok = now.ok;
-      now = next;
-      next = id_of(g + 2 * kWaves);
-      step(b0, g, ok);
+  if (g < end) {
+    const auto turn = [&](int now) {
+      const int last = (now + kAhead) % kBufs;
+      ok[last] = next.ok;
+      fetch(a, next, lane, b[last]);
+      to += kWaves;
+      next = id_of(to);
+      // (they go out before anything of this turn waits for its own)
+      __builtin_amdgcn_sched_barrier(0);
+      step(b[now], g, ok[now]);
       g += kWaves;
-      if (g >= end) break;
-      fetch<D>(a, next, lane, b0);
-      ok = now.ok;
-      now = next;
-      next = id_of(g + 2 * kWaves);
-      step(b1, g, ok);
-      g += kWaves;
-      if (g >= end) break;
-    }
+      return g < end;
+    };
+    while (turn(0) && turn(1)) {}
   }
 
   // ---- the four wavefronts' results
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    l[r] += __shfl_xor(l[r], 16);
-    l[r] += __shfl_xor(l[r], 32);
-    if (lg == 0) {
-      red_m[wave][16 * r + col] = m[r];
-      red_l[wave][16 * r + col] = l[r];
-    }
-  }
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    __syncthreads();
-    const int rr = 16 * r + col;
-    float top = red_m[0][rr];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, red_m[w][rr]);
-    const float f = exp2_fast(m[r] - top);
-#pragma unroll
-    for (int i = 0; i < A; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        floatx4 o;
-#pragma unroll
-        for (int n = 0; n < 4; ++n) o[n] = acc[r][4 * i + n][j] * f;
-        *reinterpret_cast<floatx4*>(&red[wave][col][64 * i + 16 * lg + 4 * j]) = o;
-      }
-    __syncthreads();
-    for (int it = tid; it < 16 * (D / 4); it += kThreads) {
-      const int c = it / (D / 4), d = it % (D / 4) * 4, rc = 16 * r + c;
-      if (rc >= rows) continue;
-      float mm = red_m[0][rc];
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w) mm = fmaxf(mm, red_m[w][rc]);
-      float ll = 0.0f;
-      floatx4 o = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        ll += red_l[w][rc] * exp2_fast(red_m[w][rc] - mm);
-        o += *reinterpret_cast<const floatx4*>(&red[w][c][d]);
-      }
-      const int64_t to = out_row(a, t, h, rc);
-      if (partial) {
-        const Partials parts(a);
-        const int i = a.merge ? (int)to * a.splits + split : (int)id * R + rc;
-        parts.store(i * D + d, o);
-        if (d == 0) parts.store_stat(i, mm, ll);
-      } else {
-        finish<T>(a, to, D, d, o, mm, ll);
-      }
-    }
-  }
-  if (partial && !a.merge)
-    join<T, D>(a, t, h, rows, share.splits, ((int)id - split * a.hk) * R, a.hk * R,
-               a.counters + (id - (unsigned)(split * a.hk)), &red[0][0][0]);
+  finish_tile<T, D, RT, W>(a, t, h, rows, split, share.splits, partial, id, m, l, acc, red, red_m, red_l);
 }
 
 // ---------------------------------------------------------------------------
@@ -499,15 +590,15 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv4_prefill_kernel(AttnArgs a) {
       for (int tt = 0; tt < 2; ++tt) {
         const uint32_t w = __builtin_amdgcn_perm(x.kw, x.kw, tt ? 0x03020302u : 0x01000100u);
         const half2v s = as_half2(w & kStepBits);
-        const uint32_t z = and_or(w, kNibbles, kBase), z4 = and_or(w << 4, kNibbles4, kBase4);
+        const uint32_t z = mask_or(w, kNibbles, kBase), z4 = mask_or(w << 4, kNibbles4, kBase4);
         const int row = 16 * (l16 / 8) + 8 * tt + 4 * (l16 / 4 % 2) + l16 % 4;
         uint8_t* p = buf + ((my_group * (D / 16) + my_tile * 4 + g16) * kWave + row) * 16;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const uint32_t u = d[2 * tt + j], u8 = u >> 8;
           *reinterpret_cast<half8*>(p + j * 32 * 16) =
-              join8(less(and_or(u, kNibbles, kBase), z) * s, less(and_or(u, kNibbles4, kBase4), z4) * s,
-                    less(and_or(u8, kNibbles, kBase), z) * s, less(and_or(u8, kNibbles4, kBase4), z4) * s);
+              join8(less(mask_or(u, kNibbles, kBase), z) * s, less(mask_or(u, kNibbles4, kBase4), z4) * s,
+                    less(mask_or(u8, kNibbles, kBase), z) * s, less(mask_or(u8, kNibbles4, kBase4), z4) * s);
         }
       }
     }
@@ -522,8 +613,8 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv4_prefill_kernel(AttnArgs a) {
         for (int i = 0; i < 4; ++i) {
           const uint32_t u = n < 2 ? d[i] : d[i] >> 8;
           const half2v s = as_half2(w[i] & kStepBits);
-          v[i] = n % 2 ? less(and_or(u, kNibbles4, kBase4), and_or(w[i] << 4, kNibbles4, kBase4)) * s
-                       : less(and_or(u, kNibbles, kBase), and_or(w[i], kNibbles, kBase)) * s;
+          v[i] = n % 2 ? less(mask_or(u, kNibbles4, kBase4), mask_or(w[i] << 4, kNibbles4, kBase4)) * s
+                       : less(mask_or(u, kNibbles, kBase), mask_or(w[i], kNibbles, kBase)) * s;
         }
         *reinterpret_cast<half8*>(p + n * 8 * 16) = join8(v[0], v[1], v[2], v[3]);
       }
@@ -727,10 +818,12 @@ hipError_t launch_sized(AttnArgs a, const PagedPlan& p, hipStream_t stream) {
     a.first = (unsigned)i;
     const unsigned grid = (unsigned)(p.grid - i < most ? p.grid - i : most);
     if (p.kernel == 1 && p.gangs == 1) kv4_prefill_kernel<T, D, 1><<<grid, kThreads, kLds, stream>>>(a);
-    else if (p.kernel == 0 && p.rows == 16) kv4_decode_kernel<T, D, 1><<<grid, kThreads, 0, stream>>>(a);
+    else if (p.kernel == 0 && p.rows == 4) kv4_decode_kernel<T, D, 1, 4><<<grid, kThreads, 0, stream>>>(a);
+    else if (p.kernel == 0 && p.rows == 8) kv4_decode_kernel<T, D, 1, 2><<<grid, kThreads, 0, stream>>>(a);
+    else if (p.kernel == 0 && p.rows == 16) kv4_decode_kernel<T, D, 1, 1><<<grid, kThreads, 0, stream>>>(a);
     else if constexpr (D <= 128) {
       if (p.kernel == 1) kv4_prefill_kernel<T, D, 2><<<grid, 2 * kThreads, kLds2, stream>>>(a);
-      else kv4_decode_kernel<T, D, 2><<<grid, kThreads, 0, stream>>>(a);
+      else kv4_decode_kernel<T, D, 2, 1><<<grid, kThreads, 0, stream>>>(a);
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -744,15 +837,21 @@ hipError_t launch_sized(AttnArgs a, const PagedPlan& p, hipStream_t stream) {
 struct Kv4Costs {
   static double base(bool prefill, int rows, int D) {
     return prefill ? (D == 64 ? 1.1 : D == 128 ? 1.5 : 1.35)
-                   : D == 256 ? 1.1 : (rows == 16 ? 0.55 : 0.85) * (D == 64 ? 0.75 : 1.0);
+                   : D == 256 ? 1.1 : (rows <= 16 ? 0.55 : 0.85) * (D == 64 ? 0.75 : 1.0);
   }
   static double more(bool prefill, int rows, int D) {
-    return prefill ? (D == 256 ? 0.6 : 0.4) : D == 256 ? 1.2 : (rows == 16 ? 0.25 : 0.58) * (D == 64 ? 0.6 : 1.0);
+    return prefill ? (D == 256 ? 0.6 : 0.4) : D == 256 ? 1.2 : (rows <= 16 ? 0.25 : 0.58) * (D == 64 ? 0.6 : 1.0);
   }
   static double slots(bool prefill, int gangs, int rows, int D) {
     return gangs == 2 ? 1.0 : prefill || D == 256 || rows > 16 ? 2.0 : 3.0;
   }
   static double token_bytes(int D) { return D + 4.0; }
+  static int few(int64_t rows, int D) { return rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 || D > 128 ? 16 : 32; }
+  static double merge(int splits) { return 4.5 + 0.1 * splits; }
+  // (tiles that the offsets might ask for, but that no batch of this length has, are
+  // room in the grid and no workgroups to cut for: 48 requests, 776 workgroups on 256
+  // CUs instead of 768 held up the last eight of them to the end, 51 -> 43 us)
+  static constexpr bool aim = true;
   static int share_least(int rows, int D) { return rows == 32 ? 32 : D == 256 ? 8 : 16; }
 };
 

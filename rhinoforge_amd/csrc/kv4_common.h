@@ -13,6 +13,13 @@ constexpr uint32_t kStepBits = 0xfff0fff0u;    // a word's step, both halves
 // bits 4..7.
 constexpr uint32_t kBase = 0x64006400u, kBase4 = 0x54005400u;
 
+// (a & m) | c in one instruction, the mask in a scalar register.
+__device__ __forceinline__ uint32_t mask_or(uint32_t a, uint32_t m, uint32_t c) {
+  uint32_t r;
+  asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "s"(m), "v"(c));
+  return r;
+}
+
 __device__ __forceinline__ half2v as_half2(uint32_t v) { return __builtin_bit_cast(half2v, v); }
 __device__ __forceinline__ half8 join8(half2v a, half2v b, half2v c, half2v d) {
   return __builtin_shufflevector(__builtin_shufflevector(a, b, 0, 1, 2, 3), __builtin_shufflevector(c, d, 0, 1, 2, 3),

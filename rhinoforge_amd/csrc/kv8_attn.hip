@@ -802,6 +802,10 @@ struct Kv8Costs {
     return gangs == 2 ? 1.0 : prefill || D == 256 || rows > 16 ? 2.0 : 3.0;
   }
   static double token_bytes(int D) { return 2.0 * D; }
+  // (two tiles of 16 rows of size 256 would not fit the registers)
+  static int few(int64_t rows, int D) { return rows <= 16 || D > 128 ? 16 : 32; }
+  static double merge(int splits) { return 4.5; }
+  static constexpr bool aim = false;
   static int share_least(int rows, int D) { return rows == 32 ? 32 : D == 256 ? 8 : 16; }
 };
 

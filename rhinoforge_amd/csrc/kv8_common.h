@@ -63,6 +63,7 @@ struct PagedPlan {
   int least;      // 32-token groups of a split, at least
   bool merge;     // a second kernel adds the splits
   int shares = 0; // of all tiles of a key/value head together, for batches of unequal lengths
+  int aim = 0;    // that many of them, unless there are more tiles
   int64_t grid;   // workgroups
   int64_t partials;  // rows of partial results
   size_t workspace;  // their bytes

@@ -31,7 +31,8 @@ struct PagedArgs {
   int per_request;     // cu == nullptr: queries of a request
   int splits, least, tiles;
   unsigned first;      // workgroup that the launch begins at
-  int shares;          // find_share: of all tiles together (0: not used)
+  int shares;          // find_share: of all tiles together, at most (0: not used)
+  int aim;             // that many of them, unless there are more tiles
   bool merge;          // partial results are added by merge_splits_kernel, else by join()
   int causal, window;  // window 0: none
   float scale_log2e;
@@ -157,7 +158,7 @@ __device__ __forceinline__ void seen(const PagedArgs& a, const Tile& t, int row,
 
 // Split `split` of tile `tile` as workgroup x of a batch of unequal lengths
 // finds it.  Every tile is cut into shares of at most L groups, with the
-// smallest L that leaves no more than `shares` of them: a batch takes as long as
+// smallest L that leaves no more than `aim` of them: a batch takes as long as
 // its mean, not as its longest request, and its workgroups fill the CUs evenly.
 // Each lane holds ceil(requests / 64) requests, so up to 64 of them cost one
 // memory round trip; for more, L is a bound that needs no search.
@@ -194,22 +195,22 @@ __device__ __forceinline__ bool find_share(const PagedArgs& a, int x, Tile* t, i
   }
   const auto all = [&](int v) { return __builtin_amdgcn_readlane(scan(v, add), kWave - 1); };
   const unsigned total = (unsigned)all(work);
-  const int over = a.shares - all(tiles);  // sum ceil(n / L) < sum n / L + tiles
+  const int over = a.aim - all(tiles);  // sum ceil(n / L) < sum n / L + tiles
   longest = __builtin_amdgcn_readlane(scan(longest, most), kWave - 1);
   const auto ratio = [](unsigned u, unsigned v) { return (u + v - 1) / v; };
   const unsigned least = max((unsigned)a.least, ratio((unsigned)longest, (unsigned)a.splits));
   unsigned length = max(over > 0 ? min(ratio(total, (unsigned)over), (unsigned)longest) : (unsigned)longest, least);
   // ceil(n / length) or, by rounding, one less (never more: there is room for
-  // `shares`); all workgroups come to the same
+  // `aim`); all workgroups come to the same
   const auto cut = [](int n, unsigned length) {
     const float inv = (1.0f - 0x1p-20f) * __builtin_amdgcn_rcpf((float)length);
     return max((int)__builtin_ceilf((float)n * inv), 1);
   };
   if (per == 1) {
-    unsigned few = max(ratio(total, (unsigned)a.shares), least) - 1;  // too short, or not allowed
+    unsigned few = max(ratio(total, (unsigned)a.aim), least) - 1;  // too short, or not allowed
     for (int i = 0; i < 7 && few + 1 < length; ++i) {
       const unsigned mid = (few + length) / 2;
-      const bool fits = all(__mul24(e.tiles, cut(e.n, mid))) <= a.shares;
+      const bool fits = all(__mul24(e.tiles, cut(e.n, mid))) <= a.aim;
       if (fits) length = mid;
       else few = mid;
     }
@@ -321,6 +322,8 @@ __device__ __forceinline__ float log2_fast(float x) { return __builtin_amdgcn_lo
 // of 50 queries, 8 heads of 256, 8 splits: 87 us with join(), 36 with it).
 // ---------------------------------------------------------------------------
 constexpr int kThreads = 256;
+constexpr int kWaves = 4;
+constexpr int kMaxRows = 32;  // of a tile whose splits are joined
 constexpr int kDeviceScope = 16;  // sc1 of a buffer access
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -398,13 +401,32 @@ __device__ __forceinline__ void join(const PagedArgs& a, const Tile& t, int h, i
   const int units = rows * (D / 4);
   int ways = 1;
   while (units * ways * 2 <= kThreads && ways * 2 <= splits) ways *= 2;
-  float* stat = buf;  // [rows][splits][m, l]
+  float* stat = buf;  // [rows][splits][2^(m - the row's), l]
   floatx4* sums = reinterpret_cast<floatx4*>(buf + (rows * splits * 2 + 3) / 4 * 4);
-  for (int i = tid; i < rows * splits; i += kThreads) {
-    const int rc = (int)((unsigned)i / (unsigned)splits);
-    *reinterpret_cast<floatx2*>(stat + 2 * i) =
-        parts.load_stat(first + (i - rc * splits) * stride + rc);
+  __shared__ float tops[kMaxRows];
+  // A wavefront takes every fourth row, a lane one of its splits (at most 64).
+  const int lane = tid % kWave, wave = tid / kWave;
+  floatx2 own[kMaxRows / kWaves];
+#pragma unroll
+  for (int i = 0; i < kMaxRows / kWaves; ++i) {
+    own[i] = floatx2{-__builtin_inff(), 0.0f};
+    const int rc = wave + i * kWaves;
+    if (rc < rows && lane < splits) own[i] = parts.load_stat(first + lane * stride + rc);
   }
+  const auto factors = [&] {
+#pragma unroll
+    for (int i = 0; i < kMaxRows / kWaves; ++i) {
+      const int rc = wave + i * kWaves;
+      if (rc >= rows) break;
+      float m = own[i][0];
+#pragma unroll
+      for (int n = 1; n < kWave; n *= 2) m = fmaxf(m, __shfl_xor(m, n));
+      if (lane == 0) tops[rc] = m;
+      if (lane < splits)
+        *reinterpret_cast<floatx2*>(stat + 2 * (rc * splits + lane)) =
+            floatx2{exp2_fast(own[i][0] - safe(m)), own[i][1]};
+    }
+  };
   for (int u0 = 0; u0 < units; u0 += kThreads) {
     const int way = ways == 1 ? 0 : (int)((unsigned)tid / (unsigned)units);
     const int u = u0 + (ways == 1 ? tid : tid - way * units);
@@ -415,11 +437,15 @@ __device__ __forceinline__ void join(const PagedArgs& a, const Tile& t, int h, i
     floatx4 x[kFlight];
 #pragma unroll
     for (int k = 0; k < kFlight; ++k) x[k] = parts.load(at + min(way + k * ways, splits - 1) * next);
-    if (u0 == 0) __syncthreads();  // stat
-    const float* st = stat + rc * splits * 2;
-    float m = -__builtin_inff(), l = 0.0f;
-    for (int s = 0; s < splits; ++s) m = fmaxf(m, st[2 * s]);
-    for (int s = 0; s < splits; ++s) l += st[2 * s + 1] * exp2_fast(st[2 * s] - safe(m));
+    if (u0 == 0) {
+      factors();
+      __syncthreads();
+    }
+    const floatx2* st = reinterpret_cast<const floatx2*>(stat) + rc * splits;
+    const float m = tops[rc];
+    float l = 0.0f;
+#pragma unroll 8
+    for (int s = 0; s < splits; ++s) l += st[s][1] * st[s][0];
     floatx4 o = 0.0f;
     for (int s0 = way; s0 < splits; s0 += kFlight * ways) {
       floatx4 y[kFlight];
@@ -433,7 +459,7 @@ __device__ __forceinline__ void join(const PagedArgs& a, const Tile& t, int h, i
 #pragma unroll
       for (int k = 0; k < kFlight; ++k) {
         const int s = s0 + k * ways;
-        if (s < splits) o += y[k] * exp2_fast(st[2 * s] - safe(m));
+        if (s < splits) o += y[k] * st[s][0];
       }
     }
     if (ways > 1) {  // (units < kThreads: one turn of the outer loop)
@@ -446,7 +472,6 @@ __device__ __forceinline__ void join(const PagedArgs& a, const Tile& t, int h, i
   }
 }
 
-constexpr int kWaves = 4;
 
 __device__ __forceinline__ floatx16 mfma32x32x16(half8 a, half8 b, floatx16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
@@ -493,7 +518,9 @@ struct Estimate {
 
 // Times of the kernels, fitted (Costs, one for each cache): base and more, us of a
 // workgroup's turn alone and for each workgroup beside it on its CU; slots, the
-// workgroups that a CU runs at a time; token_bytes, a token's keys and values;
+// workgroups that a CU runs at a time; token_bytes, a token's keys and values; few, rows of a
+// tile of the decode kernel; merge, us of the second kernel before its bytes; aim,
+// whether shares are cut for the workgroups that run at a time, not for all in the grid;
 // share_least, 32-token groups of a share, at least.
 template <typename Costs>
 Estimate estimate(bool prefill, int gangs, int rows, double tiles, double groups, double longest, double tokens_heads, bool ragged,
@@ -523,7 +550,7 @@ Estimate estimate(bool prefill, int gangs, int rows, double tiles, double groups
     if (s > 1) {
       const double units = held * (D / 4), ways = units < kThreads ? kThreads / units : 1.0;
       const double join = 2.0 + 1.2 * ceil(units / kThreads) * ceil(s / (8.0 * ways));
-      const double second = 4.5 + tokens_heads * s * D * 8.0 / 3e6;
+      const double second = Costs::merge(s) + tokens_heads * s * D * 8.0 / 3e6;
       merge = prefill || second < join || tiles * hk > kMaxSplitCounters;
       us += merge ? second : join;
     }
@@ -569,8 +596,7 @@ PagedPlan plan_paged_attention(const PagedShape& a, int cus) {
     return (n < 1 ? 1 : n) / RF_KV8_GROUP + 0.5;
   };
   const double tokens_heads = (double)a.tokens * a.heads, longest = most_kv / (double)RF_KV8_GROUP + 0.5;
-  // (two tiles of 16 rows of size 256 would not fit the registers)
-  const int few = most_rows <= 16 || D > 128 ? 16 : 32;
+  const int few = Costs::few(most_rows, D);
   const int most = (int)(most_rows < 1024 ? most_rows : 1024);
   Estimate e = estimate<Costs>(false, 1, few, (double)useful(few), groups(few), longest, tokens_heads, ragged,
                         1.0 / ceil_div(most_rows, few), most, D, (int)hk, cus);
@@ -605,7 +631,9 @@ PagedPlan plan_paged_attention(const PagedShape& a, int cus) {
     // cut, in shares that are long enough for the join they cost (what was
     // measured stands at each Costs).
     int64_t shares = ceil_div(3 * useful(p.rows) * hk, 2 * cus) * cus / hk;
+    p.aim = (int)shares;
     if (shares < p.tiles) shares = p.tiles;
+    if (!Costs::aim || p.aim < 1) p.aim = (int)shares;
     // (16 workgroups a CU even out by themselves, and their partial results stay
     // below 70 MB)
     if (shares * hk <= 16 * cus && fits(shares * hk * p.rows, shares * hk)) {
@@ -661,6 +689,7 @@ void fill_paged(PagedArgs& a, const In& in, const PagedPlan& p) {
   a.least = p.least;
   a.merge = p.merge;
   a.shares = p.shares;
+  a.aim = p.aim;
   a.tiles = (int)p.tiles;
   a.causal = in.causal;
   a.window = in.window > (1 << 30) ? 1 << 30 : (int)in.window;

@@ -430,3 +430,25 @@ def test_long_and_ragged_batches(lens, n):
     for _ in range(3):
         again, l2 = _check(q, k, v, table, lens, [n] * len(lens), max_q_len=n, max_kv_len=max(lens))
         assert torch.equal(again, got) and torch.equal(l2, lse)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_read_of_mixed_lists(d):
+    """Runs of all lengths from every place, single tokens and what is outside, in lists of odd lengths."""
+    bs, hk, nb = 64, 5, 40
+    k, v = _filled(nb, hk, bs, d, 30), _filled(nb, hk, bs, d, 31)
+    cache = _cache(k, v)
+    refs = [o.values(*(_np(t) for t in side)) for side in (k, v)]
+    for n in (17, 49, 1650, 2003):
+        r, slots = np.random.default_rng(n), []
+        while len(slots) < n:
+            at = int(r.integers(-5, nb * bs))
+            slots += range(at, at + int(r.choice([1, 1, 1, 2, 7, 8, 9, 31, 70])))
+            if r.random() < 0.3:
+                slots += [int(r.integers(0, nb * bs))] * 2 + r.integers(0, nb * bs, int(r.integers(0, 40))).tolist()
+        slots = np.array(slots[:n], np.int32)
+        got = cache.read(torch.from_numpy(slots).to(DEV), torch.float32)
+        inside = (slots >= 0) & (slots < nb * bs)
+        at = np.clip(slots, 0, nb * bs - 1)
+        for ref, y in zip(refs, got):
+            assert np.array_equal(_np(y), ref[at // bs, :, at % bs] * inside[:, None, None]), n
