@@ -125,11 +125,11 @@ __device__ __forceinline__ half8 centred8(uint32_t d) {
 // The wavefronts' sums meet in LDS, and go out or wait for those of other splits.
 // (Lane numbers are made anew here: kept through the loop, what follows from them
 // would take registers there.)
-template <typename T, int D, int RT, int W>
+template <typename T, int D, int RT, int W, int NW>
 __device__ __forceinline__ void finish_tile(const AttnArgs& a, const Tile& t, int h, int rows, int split, int splits,
                                             bool partial, unsigned id, const float (&m)[RT], float (&l)[RT],
-                                            const floatx4 (&acc)[RT][D / 16], float (&red)[kWaves][16][D + 4],
-                                            float (&red_m)[kWaves][16 / W * RT], float (&red_l)[kWaves][16 / W * RT]) {
+                                            const floatx4 (&acc)[RT][D / 16], float (&red)[NW][16 / W][D + 4],
+                                            float (&red_m)[NW][16 / W * RT], float (&red_l)[NW][16 / W * RT]) {
   constexpr int C = 16 / W, R = C * RT, A = D / 64;
   int tid = threadIdx.x;
   asm volatile("" : "+v"(tid));
@@ -150,7 +150,7 @@ __device__ __forceinline__ void finish_tile(const AttnArgs& a, const Tile& t, in
     const int rr = C * r + col;
     float top = red_m[0][rr];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, red_m[w][rr]);
+    for (int w = 1; w < NW; ++w) top = fmaxf(top, red_m[w][rr]);
     const float f = exp2_fast(m[r] - top);
     if (part == 0) {
 #pragma unroll
@@ -164,16 +164,16 @@ __device__ __forceinline__ void finish_tile(const AttnArgs& a, const Tile& t, in
         }
     }
     __syncthreads();
-    for (int it = tid; it < C * (D / 4); it += kThreads) {
+    for (int it = tid; it < C * (D / 4); it += NW * kWave) {
       const int c = it / (D / 4), d = it % (D / 4) * 4, rc = C * r + c;
       if (rc >= rows) continue;
       float mm = red_m[0][rc];
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) mm = fmaxf(mm, red_m[w][rc]);
+      for (int w = 1; w < NW; ++w) mm = fmaxf(mm, red_m[w][rc]);
       float ll = 0.0f;
       floatx4 o = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
+      for (int w = 0; w < NW; ++w) {
         ll += red_l[w][rc] * exp2_fast(red_m[w][rc] - mm);
         o += *reinterpret_cast<const floatx4*>(&red[w][c][d]);
       }
@@ -189,17 +189,20 @@ __device__ __forceinline__ void finish_tile(const AttnArgs& a, const Tile& t, in
     }
   }
   if (partial && !a.merge)
-    join<T, D>(a, t, h, rows, splits, ((int)id - split * a.hk) * R, a.hk * R,
+    join<T, D, NW * kWave>(a, t, h, rows, splits, ((int)id - split * a.hk) * R, a.hk * R,
                a.counters + (id - (unsigned)(split * a.hk)), &red[0][0][0]);
 }
 
-template <typename T, int D, int RT, int W>
-__global__ __launch_bounds__(kWaves* kWave)
+template <typename T, int D, int RT, int W, int NW>
+__global__ __launch_bounds__(NW* kWave)
 __attribute__((amdgpu_waves_per_eu(D <= 128 && RT == 1 ? 3 : 2))) void kv4_decode_kernel(AttnArgs a) {
   static_assert(RT == 1 || W == 1);
   constexpr int C = 16 / W, N = 8 / W, R = C * RT, A = D / 64, kAhead = 1;
-  __shared__ __align__(16) float red[kWaves][16][D + 4];
-  __shared__ float red_m[kWaves][R], red_l[kWaves][R];
+  // (join() wants room for the splits' numbers)
+  constexpr int kRed = NW * C * (D + 4), kJoin = R * 64 * 2 + NW * kWave * 4;
+  __shared__ __align__(16) float lds[kRed > kJoin ? kRed : kJoin];
+  float(&red)[NW][C][D + 4] = *reinterpret_cast<float(*)[NW][C][D + 4]>(&lds);
+  __shared__ float red_m[NW][R], red_l[NW][R];
   const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int lg = lane / 16, col = lane % C, part = lane % 16 / C;
   const unsigned id = a.first + blockIdx.x, pair = id / (unsigned)a.hk;
@@ -244,14 +247,14 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 && RT == 1 ? 3 : 2))) void kv4_decod
   // ids of the turn after them.  The first go out before the queries are looked at.
   const auto id_of = [&](int g) { return group_of(a, t, h, min(g, end - 1)); };
   constexpr int kBufs = kAhead + 1;
-  int g = begin + wave, to = g + kAhead * kWaves;
+  int g = begin + wave, to = g + kAhead * NW;
   Bytes<D, N> b[kBufs];
   bool ok[kBufs];
   Group next;
   if (g < end) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const Group x = id_of(g + i * kWaves);
+      const Group x = id_of(g + i * NW);
       ok[i] = x.ok;
       fetch(a, x, lane, b[i]);
       __builtin_amdgcn_sched_barrier(0);  // (in this order: what is waited for is counted back)
@@ -434,19 +437,19 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 && RT == 1 ? 3 : 2))) void kv4_decod
       const int last = (now + kAhead) % kBufs;
       ok[last] = next.ok;
       fetch(a, next, lane, b[last]);
-      to += kWaves;
+      to += NW;
       next = id_of(to);
       // (they go out before anything of this turn waits for its own)
       __builtin_amdgcn_sched_barrier(0);
       step(b[now], g, ok[now]);
-      g += kWaves;
+      g += NW;
       return g < end;
     };
     while (turn(0) && turn(1)) {}
   }
 
   // ---- the four wavefronts' results
-  finish_tile<T, D, RT, W>(a, t, h, rows, split, share.splits, partial, id, m, l, acc, red, red_m, red_l);
+  finish_tile<T, D, RT, W, NW>(a, t, h, rows, split, share.splits, partial, id, m, l, acc, red, red_m, red_l);
 }
 
 // ---------------------------------------------------------------------------
@@ -818,12 +821,14 @@ hipError_t launch_sized(AttnArgs a, const PagedPlan& p, hipStream_t stream) {
     a.first = (unsigned)i;
     const unsigned grid = (unsigned)(p.grid - i < most ? p.grid - i : most);
     if (p.kernel == 1 && p.gangs == 1) kv4_prefill_kernel<T, D, 1><<<grid, kThreads, kLds, stream>>>(a);
-    else if (p.kernel == 0 && p.rows == 4) kv4_decode_kernel<T, D, 1, 4><<<grid, kThreads, 0, stream>>>(a);
-    else if (p.kernel == 0 && p.rows == 8) kv4_decode_kernel<T, D, 1, 2><<<grid, kThreads, 0, stream>>>(a);
-    else if (p.kernel == 0 && p.rows == 16) kv4_decode_kernel<T, D, 1, 1><<<grid, kThreads, 0, stream>>>(a);
+    else if (p.kernel == 0 && p.rows == 4 && p.gangs == 2) kv4_decode_kernel<T, D, 1, 4, 8><<<grid, 512, 0, stream>>>(a);
+    else if (p.kernel == 0 && p.rows == 8 && p.gangs == 2) kv4_decode_kernel<T, D, 1, 2, 8><<<grid, 512, 0, stream>>>(a);
+    else if (p.kernel == 0 && p.rows == 4) kv4_decode_kernel<T, D, 1, 4, 4><<<grid, kThreads, 0, stream>>>(a);
+    else if (p.kernel == 0 && p.rows == 8) kv4_decode_kernel<T, D, 1, 2, 4><<<grid, kThreads, 0, stream>>>(a);
+    else if (p.kernel == 0 && p.rows == 16) kv4_decode_kernel<T, D, 1, 1, 4><<<grid, kThreads, 0, stream>>>(a);
     else if constexpr (D <= 128) {
       if (p.kernel == 1) kv4_prefill_kernel<T, D, 2><<<grid, 2 * kThreads, kLds2, stream>>>(a);
-      else kv4_decode_kernel<T, D, 2, 1><<<grid, kThreads, 0, stream>>>(a);
+      else kv4_decode_kernel<T, D, 2, 1, 4><<<grid, kThreads, 0, stream>>>(a);
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -847,12 +852,69 @@ struct Kv4Costs {
   }
   static double token_bytes(int D) { return D + 4.0; }
   static int few(int64_t rows, int D) { return rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 || D > 128 ? 16 : 32; }
-  static double merge(int splits) { return 4.5 + 0.1 * splits; }
+  // The decode kernel, with four or eight wavefronts a workgroup, fitted to 1 x 100 to
+  // 131000 tokens of four head layouts at 1 to 64 splits on either: us of a turn, of what
+  // surrounds the turns, and of the join, which one workgroup does for a tile (32 rows
+  // of 128, 8 and 32 splits of 4000 tokens: 20.8 and 27 us, with the second kernel 13.9 and
+  // 14; 4 rows, 8 splits of 777: 8.6 and 8.2, but 9.4 and 11.8 for a caller that launches
+  // them itself: a call of one launch takes the host 8.7 us, one of two 11.7).
+  // Eight wavefronts halve the splits of long contexts (131000 tokens, 32 + 8 heads: 64
+  // splits of four 31.3 us, 32 of eight 29.5; 60000 tokens, 8 + 1 heads of 256: 27.5 and
+  // 22.7) and do without any in middling ones (777 tokens, 12 heads of 64: 7.5 and 6.8).
+  static Estimate decode(int64_t requests, int rows, double tiles, double groups, double longest, double tokens_heads,
+                         bool ragged, double shared, int most_rows, int D, int hk, int cus) {
+    const int held = rows < most_rows ? rows : most_rows, cap = most_splits(rows);
+    constexpr double kOneLaunch = 8.5, kTwoLaunches = 11.5;
+    Estimate best{1e30, 1, false};
+    for (int gangs = 1; gangs <= (rows <= 8 && requests == 1 ? 2 : 1); ++gangs) {
+      const double compute = rows <= 8 ? 1.0 : rows == 16 ? 1.15 : 1.65;
+      const double turn = compute * (D == 64 ? (gangs == 1 ? 0.43 : 0.63) : D == 128 ? (gangs == 1 ? 0.61 : 0.94)
+                                                                                     : (gangs == 1 ? 1.02 : 1.66));
+      const int slots = rows == 32 ? 2 : gangs == 1 ? (D == 64 ? 4 : D == 128 ? 3 : 2) : (D == 64 ? 2 : 1);
+      for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+        if (s > cap || (s > 1 && s > groups)) break;
+        const double turns = ceil(ceil(groups / s) / (kWaves * gangs)), w = tiles * hk * s;
+        const auto round = [&](double n) {  // n workgroups at a time
+          const double bytes = n * kWaves * gangs * 32.0 * token_bytes(D) * shared / (gangs == 1 ? 6.5e6 : 7.0e6);
+          const double beside = turn * (1.0 + 0.3 * (n > cus ? n / cus - 1.0 : 0.0));
+          return turns * (beside > bytes ? beside : bytes);
+        };
+        const double room = (double)cus * slots, full = floor(w / room), rest = w - full * room;
+        double us = 4.2 + 0.5 * gangs + full * round(room) + (rest >= 1 ? round(rest) : 0.0) + 1.5 * (ceil(w / room) - 1.0);
+        bool merge = false;
+        if (s > 1) {
+          const double join = 2.2 + 0.08 * s + held * D / 512.0 * (0.7 + 0.037 * s);
+          const double second = 2.9 + 0.09 * s + tokens_heads * s * D * 8.0 / 3e6;
+          // (a caller that does not replay graphs pays for the second launch)
+          merge = (second < join && us + join > kTwoLaunches) || tiles * hk > kMaxSplitCounters;
+          us += merge ? second : join;
+        }
+        const double host = merge ? kTwoLaunches : kOneLaunch, cost = (us > host ? us : host) + 0.1 * us;
+        if (cost < best.us) best = {cost, s, merge, gangs};
+      }
+    }
+    return best;
+  }
   // (tiles that the offsets might ask for, but that no batch of this length has, are
   // room in the grid and no workgroups to cut for: 48 requests, 776 workgroups on 256
   // CUs instead of 768 held up the last eight of them to the end, 51 -> 43 us)
   static constexpr bool aim = true;
-  static int share_least(int rows, int D) { return rows == 32 ? 32 : D == 256 ? 8 : 16; }
+  // Workgroups of a batch, a multiple of the CUs: those that a CU runs at a time where
+  // they get enough to do (16 requests of up to 15000 tokens, 32 + 8 heads, 1, 2, 3 and
+  // 4 a CU: 38.2, 31.6, 32.3, 36.3 us; of 15000 each 52.2, 51.9, 49.5, 54.7; of 4000 each
+  // 20.5, 19.9, 20.3, 24.4; 12 heads of 64, of 15000: 64.0, 47.5, 40.7, 41.8; 8 + 1 heads of
+  // 256: 22.0, 27.0, 37.4, 40.1), and room for the tiles to be cut.
+  static int64_t shares(double tiles, double groups, int D, int cus) {  // of all heads
+    const double most = D == 256 ? 1 : D == 64 || tiles * groups > 3 * 45.0 * cus ? 3 : 2;
+    const double room = ceil(1.5 * tiles / cus);
+    return (int64_t)(room > most ? room : most) * cus;
+  }
+  // (4 requests of up to 2000 tokens, 32 + 8 heads, 8, 12, 16 and 24 groups: 10.0, 10.4, 10.9,
+  // 12.0 us; 16 of those 12.4, 12.2, 13.0, 12.3; of up to 500 tokens 9.5, 10.2, 8.1, 8.1; 8 + 1
+  // heads of 256, 16 of up to 2000: 13.2, 14.2, 15.1, 16.9; of up to 500: 12.8, 13.6, 10.5, 10.5)
+  static int share_least(int rows, int D, double longest) {
+    return longest < 32 || rows == 32 ? 16 : D == 256 ? 8 : 12;
+  }
 };
 
 }  // namespace

@@ -8,31 +8,42 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// LP = D / 8 lanes hold one row (token, head, side), eight dimensions each; the
-// lanes after them hold the other side's row.  A workgroup takes the tokens of one
-// head, 256 / (2 LP) at a time, kTurns times: 32 tokens that follow each other are
-// what fills the cache lines they are written to.
+// ---------------------------------------------------------------------------
+// Append.  LP = D / 16 lanes hold one row (token, head, side), sixteen dimensions
+// each; the LP lanes after them hold the other side's row.  A workgroup takes 256 /
+// (2 LP) tokens of one head.  A prompt runs in one or two rounds of workgroups, which
+// load, compute and store one after the other, so what counts beside the bytes are
+// the vector instructions: 6874 tokens of 8 heads of 128 take 10.5 us (35.6 MB, 3.4
+// TB/s), with eight dimensions a lane and the numbers put together by shifts and ORs
+// 13.8.  Workgroups that take several tokens a lane gain nothing (2000 tokens: 5.0
+// us, in half as many workgroups 5.0; 1000: 3.1 and 3.8).
+// ---------------------------------------------------------------------------
 template <typename Op>
 __device__ __forceinline__ float over_lanes(float v, int lp, Op op) {
   const auto step = [&](auto ctrl) {
-    v = op(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl(), 0xf,
-                                                                    0xf, true)));
+    v = op(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl(), 0xf, 0xf,
+                                                                    true)));
   };
-  step([] { return 0xB1; });             // lanes 1, 0, 3, 2 of a quad
-  step([] { return 0x4E; });             // 2, 3, 0, 1
-  step([] { return 0x141; });            // mirrored in eight
+  step([] { return 0xB1; });                 // lanes 1, 0, 3, 2 of a quad
+  step([] { return 0x4E; });                 // 2, 3, 0, 1
+  if (lp >= 8) step([] { return 0x141; });   // mirrored in eight
   if (lp >= 16) step([] { return 0x140; });  // mirrored in sixteen
-  if (lp >= 32) v = op(v, __shfl_xor(v, 16));
   return v;
 }
 
-// rint(x / s), where r is 1 / s to an ulp: the quotient's one correction, t + r (x -
-// t s) (Markstein 1990), makes it exact where it is a tie, and x / s with x of 11
-// bits and s of 7 is at least 2^-19 of itself away from every other one.
-__device__ __forceinline__ float rounded_quotient(float x, float s, float r) {
+// x / s, where r is 1 / s to an ulp: the quotient's one correction, t + r (x - t s)
+// (Markstein 1990), makes it exact where it is a tie, and x / s with x of 11 bits and
+// s of 7 is at least 2^-19 of itself away from every other one.
+__device__ __forceinline__ float quotient(float x, float s, float r) {
   const float t = x * r;
-  return __builtin_rintf(__builtin_fmaf(__builtin_fmaf(-t, s, x), r, t));
+  return __builtin_fmaf(__builtin_fmaf(-t, s, x), r, t);
 }
+
+// The bits of 1.5 2^23: the sum with a small number holds its nearest integer (ties
+// to even) in its low bits, and sums of those with shifts of 4, 8, .. put numbers
+// next to each other.
+constexpr float kMagic = 12582912.0f;
+constexpr int kMagicBits = 0x4b400000;
 
 struct AppendArgs {
   const uint8_t* x[2];   // k, v
@@ -44,78 +55,92 @@ struct AppendArgs {
   int heads, shift;      // log2(block size)
 };
 
-template <typename T, int D, int kTurns>
+template <typename T, int D>
 __global__ __launch_bounds__(kThreads) void kv4_append_kernel(AppendArgs a) {
-  constexpr int LP = D / 8, kTokens = kThreads / (2 * LP);
-  const int tid = threadIdx.x, sub = tid % LP, side = tid / LP % 2, d = sub * 8;
+  constexpr int LP = D / 16, kTokens = kThreads / (2 * LP);
+  const int tid = threadIdx.x, sub = tid % LP, side = tid / LP % 2, d = sub * 16;
   const unsigned part = blockIdx.x / (unsigned)a.heads;
   const int h = (int)(blockIdx.x - part * a.heads);
-  const int64_t t0 = (int64_t)part * (kTokens * kTurns) + tid / (2 * LP);
+  const int64_t t = (int64_t)part * kTokens + tid / (2 * LP);
   const uint8_t* src = (side ? a.x[1] : a.x[0]) + h * (side ? a.hs[1] : a.hs[0]) + d * 2;
-  const int64_t ts = side ? a.ts[1] : a.ts[0];
-  uint4 raw[kTurns];
-  int32_t slot[kTurns];
-#pragma unroll
-  for (int i = 0; i < kTurns; ++i) {
-    const int64_t t = t0 + i * kTokens;
-    raw[i] = make_uint4(0, 0, 0, 0);
-    slot[i] = -1;
-    if (t < a.tokens) {
-      raw[i] = load_u4(src + t * ts);
-      slot[i] = a.slots[t];
-    }
+  uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+  int32_t slot = -1;
+  if (t < a.tokens) {
+    src += t * (side ? a.ts[1] : a.ts[0]);
+    raw[0] = load_u4(src);
+    raw[1] = load_u4(src + 16);
+    slot = a.slots[t];
   }
+  float x[16];
 #pragma unroll
-  for (int i = 0; i < kTurns; ++i) {
-    const floatx8 x = Eight<T>::load(&raw[i]);
-    float low = 0.0f, high = 0.0f, nan = 0.0f;
+  for (int j = 0; j < 2; ++j) {
+    const floatx8 f = Eight<T>::load(&raw[j]);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      low = fminf(low, x[j]);
-      high = fmaxf(high, x[j]);
-      nan = __builtin_fmaf(x[j], 0.0f, nan);  // (NaN where x is not finite)
-    }
-    low = over_lanes(low, LP, [](float u, float v) { return fminf(u, v); });
-    high = over_lanes(high, LP, [](float u, float v) { return fmaxf(u, v); });
-    // either side of the token's row
-    const uint64_t odd = __ballot(nan != nan);
-    const int lane = tid % kWave, from = lane / (2 * LP) * (2 * LP);
-    const bool bad = (odd >> from & (~0ull >> (kWave - 2 * LP))) != 0;
-    const float span = high - low;
-    // the least step of seven bits (of 2^-20 where fp16 has no more) with 15 of it
-    // at least the span: span / 15 cut to those bits, and one up where that was less
-    const float least = fminf(fmaxf(span * (1.0f / 15.0f), 0x1p-20f), 4352.0f);
-    const uint32_t power = __builtin_bit_cast(uint32_t, least) & 0x7f800000u;
-    const float ulp = fmaxf(__builtin_bit_cast(float, power) * 0x1p-6f, 0x1p-20f);
-    const float inv = __builtin_bit_cast(float, 0x7f000000u - __builtin_bit_cast(uint32_t, ulp));
-    float s = __builtin_truncf(least * inv) * ulp;
-    if (15.0f * s < span) s = fminf(s + ulp, 4352.0f);
-    const float r = __builtin_amdgcn_rcpf(s);
-    const float z = fminf(rounded_quotient(-low, s, r), 15.0f);
-    uint32_t n[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      n[j] = (uint32_t)__builtin_amdgcn_fmed3f(rounded_quotient(x[j], s, r) + z, 0.0f, 15.0f);
-    uint32_t word = __builtin_bit_cast(uint16_t, (_Float16)s) | (uint32_t)z;
-    uint32_t even = n[0] | n[2] << 4 | n[4] << 8 | n[6] << 12, odds = n[1] | n[3] << 4 | n[5] << 8 | n[7] << 12;
-    uint32_t lo = n[0] | n[1] << 4 | n[2] << 8 | n[3] << 12, hi = n[4] | n[5] << 4 | n[6] << 8 | n[7] << 12;
-    if (bad) {
-      word = side ? RF_KV4_EMPTY : RF_KV4_NAN;
-      even = odds = lo = hi = 0;
-    }
-    const int64_t block = slot[i] >> a.shift;
-    if (slot[i] < 0 || block >= a.num_blocks) continue;
-    const int o = slot[i] & ((1 << a.shift) - 1);
-    const int64_t group = (block * a.heads + h) * (1 << (a.shift - 5)) + o / 32;
-    if (side) {
-      uint8_t* p = a.store[1] + group * (16 * D) + v4_at<D>(o % 32, d);
-      *reinterpret_cast<uint16_t*>(p) = (uint16_t)lo;
-      *reinterpret_cast<uint16_t*>(p + 16) = (uint16_t)hi;
-    } else {
-      *reinterpret_cast<uint32_t*>(a.store[0] + group * (16 * D) + k4_at<D>(o % 32, d)) = even | odds << 16;
-    }
-    if (sub == 0) a.rows[group * 64 + side * 32 + o % 32] = (uint16_t)word;
+    for (int e = 0; e < 8; ++e) x[8 * j + e] = f[e];
   }
+  float low = 0.0f, high = 0.0f;  // (NaN where an x is)
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    low = __builtin_elementwise_minimum(low, x[j]);
+    high = __builtin_elementwise_maximum(high, x[j]);
+  }
+  // an infinity or NaN on either side of the token's row
+  const uint64_t odd = __ballot(!(high < __builtin_inff()) || !(low > -__builtin_inff()));
+  const int lane = tid % kWave, from = lane / (2 * LP) * (2 * LP);
+  const bool bad = (odd >> from & (~0ull >> (kWave - 2 * LP))) != 0;
+  low = over_lanes(low, LP, [](float u, float v) { return fminf(u, v); });
+  high = over_lanes(high, LP, [](float u, float v) { return fmaxf(u, v); });
+  const float span = high - low;
+  // the least step of seven bits (of 2^-20 where fp16 has no more) with 15 of it
+  // at least the span: span / 15 cut to those bits, and one up where that was less
+  const float least = fminf(fmaxf(span * (1.0f / 15.0f), 0x1p-20f), 4352.0f);
+  const uint32_t power = __builtin_bit_cast(uint32_t, least) & 0x7f800000u;
+  const float ulp = fmaxf(__builtin_bit_cast(float, power) * 0x1p-6f, 0x1p-20f);
+  const float inv = __builtin_bit_cast(float, 0x7f000000u - __builtin_bit_cast(uint32_t, ulp));
+  float s = __builtin_truncf(least * inv) * ulp;
+  if (15.0f * s < span) s = fminf(s + ulp, 4352.0f);
+  const float r = __builtin_amdgcn_rcpf(s);
+  const int z = (int)fminf(__builtin_rintf(quotient(-low, s, r)), 15.0f);
+  // numbers plus (magic - z), within magic - z .. magic - z + 15
+  const int base = kMagicBits - z;
+  const float least_n = __builtin_bit_cast(float, base), most_n = __builtin_bit_cast(float, base + 15);
+  uint32_t word[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    uint32_t sum = 0;
+#pragma unroll
+    for (int e = 7; e >= 0; --e) {
+      const float n = __builtin_amdgcn_fmed3f(quotient(x[8 * j + e], s, r) + kMagic, least_n, most_n);
+      sum = (sum << 4) + __builtin_bit_cast(uint32_t, n);
+    }
+    word[j] = sum - (uint32_t)base * 0x11111111u;
+  }
+  uint32_t row = __builtin_bit_cast(uint16_t, (_Float16)s) | (uint32_t)z;
+  if (bad) {
+    row = side ? RF_KV4_EMPTY : RF_KV4_NAN;
+    word[0] = word[1] = 0;
+  }
+  const int64_t block = slot >> a.shift;
+  if (slot < 0 || block >= a.num_blocks) return;
+  const int o = slot & ((1 << a.shift) - 1);
+  const int64_t group = (block * a.heads + h) * (1 << (a.shift - 5)) + o / 32;
+  if (side) {
+    uint8_t* p = a.store[1] + group * (16 * D) + v4_at<D>(o % 32, d);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      *reinterpret_cast<uint16_t*>(p + 16 * j) = (uint16_t)(word[j / 2] >> (16 * (j % 2)));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {  // even dimensions to the low half, odd ones to the high half
+      uint32_t w = word[j];
+      uint32_t m = (w ^ (w >> 4)) & 0x00f000f0u;
+      w ^= m ^ (m << 4);
+      m = (w ^ (w >> 8)) & 0x0000ff00u;
+      word[j] = w ^ m ^ (m << 8);
+    }
+    *reinterpret_cast<uint2*>(a.store[0] + group * (16 * D) + k4_at<D>(o % 32, d)) = make_uint2(word[0], word[1]);
+  }
+  if (sub == 0) a.rows[group * 64 + side * 32 + o % 32] = (uint16_t)row;
 }
 
 // ---------------------------------------------------------------------------
@@ -261,30 +286,19 @@ __global__ __launch_bounds__(kThreads) void kv4_read_kernel(ReadArgs a) {
 
 inline int log2i(int v) { return __builtin_ctz((unsigned)v); }
 
-// Workgroups of one turn while they leave CUs idle, of 32 tokens after.
-template <int D>
-bool few(int64_t tokens, int heads) {
-  return tokens * heads <= 256 * (kThreads / (D / 4)) * 4;
-}
-
-template <typename T, int D, int kTurns>
-hipError_t append_turns(AppendArgs a, hipStream_t stream) {
-  constexpr int64_t kTokens = kThreads / (D / 4) * kTurns;
+template <typename T, int D>
+hipError_t append_sized(AppendArgs a, hipStream_t stream) {
+  constexpr int64_t kTokens = kThreads / (D / 8);
   const int64_t most = kMaxThreads / kThreads / a.heads * kTokens;  // tokens of a launch
   for (int64_t left = a.tokens; left > 0; left -= most) {
     a.tokens = left < most ? left : most;
-    kv4_append_kernel<T, D, kTurns><<<(unsigned)(ceil_div(a.tokens, kTokens) * a.heads), kThreads, 0, stream>>>(a);
+    kv4_append_kernel<T, D><<<(unsigned)(ceil_div(a.tokens, kTokens) * a.heads), kThreads, 0, stream>>>(a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     a.slots += a.tokens;
     for (int i = 0; i < 2; ++i) a.x[i] += a.tokens * a.ts[i];
   }
   return hipSuccess;
-}
-
-template <typename T, int D>
-hipError_t append_sized(const AppendArgs& a, hipStream_t stream) {
-  return few<D>(a.tokens, a.heads) ? append_turns<T, D, 1>(a, stream) : append_turns<T, D, D / 32>(a, stream);
 }
 
 template <typename T>

@@ -804,9 +804,16 @@ struct Kv8Costs {
   static double token_bytes(int D) { return 2.0 * D; }
   // (two tiles of 16 rows of size 256 would not fit the registers)
   static int few(int64_t rows, int D) { return rows <= 16 || D > 128 ? 16 : 32; }
-  static double merge(int splits) { return 4.5; }
+  static Estimate decode(int64_t requests, int rows, double tiles, double groups, double longest, double tokens_heads,
+                         bool ragged, double shared, int most_rows, int D, int hk, int cus) {
+    return estimate<Kv8Costs>(false, 1, rows, tiles, groups, longest, tokens_heads, ragged, shared, most_rows, D, hk, cus);
+  }
   static constexpr bool aim = false;
-  static int share_least(int rows, int D) { return rows == 32 ? 32 : D == 256 ? 8 : 16; }
+  // (the multiple of the CUs that leaves tiles half a share each to cut)
+  static int64_t shares(double tiles, double groups, int D, int cus) {
+    return ceil_div(3 * (int64_t)tiles, 2 * cus) * cus;
+  }
+  static int share_least(int rows, int D, double longest) { return rows == 32 ? 32 : D == 256 ? 8 : 16; }
 };
 
 }  // namespace

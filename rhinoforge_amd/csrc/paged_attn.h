@@ -371,14 +371,14 @@ __device__ __forceinline__ void finish(const PagedArgs& a, int64_t to, int D, in
 // A split with nothing to do, for merge_splits_kernel.
 __device__ __forceinline__ void no_share(const PagedArgs& a, const Tile& t, int h, int rows, int split) {
   const Partials parts(a);
-  for (int rc = threadIdx.x; rc < rows; rc += kThreads)
+  for (int rc = threadIdx.x; rc < rows; rc += blockDim.x)
     parts.store_stat((int)out_row(a, t, h, rc) * a.splits + split, -__builtin_inff(), 0.0f);
 }
 
 // All threads call it after their stores of partial results.  buf: LDS of
-// rows * splits * 8 + 4096 bytes, free for use.  Row rc of split s is at
+// rows * splits * 8 + 16 kT bytes, free for use; kT threads.  Row rc of split s is at
 // first + s * stride + rc of the partial results.
-template <typename T, int D>
+template <typename T, int D, int kT = kThreads>
 __device__ __forceinline__ void join(const PagedArgs& a, const Tile& t, int h, int rows, int splits,
                                      int first, int stride, uint32_t* counter, float* buf) {
   const int tid = threadIdx.x;
@@ -400,23 +400,24 @@ __device__ __forceinline__ void join(const PagedArgs& a, const Tile& t, int h, i
   constexpr int kFlight = 8;
   const int units = rows * (D / 4);
   int ways = 1;
-  while (units * ways * 2 <= kThreads && ways * 2 <= splits) ways *= 2;
+  while (units * ways * 2 <= kT && ways * 2 <= splits) ways *= 2;
   float* stat = buf;  // [rows][splits][2^(m - the row's), l]
   floatx4* sums = reinterpret_cast<floatx4*>(buf + (rows * splits * 2 + 3) / 4 * 4);
   __shared__ float tops[kMaxRows];
-  // A wavefront takes every fourth row, a lane one of its splits (at most 64).
+  constexpr int kEach = kMaxRows / (kT / kWave);
+  // A wavefront takes some of the rows, a lane one of its splits (at most 64).
   const int lane = tid % kWave, wave = tid / kWave;
-  floatx2 own[kMaxRows / kWaves];
+  floatx2 own[kEach];
 #pragma unroll
-  for (int i = 0; i < kMaxRows / kWaves; ++i) {
+  for (int i = 0; i < kEach; ++i) {
     own[i] = floatx2{-__builtin_inff(), 0.0f};
-    const int rc = wave + i * kWaves;
+    const int rc = wave + i * (kT / kWave);
     if (rc < rows && lane < splits) own[i] = parts.load_stat(first + lane * stride + rc);
   }
   const auto factors = [&] {
 #pragma unroll
-    for (int i = 0; i < kMaxRows / kWaves; ++i) {
-      const int rc = wave + i * kWaves;
+    for (int i = 0; i < kEach; ++i) {
+      const int rc = wave + i * (kT / kWave);
       if (rc >= rows) break;
       float m = own[i][0];
 #pragma unroll
@@ -427,7 +428,7 @@ __device__ __forceinline__ void join(const PagedArgs& a, const Tile& t, int h, i
             floatx2{exp2_fast(own[i][0] - safe(m)), own[i][1]};
     }
   };
-  for (int u0 = 0; u0 < units; u0 += kThreads) {
+  for (int u0 = 0; u0 < units; u0 += kT) {
     const int way = ways == 1 ? 0 : (int)((unsigned)tid / (unsigned)units);
     const int u = u0 + (ways == 1 ? tid : tid - way * units);
     const bool on = u < units && way < ways;
@@ -462,7 +463,7 @@ __device__ __forceinline__ void join(const PagedArgs& a, const Tile& t, int h, i
         if (s < splits) o += y[k] * st[s][0];
       }
     }
-    if (ways > 1) {  // (units < kThreads: one turn of the outer loop)
+    if (ways > 1) {  // (units < kT: one turn of the outer loop)
       sums[tid] = o;
       __syncthreads();
       if (on && way == 0)
@@ -514,13 +515,14 @@ struct Estimate {
   double us;
   int splits;
   bool merge;
+  int gangs = 1;
 };
 
 // Times of the kernels, fitted (Costs, one for each cache): base and more, us of a
 // workgroup's turn alone and for each workgroup beside it on its CU; slots, the
 // workgroups that a CU runs at a time; token_bytes, a token's keys and values; few, rows of a
-// tile of the decode kernel; merge, us of the second kernel before its bytes; aim,
-// whether shares are cut for the workgroups that run at a time, not for all in the grid;
+// tile of the decode kernel; decode, its estimate; aim, whether shares are cut for the
+// workgroups that run at a time, not for all in the grid; shares, how many those are;
 // share_least, 32-token groups of a share, at least.
 template <typename Costs>
 Estimate estimate(bool prefill, int gangs, int rows, double tiles, double groups, double longest, double tokens_heads, bool ragged,
@@ -550,7 +552,7 @@ Estimate estimate(bool prefill, int gangs, int rows, double tiles, double groups
     if (s > 1) {
       const double units = held * (D / 4), ways = units < kThreads ? kThreads / units : 1.0;
       const double join = 2.0 + 1.2 * ceil(units / kThreads) * ceil(s / (8.0 * ways));
-      const double second = Costs::merge(s) + tokens_heads * s * D * 8.0 / 3e6;
+      const double second = 4.5 + tokens_heads * s * D * 8.0 / 3e6;
       merge = prefill || second < join || tiles * hk > kMaxSplitCounters;
       us += merge ? second : join;
     }
@@ -598,9 +600,10 @@ PagedPlan plan_paged_attention(const PagedShape& a, int cus) {
   const double tokens_heads = (double)a.tokens * a.heads, longest = most_kv / (double)RF_KV8_GROUP + 0.5;
   const int few = Costs::few(most_rows, D);
   const int most = (int)(most_rows < 1024 ? most_rows : 1024);
-  Estimate e = estimate<Costs>(false, 1, few, (double)useful(few), groups(few), longest, tokens_heads, ragged,
-                        1.0 / ceil_div(most_rows, few), most, D, (int)hk, cus);
+  Estimate e = Costs::decode(a.requests, few, (double)useful(few), groups(few), longest, tokens_heads, ragged,
+                             1.0 / ceil_div(most_rows, few), most, D, (int)hk, cus);
   p.kernel = 0;
+  p.gangs = e.gangs;
   p.rows = few;
   if (most_rows > 16) {
     for (int gangs = 1; gangs <= (D == 256 ? 1 : 2); ++gangs) {
@@ -614,7 +617,7 @@ PagedPlan plan_paged_attention(const PagedShape& a, int cus) {
     }
   }
   p.tiles = bound(p.rows);
-  p.least = p.kernel ? (D == 256 ? 1 : 2) : kWaves;
+  p.least = p.kernel ? (D == 256 ? 1 : 2) : kWaves * p.gangs;
   p.splits = e.splits;
   p.merge = e.merge;
   p.grid = p.tiles * hk * p.splits;
@@ -625,12 +628,11 @@ PagedPlan plan_paged_attention(const PagedShape& a, int cus) {
     return p.workspace <= 0x7fffffff && grid <= (p.merge ? 0x7fffffff : kMaxSplitCounters);
   };
   // (the sums of tiles times groups fit, whatever the offsets say)
-  if (p.kernel == 0 && !p.merge && a.requests > 1 && a.requests < kShareRequests &&
+  if (p.kernel == 0 && p.gangs == 1 && !p.merge && a.requests > 1 && a.requests < kShareRequests &&
       (double)p.tiles * (double)a.requests * (double)(a.width * a.block_size / RF_KV8_GROUP + 1) < 2147483647.0) {
-    // Workgroups: the multiple of the CUs that leaves tiles half a share each to
-    // cut, in shares that are long enough for the join they cost (what was
-    // measured stands at each Costs).
-    int64_t shares = ceil_div(3 * useful(p.rows) * hk, 2 * cus) * cus / hk;
+    // Shares that are long enough for the join they cost (what was measured stands
+    // at each Costs).
+    int64_t shares = Costs::shares((double)(useful(p.rows) * hk), groups(p.rows), D, cus) / hk;
     p.aim = (int)shares;
     if (shares < p.tiles) shares = p.tiles;
     if (!Costs::aim || p.aim < 1) p.aim = (int)shares;
@@ -639,7 +641,7 @@ PagedPlan plan_paged_attention(const PagedShape& a, int cus) {
     if (shares * hk <= 16 * cus && fits(shares * hk * p.rows, shares * hk)) {
       p.shares = (int)shares;
       p.splits = most_splits(p.rows);
-      p.least = Costs::share_least(p.rows, D);
+      p.least = Costs::share_least(p.rows, D, longest);
       p.grid = shares * hk;
       return p;
     }
