@@ -852,6 +852,14 @@ struct Kv4Costs {
   }
   static double token_bytes(int D) { return D + 4.0; }
   static int few(int64_t rows, int D) { return rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 || D > 128 ? 16 : 32; }
+  // Tiles are not cut where they are short, or so many that the CUs have others to go on
+  // with (200 requests of up to 1000 tokens, 64 + 8 heads: 32 us, cut 41; 128 of up to
+  // 8000 105.8 and 107.6; 48 of those 62.1 and 46.5; 12 heads of 64, 128 of up to 2000: 29.1
+  // and 34.5; 64 of up to 4000 31.9 and 30.2; 8 + 1 heads of 256, 400 of up to 2000: 33.5
+  // and 47.5; 128 of those 23.0 and 18.2).
+  static bool cut(double tiles, double longest, int D, int cus) {
+    return longest > 33 && tiles < cus * (D == 64 ? 4.0 : D == 128 ? 2.0 : 1.5);
+  }
   // The decode kernel, with four or eight wavefronts a workgroup, fitted to 1 x 100 to
   // 131000 tokens of four head layouts at 1 to 64 splits on either: us of a turn, of what
   // surrounds the turns, and of the join, which one workgroup does for a tile (32 rows
@@ -865,6 +873,7 @@ struct Kv4Costs {
                          bool ragged, double shared, int most_rows, int D, int hk, int cus) {
     const int held = rows < most_rows ? rows : most_rows, cap = most_splits(rows);
     constexpr double kOneLaunch = 8.5, kTwoLaunches = 11.5;
+    const bool whole = requests > 1 && !cut(tiles * hk, longest, D, cus);
     Estimate best{1e30, 1, false};
     for (int gangs = 1; gangs <= (rows <= 8 && requests == 1 ? 2 : 1); ++gangs) {
       const double compute = rows <= 8 ? 1.0 : rows == 16 ? 1.15 : 1.65;
@@ -872,7 +881,7 @@ struct Kv4Costs {
                                                                                      : (gangs == 1 ? 1.02 : 1.66));
       const int slots = rows == 32 ? 2 : gangs == 1 ? (D == 64 ? 4 : D == 128 ? 3 : 2) : (D == 64 ? 2 : 1);
       for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
-        if (s > cap || (s > 1 && s > groups)) break;
+        if (s > cap || (s > 1 && (s > groups || whole))) break;
         const double turns = ceil(ceil(groups / s) / (kWaves * gangs)), w = tiles * hk * s;
         const auto round = [&](double n) {  // n workgroups at a time
           const double bytes = n * kWaves * gangs * 32.0 * token_bytes(D) * shared / (gangs == 1 ? 6.5e6 : 7.0e6);
@@ -895,9 +904,8 @@ struct Kv4Costs {
     }
     return best;
   }
-  // (tiles that the offsets might ask for, but that no batch of this length has, are
-  // room in the grid and no workgroups to cut for: 48 requests, 776 workgroups on 256
-  // CUs instead of 768 held up the last eight of them to the end, 51 -> 43 us)
+  // (48 requests of up to 9000 tokens, 64 + 8 heads: 776 workgroups, four on eight of the
+  // CUs and three on the others, take 60 us, 768 of them 52)
   static constexpr bool aim = true;
   // Workgroups of a batch, a multiple of the CUs: those that a CU runs at a time where
   // they get enough to do (16 requests of up to 15000 tokens, 32 + 8 heads, 1, 2, 3 and

@@ -808,6 +808,7 @@ struct Kv8Costs {
                          bool ragged, double shared, int most_rows, int D, int hk, int cus) {
     return estimate<Kv8Costs>(false, 1, rows, tiles, groups, longest, tokens_heads, ragged, shared, most_rows, D, hk, cus);
   }
+  static bool cut(double, double, int, int) { return true; }
   static constexpr bool aim = false;
   // (the multiple of the CUs that leaves tiles half a share each to cut)
   static int64_t shares(double tiles, double groups, int D, int cus) {

@@ -71,68 +71,20 @@ __device__ __forceinline__ T read_scalar(const T* p, int64_t i) {
   return reinterpret_cast<const __attribute__((address_space(4))) T*>(reinterpret_cast<uintptr_t>(p))[i];
 }
 
-__device__ __forceinline__ int cu_at(const PagedArgs& a, int b) {
-  if (b <= 0) return 0;
-  if (b > a.requests) return a.tokens;
-  return min(max(a.cu[b], 0), a.tokens);
+// First token of request b's queries and its keys, for any b >= 0 (b >= requests: the
+// tokens past the batch, which see nothing).  No branches, and loads apart from what
+// looks at them: the compiler waits for a load at the end of a branch.
+__device__ __forceinline__ int read_cu(const PagedArgs& a, int b) { return a.cu[min(b, a.requests)]; }
+__device__ __forceinline__ int read_len(const PagedArgs& a, int b) { return a.lens[min(b, a.requests - 1)]; }
+__device__ __forceinline__ int checked_cu(const PagedArgs& a, int b, int c) {
+  const int lo = b > a.requests ? a.tokens : 0, hi = b <= 0 ? 0 : a.tokens;
+  return min(max(c, lo), hi);
 }
-
-// Tile x of the launch: request b's tiles begin at floor(cu[b] group / R) + b,
-// which leaves room for all of them.  Each lane looks at one boundary (and up
-// to 62 requests at their lengths too: one memory round trip); more requests
-// take a round per factor of 64.
-template <int R>
-__device__ __forceinline__ bool find_tile(const PagedArgs& a, int x, Tile* t) {
-  int b, len;
-  if (a.cu == nullptr) {
-    const int per = (a.per_request * a.group + R - 1) / R;
-    b = (int)((unsigned)x / (unsigned)per);
-    if (b >= a.requests) return false;
-    t->first_token = b * a.per_request;
-    t->queries = a.per_request;
-    t->row0 = (x - b * per) * R;
-    len = a.lens[b];
-  } else {
-    const int lane = threadIdx.x % kWave;
-    const auto begin = [&](int c, int i) { return (int)((int64_t)c * a.group / R) + i; };
-    int first, next;
-    if (a.requests < kWave - 1) {
-      const int c = cu_at(a, lane);
-      const int n = lane < a.requests ? a.lens[lane] : 0;
-      const int hits = __popcll(__ballot(lane <= a.requests && begin(c, lane) <= x));
-      b = hits - 1;
-      first = __builtin_amdgcn_readlane(c, b);
-      next = __builtin_amdgcn_readlane(c, b + 1);
-      len = __builtin_amdgcn_readlane(n, b);
-    } else {
-      int lo = 0, n = a.requests + 1;  // the answer is in [lo, lo + n)
-      while (n > 1) {
-        const int step = (n + kWave - 1) / kWave, at = lo + lane * step;
-        const bool below = at < lo + n && begin(cu_at(a, at), at) <= x;
-        const int hits = __popcll(__ballot(below));
-        const int base = lo + (hits > 0 ? hits - 1 : 0) * step;
-        n = min(step, lo + n - base);
-        lo = base;
-      }
-      b = __builtin_amdgcn_readfirstlane(lo);
-      first = cu_at(a, b);
-      next = cu_at(a, b + 1);
-      len = b < a.requests ? a.lens[b] : 0;
-    }
-    t->first_token = first;
-    t->queries = max(next - first, 0);
-    t->row0 = (x - begin(first, b)) * R;
-  }
-  if (t->row0 < 0 || t->row0 >= t->queries * a.group) return false;
-  // (b == requests: the tokens past the batch, which see nothing)
-  b = uniform(b);
-  t->first_token = uniform(t->first_token);
-  t->queries = uniform(t->queries);
-  t->row0 = uniform(t->row0);
-  t->kv_len = uniform(min(max(len, 0), a.width << a.shift));
-  t->table = a.table + (b < a.requests ? b * a.table_stride : 0);
-  return true;
+__device__ __forceinline__ int checked_len(const PagedArgs& a, int b, int len) {
+  return min(max(len, 0), b < a.requests ? a.width << a.shift : 0);
 }
+__device__ __forceinline__ int cu_at(const PagedArgs& a, int b) { return checked_cu(a, b, read_cu(a, b)); }
+__device__ __forceinline__ int len_at(const PagedArgs& a, int b) { return checked_len(a, b, read_len(a, b)); }
 
 // Sums and maxima over the lanes up to each one.
 template <typename Op>
@@ -143,6 +95,90 @@ __device__ __forceinline__ int scan(int v, Op op) {  // op(v, 0) == v
   v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false));  // row_shr:8
   v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));  // row_bcast:15
   return op(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));  // row_bcast:31
+}
+
+// Requests up to which every workgroup counts all tiles: eight of them a lane.
+constexpr int kCountRequests = 512;
+
+// Tile x of the launch.  The wavefront counts the tiles of up to 512 requests, whose
+// offsets and lengths it reads at once, so that the tiles follow each other and what the
+// grid has more, for any offsets, ends after them.  (With tiles at places that the
+// offsets alone give, floor(cu[b] group / R) + b, half the workgroups of a batch of
+// single tokens were empty ones among the others: 128 x 300 tokens, 64 + 8 heads of a
+// 4-bit cache 25 us, now 14.5.)  More requests are found like that, 64 boundaries at a
+// time.
+template <int R>
+__device__ __forceinline__ bool find_tile(const PagedArgs& a, int x, Tile* t) {
+  int b, len;
+  if (a.cu == nullptr) {
+    const int per = (a.per_request * a.group + R - 1) / R;
+    b = (int)((unsigned)x / (unsigned)per);
+    if (b >= a.requests) return false;
+    t->first_token = b * a.per_request;
+    t->queries = a.per_request;
+    t->row0 = (x - b * per) * R;
+    len = len_at(a, b);
+  } else if (a.requests < kCountRequests) {
+    const int lane = threadIdx.x % kWave;
+    constexpr int kChunks = kCountRequests / kWave;
+    int first[kChunks], next[kChunks], lens[kChunks];
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i)
+      if (i == 0 || i * kWave <= a.requests) {
+        const int at = i * kWave + lane;
+        first[i] = read_cu(a, at);
+        next[i] = read_cu(a, at + 1);
+        lens[i] = read_len(a, at);
+      }
+    int before = 0;
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i)
+      if (!found && (i == 0 || i * kWave <= a.requests)) {
+        const int at = i * kWave + lane, from = checked_cu(a, at, first[i]);
+        const int queries = max(checked_cu(a, at + 1, next[i]) - from, 0);
+        const int tiles = (int)(((unsigned)(queries * a.group) + R - 1) / R);
+        const int upto = scan(tiles, [](int u, int v) { return u + v; }) + before;
+        const int holder = __popcll(__ballot(upto <= x));
+        found = holder < kWave;
+        if (found) {
+          b = i * kWave + holder;
+          t->first_token = __builtin_amdgcn_readlane(from, holder);
+          t->queries = __builtin_amdgcn_readlane(queries, holder);
+          t->row0 = (x - __builtin_amdgcn_readlane(upto - tiles, holder)) * R;
+          len = checked_len(a, b, __builtin_amdgcn_readlane(lens[i], holder));
+        } else {
+          before = __builtin_amdgcn_readlane(upto, kWave - 1);
+        }
+      }
+    if (!found) return false;
+  } else {
+    const int lane = threadIdx.x % kWave;
+    const auto begin = [&](int c, int i) { return (int)((int64_t)c * a.group / R) + i; };
+    int lo = 0, n = a.requests + 1;  // the answer is in [lo, lo + n)
+    while (n > 1) {
+      const int step = (n + kWave - 1) / kWave, at = lo + lane * step;
+      const bool below = at < lo + n && begin(cu_at(a, at), at) <= x;
+      const int hits = __popcll(__ballot(below));
+      const int base = lo + (hits > 0 ? hits - 1 : 0) * step;
+      n = min(step, lo + n - base);
+      lo = base;
+    }
+    b = __builtin_amdgcn_readfirstlane(lo);
+    const int first = cu_at(a, b);
+    t->first_token = first;
+    t->queries = max(cu_at(a, b + 1) - first, 0);
+    t->row0 = (x - begin(first, b)) * R;
+    len = len_at(a, b);
+  }
+  if (t->row0 < 0 || t->row0 >= t->queries * a.group) return false;
+  b = uniform(b);
+  t->first_token = uniform(t->first_token);
+  t->queries = uniform(t->queries);
+  t->row0 = uniform(t->row0);
+  t->kv_len = uniform(len);
+  t->table = a.table + (b < a.requests ? b * a.table_stride : 0);
+  return true;
 }
 
 // Tokens [lo, hi) that row `row` of a request sees.
@@ -169,11 +205,16 @@ __device__ __forceinline__ bool find_share(const PagedArgs& a, int x, Tile* t, i
   };
   const int lane = threadIdx.x % kWave, entries = a.requests + (a.cu ? 1 : 0);
   const int per = (int)((unsigned)(entries + kWave - 1) / kWave);
-  const auto entry = [&](int b) {  // (b == requests: the tokens past the batch, which see nothing)
+  const auto entry = [&](int b) {
     Entry e;
-    e.len = b < a.requests ? min(max(a.lens[b], 0), a.width << a.shift) : 0;
-    e.first = a.cu ? cu_at(a, b) : b * a.per_request;
-    e.queries = b >= entries ? 0 : a.cu ? max(cu_at(a, b + 1) - e.first, 0) : a.per_request;
+    e.len = len_at(a, b);
+    e.first = b * a.per_request;
+    e.queries = a.per_request;
+    if (a.cu) {
+      e.first = cu_at(a, b);
+      e.queries = max(cu_at(a, b + 1) - e.first, 0);
+    }
+    if (b >= entries) e.queries = 0;
     e.tiles = (int)(((unsigned)(e.queries * a.group) + R - 1) / R);
     int lo = 0;
     if (a.causal && a.window > 0) {
@@ -521,9 +562,10 @@ struct Estimate {
 // Times of the kernels, fitted (Costs, one for each cache): base and more, us of a
 // workgroup's turn alone and for each workgroup beside it on its CU; slots, the
 // workgroups that a CU runs at a time; token_bytes, a token's keys and values; few, rows of a
-// tile of the decode kernel; decode, its estimate; aim, whether shares are cut for the
-// workgroups that run at a time, not for all in the grid; shares, how many those are;
-// share_least, 32-token groups of a share, at least.
+// tile of the decode kernel; decode, its estimate; cut, whether the tiles of a batch of
+// several requests are cut into shares; shares, how many, and aim, whether no more of
+// them where the grid has room for more tiles; share_least, 32-token groups of one, at
+// least.
 template <typename Costs>
 Estimate estimate(bool prefill, int gangs, int rows, double tiles, double groups, double longest, double tokens_heads, bool ragged,
                   double shared, int most_rows, int D, int hk, int cus) {
@@ -629,6 +671,7 @@ PagedPlan plan_paged_attention(const PagedShape& a, int cus) {
   };
   // (the sums of tiles times groups fit, whatever the offsets say)
   if (p.kernel == 0 && p.gangs == 1 && !p.merge && a.requests > 1 && a.requests < kShareRequests &&
+      Costs::cut((double)(useful(p.rows) * hk), longest, D, cus) &&
       (double)p.tiles * (double)a.requests * (double)(a.width * a.block_size / RF_KV8_GROUP + 1) < 2147483647.0) {
     // Shares that are long enough for the join they cost (what was measured stands
     // at each Costs).
