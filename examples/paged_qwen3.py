@@ -1,6 +1,6 @@
-"""Greedy generation with a W8A16 Qwen3 checkpoint over the int8 paged cache.
+"""Greedy generation with a W8A16 Qwen3 checkpoint over the int8 or the 4-bit paged cache.
 
-    python examples/paged_qwen3.py CHECKPOINT --prompts "9707,11,1879" "785,3974" --new 64
+    python examples/paged_qwen3.py CHECKPOINT --prompts "9707,11,1879" "785,3974" --new 64 --bits 4
 
 ``CHECKPOINT`` is a W8A16 directory as ``python -m rhinoforge_amd.quant.convert``
 writes it; prompts are token ids.  All prompts run as one ragged batch: one pass
@@ -20,15 +20,19 @@ from rhinoforge_amd.quant.load import load_w8a16_model
 
 
 class PagedQwen3:
-    """A loaded model's layers around one :class:`rf.KV8Cache` each."""
+    """A loaded model's layers around one :class:`rf.KV8Cache` each, or one
+    :class:`rf.KV4Cache` (``bits``: of a cached value)."""
 
-    def __init__(self, model, num_blocks: int, block_size: int = 64) -> None:
+    def __init__(self, model, num_blocks: int, block_size: int = 64, bits: int = 8) -> None:
+        if bits not in (4, 8):
+            raise ValueError(f"bits must be 4 or 8, got {bits}")
+        kind = rf.KV4Cache if bits == 4 else rf.KV8Cache
         cfg = model.config
         self.model, self.block_size = model, block_size
         self.heads, self.kv_heads = cfg.num_attention_heads, cfg.num_key_value_heads
         self.head_dim, self.eps = cfg.head_dim, cfg.rms_norm_eps
         self.device = model.model.norm.weight.device
-        self.caches = [rf.KV8Cache(num_blocks, self.kv_heads, self.head_dim, block_size, device=self.device)
+        self.caches = [kind(num_blocks, self.kv_heads, self.head_dim, block_size, device=self.device)
                        for _ in model.model.layers]
         rope = model.model.rotary_emb
         if getattr(rope, "rope_type", "default") == "longrope":
@@ -56,8 +60,8 @@ class PagedQwen3:
             q, k = rf.qk_norm_rope(q, k, at.q_norm.weight, at.k_norm.weight, self.cos, self.sin,
                                    plan.positions, eps=self.eps)
             cache.append(k, v, plan.slots)
-            o = rf.kv8_attention(q, cache, table, plan.kv_lens, cu, max_q_len=max_new, max_kv_len=max_kv,
-                                 window=at.sliding_window or 0, scale=at.scaling)
+            o = cache.attention(q, table, plan.kv_lens, cu, max_q_len=max_new, max_kv_len=max_kv,
+                                window=at.sliding_window or 0, scale=at.scaling)
             h = h + at.o_proj(o.flatten(1))
             h = h + layer.mlp(layer.post_attention_layernorm(h))
         last = h if max_new == 1 else h[plan.cu_new[1:].long() - 1]
@@ -120,8 +124,9 @@ def main() -> None:
     ap.add_argument("--prompts", nargs="+", default=["1,2,3"], help="token ids, separated by commas")
     ap.add_argument("--new", type=int, default=32, help="tokens to generate for each prompt")
     ap.add_argument("--blocks", type=int, default=1024, help="blocks of each layer's cache")
+    ap.add_argument("--bits", type=int, default=8, choices=(4, 8), help="of a cached key or value")
     args = ap.parse_args()
-    paged = PagedQwen3(load_w8a16_model(None, args.checkpoint), args.blocks)
+    paged = PagedQwen3(load_w8a16_model(None, args.checkpoint), args.blocks, bits=args.bits)
     prompts = [[int(t) for t in p.split(",")] for p in args.prompts]
     paged.generate(prompts, min(args.new, 4))
     torch.cuda.synchronize()
