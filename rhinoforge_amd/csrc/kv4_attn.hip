@@ -875,6 +875,7 @@ struct Kv4Costs {
     constexpr double kOneLaunch = 8.5, kTwoLaunches = 11.5;
     const bool whole = requests > 1 && !cut(tiles * hk, longest, D, cus);
     Estimate best{1e30, 1, false};
+    double least = 1e30;
     for (int gangs = 1; gangs <= (rows <= 8 && requests == 1 ? 2 : 1); ++gangs) {
       const double compute = rows <= 8 ? 1.0 : rows == 16 ? 1.15 : 1.65;
       const double turn = compute * (D == 64 ? (gangs == 1 ? 0.43 : 0.63) : D == 128 ? (gangs == 1 ? 0.61 : 0.94)
@@ -890,6 +891,11 @@ struct Kv4Costs {
         };
         const double room = (double)cus * slots, full = floor(w / room), rest = w - full * room;
         double us = 4.2 + 0.5 * gangs + full * round(room) + (rest >= 1 ? round(rest) : 0.0) + 1.5 * (ceil(w / room) - 1.0);
+        // (prompts: the kernel for many rows has its say; 13, 19 and 49 shapes of heads of 256,
+        // 64 and 128 within 0.76 to 1.17 of it)
+        const double tile = D == 64 ? 1.2 + 0.73 * turns : D == 128 ? 2.3 + 0.9 * turns : 2.9 + 1.05 * turns;
+        const double many = (D == 64 ? 6.1 : D == 128 ? 7.9 : 7.1) + w / cus * tile;
+        if (most_rows > 16 && w > cus && us < many) us = many;
         bool merge = false;
         if (s > 1) {
           const double join = 2.2 + 0.08 * s + held * D / 512.0 * (0.7 + 0.037 * s);
@@ -898,8 +904,8 @@ struct Kv4Costs {
           merge = (second < join && us + join > kTwoLaunches) || tiles * hk > kMaxSplitCounters;
           us += merge ? second : join;
         }
-        const double host = merge ? kTwoLaunches : kOneLaunch, cost = (us > host ? us : host) + 0.1 * us;
-        if (cost < best.us) best = {cost, s, merge, gangs};
+        const double host = merge ? kTwoLaunches : kOneLaunch, call = us > host ? us : host;
+        if (call + 0.1 * us < least) least = call + 0.1 * us, best = {call, s, merge, gangs};
       }
     }
     return best;
