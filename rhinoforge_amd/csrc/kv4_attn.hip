@@ -189,7 +189,7 @@ __device__ __forceinline__ void finish_tile(const AttnArgs& a, const Tile& t, in
     }
   }
   if (partial && !a.merge)
-    join<T, D, NW * kWave>(a, t, h, rows, splits, ((int)id - split * a.hk) * R, a.hk * R,
+    join<T, D, R, NW * kWave>(a, t, h, rows, splits, ((int)id - split * a.hk) * R, a.hk * R,
                a.counters + (id - (unsigned)(split * a.hk)), &red[0][0][0]);
 }
 
@@ -891,6 +891,9 @@ struct Kv4Costs {
         };
         const double room = (double)cus * slots, full = floor(w / room), rest = w - full * room;
         double us = 4.2 + 0.5 * gangs + full * round(room) + (rest >= 1 ? round(rest) : 0.0) + 1.5 * (ceil(w / room) - 1.0);
+        // (workgroups that start together hold each other up: 8000 tokens, 32 + 8 heads, 16 and
+        // 32 splits 11.1 and 12.2 us, 12 heads of 64 10.9 and 12.9)
+        if (rows <= 8) us += 2.2 * (w < 2 * cus ? w / cus : 2.0);
         // (prompts: the kernel for many rows has its say; 13, 19 and 49 shapes of heads of 256,
         // 64 and 128 within 0.76 to 1.17 of it)
         const double tile = D == 64 ? 1.2 + 0.73 * turns : D == 128 ? 2.3 + 0.9 * turns : 2.9 + 1.05 * turns;
@@ -898,7 +901,9 @@ struct Kv4Costs {
         if (most_rows > 16 && w > cus && us < many) us = many;
         bool merge = false;
         if (s > 1) {
-          const double join = 2.2 + 0.08 * s + held * D / 512.0 * (0.7 + 0.037 * s);
+          const double x = held * D / 512.0;
+          const double join = rows <= 8 ? 3.1 + 0.2 * x + (0.03 + 0.028 * x) * s * (gangs == 2 ? 0.42 : 1.0)
+                                        : 2.2 + 0.08 * s + x * (0.7 + 0.037 * s);
           const double second = 2.9 + 0.09 * s + tokens_heads * s * D * 8.0 / 3e6;
           // (a caller that does not replay graphs pays for the second launch)
           merge = (second < join && us + join > kTwoLaunches) || tiles * hk > kMaxSplitCounters;

@@ -369,7 +369,7 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_decode_kernel(AttnArgs a) {
     }
   }
   if (partial && !a.merge)
-    join<T, D>(a, t, h, rows, share.splits, ((int)id - split * a.hk) * R, a.hk * R,
+    join<T, D, R, kThreads>(a, t, h, rows, share.splits, ((int)id - split * a.hk) * R, a.hk * R,
                a.counters + (id - (unsigned)(split * a.hk)), &red[0][0][0]);
 }
 

@@ -364,7 +364,6 @@ __device__ __forceinline__ float log2_fast(float x) { return __builtin_amdgcn_lo
 // ---------------------------------------------------------------------------
 constexpr int kThreads = 256;
 constexpr int kWaves = 4;
-constexpr int kMaxRows = 32;  // of a tile whose splits are joined
 constexpr int kDeviceScope = 16;  // sc1 of a buffer access
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -417,9 +416,9 @@ __device__ __forceinline__ void no_share(const PagedArgs& a, const Tile& t, int 
 }
 
 // All threads call it after their stores of partial results.  buf: LDS of
-// rows * splits * 8 + 16 kT bytes, free for use; kT threads.  Row rc of split s is at
+// rows * splits * 8 + 16 kT bytes, free for use; kT threads, up to kRows rows.  Row rc of split s is at
 // first + s * stride + rc of the partial results.
-template <typename T, int D, int kT = kThreads>
+template <typename T, int D, int kRows, int kT>
 __device__ __forceinline__ void join(const PagedArgs& a, const Tile& t, int h, int rows, int splits,
                                      int first, int stride, uint32_t* counter, float* buf) {
   const int tid = threadIdx.x;
@@ -444,29 +443,29 @@ __device__ __forceinline__ void join(const PagedArgs& a, const Tile& t, int h, i
   while (units * ways * 2 <= kT && ways * 2 <= splits) ways *= 2;
   float* stat = buf;  // [rows][splits][2^(m - the row's), l]
   floatx4* sums = reinterpret_cast<floatx4*>(buf + (rows * splits * 2 + 3) / 4 * 4);
-  __shared__ float tops[kMaxRows];
-  constexpr int kEach = kMaxRows / (kT / kWave);
+  __shared__ float tops[kRows];
+  constexpr int kEach = (kRows + kT / kWave - 1) / (kT / kWave);
   // A wavefront takes some of the rows, a lane one of its splits (at most 64).
   const int lane = tid % kWave, wave = tid / kWave;
   floatx2 own[kEach];
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    own[i] = floatx2{-__builtin_inff(), 0.0f};
-    const int rc = wave + i * (kT / kWave);
-    if (rc < rows && lane < splits) own[i] = parts.load_stat(first + lane * stride + rc);
-  }
+  for (int i = 0; i < kEach; ++i)  // (no branches, which would wait for each load)
+    own[i] = parts.load_stat(first + min(lane, splits - 1) * stride + min(wave + i * (kT / kWave), rows - 1));
   const auto factors = [&] {
+    float top[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) top[i] = own[i][0];  // (lanes from `splits` on: the last one's)
+    for (int n = 1; n < splits; n *= 2)
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) top[i] = fmaxf(top[i], __shfl_xor(top[i], n));
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       const int rc = wave + i * (kT / kWave);
       if (rc >= rows) break;
-      float m = own[i][0];
-#pragma unroll
-      for (int n = 1; n < kWave; n *= 2) m = fmaxf(m, __shfl_xor(m, n));
-      if (lane == 0) tops[rc] = m;
+      if (lane == 0) tops[rc] = top[i];
       if (lane < splits)
         *reinterpret_cast<floatx2*>(stat + 2 * (rc * splits + lane)) =
-            floatx2{exp2_fast(own[i][0] - safe(m)), own[i][1]};
+            floatx2{exp2_fast(own[i][0] - safe(top[i])), own[i][1]};
     }
   };
   for (int u0 = 0; u0 < units; u0 += kT) {
