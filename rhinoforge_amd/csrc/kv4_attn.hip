@@ -49,9 +49,16 @@ __device__ __forceinline__ half2v less(uint32_t v, uint32_t z) { return as_half2
 
 // ---------------------------------------------------------------------------
 // Few rows (single tokens, a few drafted ones): RT tiles of 16 rows, held by
-// all four wavefronts; the wavefronts take 32-token groups in turn and read the
-// cache straight into MFMA operands (no LDS), one turn ahead of the products.  At
-// the end the wavefronts' sums meet in LDS.
+// all four or eight wavefronts; the wavefronts take 32-token groups in turn and read
+// the cache straight into MFMA operands (no LDS), one turn ahead of the products.
+// At the end the wavefronts' sums meet in LDS.
+//
+// Long contexts are bound by the cache's bytes, and by what comes before and after
+// them: 130999 tokens, 32 + 8 heads of 128 (138 MB), take 29.7 us, a plain read of as
+// much 23.4; 48 requests of up to 9000, 64 + 8 heads (237 MB), 51.1 and 36.6.  Short
+// ones by round trips: 777 tokens take 8.5 us, of which it is 1.3 until the request
+// is found, 1.2 for ids and queries, 1 a turn, 1 in LDS and, split, 4 to store, count and
+// join.
 //
 // A product has 16 columns, and a single token of a model with four query heads to
 // a key head fills four of them.  W = 2, 4: tiles of 16 / W rows, each of which has
@@ -459,7 +466,10 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 && RT == 1 ? 3 : 2))) void kv4_decod
 // MFMA), and those of the next two steps are loaded meanwhile.  G = 2: two gangs
 // of four wavefronts take the steps of the same rows in turn, and their sums join
 // at the end: what the longest tile takes is halved, which is what a prompt takes
-// that does not fill the chip several times.
+// that does not fill the chip several times (1000 tokens, 32 + 8 heads of 128: 33.3 us,
+// two gangs 26.8; 7999 tokens, 64 + 8 heads: 1145, and 916 TFLOP/s with one).  Bound by
+// the vector instructions beside the products, at the power's clock: matrix units 44%
+// busy, vector units 67% (over int8 45% and 63%).
 // ---------------------------------------------------------------------------
 template <typename T, int D, int G>
 __global__ __launch_bounds__(G* kWaves* kWave)
@@ -902,7 +912,7 @@ struct Kv4Costs {
         bool merge = false;
         if (s > 1) {
           const double x = held * D / 512.0;
-          const double join = rows <= 8 ? 3.1 + 0.2 * x + (0.03 + 0.028 * x) * s * (gangs == 2 ? 0.42 : 1.0)
+          const double join = rows <= 8 ? (gangs == 1 && D <= 128 ? 2.0 : 3.1) + 0.2 * x + (0.03 + 0.028 * x) * s * (gangs == 2 ? 0.42 : 1.0)
                                         : 2.2 + 0.08 * s + x * (0.7 + 0.037 * s);
           const double second = 2.9 + 0.09 * s + tokens_heads * s * D * 8.0 / 3e6;
           // (a caller that does not replay graphs pays for the second launch)
@@ -929,11 +939,9 @@ struct Kv4Costs {
     return (int64_t)(room > most ? room : most) * cus;
   }
   // (4 requests of up to 2000 tokens, 32 + 8 heads, 8, 12, 16 and 24 groups: 10.0, 10.4, 10.9,
-  // 12.0 us; 16 of those 12.4, 12.2, 13.0, 12.3; of up to 500 tokens 9.5, 10.2, 8.1, 8.1; 8 + 1
-  // heads of 256, 16 of up to 2000: 13.2, 14.2, 15.1, 16.9; of up to 500: 12.8, 13.6, 10.5, 10.5)
-  static int share_least(int rows, int D, double longest) {
-    return longest < 32 || rows == 32 ? 16 : D == 256 ? 8 : 12;
-  }
+  // 12.0 us; 16 of those 12.4, 12.2, 13.0, 12.3; 8 + 1 heads of 256, 16 of up to 2000: 13.2,
+  // 14.2, 15.1, 16.9)
+  static int share_least(int rows, int D, double) { return rows == 32 ? 16 : D == 256 ? 8 : 12; }
 };
 
 }  // namespace

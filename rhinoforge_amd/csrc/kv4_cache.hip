@@ -13,7 +13,7 @@ constexpr int kThreads = 256;
 // each; the LP lanes after them hold the other side's row.  A workgroup takes 256 /
 // (2 LP) tokens of one head.  A prompt runs in one or two rounds of workgroups, which
 // load, compute and store one after the other, so what counts beside the bytes are
-// the vector instructions: 6874 tokens of 8 heads of 128 take 10.5 us (35.6 MB, 3.4
+// the vector instructions: 6874 tokens of 8 heads of 128 take 10.6 us (35.6 MB, 3.4
 // TB/s), with eight dimensions a lane and the numbers put together by shifts and ORs
 // 13.8.  Workgroups that take several tokens a lane gain nothing (2000 tokens: 5.0
 // us, in half as many workgroups 5.0; 1000: 3.1 and 3.8).
@@ -149,7 +149,7 @@ __global__ __launch_bounds__(kThreads) void kv4_append_kernel(AppendArgs a) {
 // bytes of one, which are sixteen dimensions of two of its keys, or four dimensions
 // of all eight values, and writes those that the list asks for.  A list of runs,
 // wherever they begin, moves few bytes twice that way (9001 tokens, 8 heads of 128:
-// 10.6 us, 4.4 TB/s; token by token 19.8).  Where the entries are mostly single
+// 10.9 us, 4.3 TB/s; token by token 19.8).  Where the entries are mostly single
 // tokens, a thread takes eight dimensions of one.
 // ---------------------------------------------------------------------------
 struct ReadArgs {
