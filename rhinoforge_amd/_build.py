@@ -17,6 +17,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -66,11 +67,13 @@ def _atomic_link(tmp: Path, dst: Path) -> None:
 def build_capi(verbose: bool = False) -> Path:
     """Compile the HIP kernels and the C ABI into lib/librf_w8a16.so."""
     LIBDIR.mkdir(exist_ok=True)
-    objs = []
-    for src in CAPI_SOURCES:
-        obj = LIBDIR / (Path(src).stem + ".o")
-        _run([HIPCC, *HIP_FLAGS, "-I", str(INCLUDE), "-c", str(CSRC / src), "-o", str(obj)], verbose)
-        objs.append(str(obj))
+    objs = [str(LIBDIR / (Path(src).stem + ".o")) for src in CAPI_SOURCES]
+    # (four at a time: the attention kernels of one cache take as long as all the rest)
+    with ThreadPoolExecutor(4) as pool:
+        steps = [pool.submit(_run, [HIPCC, *HIP_FLAGS, "-I", str(INCLUDE), "-c", str(CSRC / src), "-o", obj], verbose)
+                 for src, obj in zip(reversed(CAPI_SOURCES), reversed(objs))]
+        for step in steps:
+            step.result()
     tmp = CAPI_LIB.with_name(CAPI_LIB.name + f".tmp{os.getpid()}")
     _run([HIPCC, f"--offload-arch={OFFLOAD_ARCH}", "-shared", "-fPIC", *objs,
           "-Wl,-soname,librf_w8a16.so", "-o", str(tmp)], verbose)

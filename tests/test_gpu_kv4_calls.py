@@ -45,6 +45,20 @@ def test_batches_of_many_requests(b, hq):
     assert (out[-9:] == 0).all() and torch.isneginf(lse2[-9:]).all()
 
 
+@pytest.mark.parametrize("b,most", [(3, 300), (63, 60), (100, 120), (511, 40), (530, 40)])
+@pytest.mark.parametrize("d,hk", [(64, 2), (128, 1), (256, 1)])
+def test_prompts_of_many_requests(b, most, d, hk):
+    """Prompts of unequal lengths, some without tokens, some behind cached ones."""
+    _say("prompts", b, most, d)
+    g = _rng(b + d)
+    news = torch.randint(0, most, (b,), generator=g).tolist()
+    lens = [n + int(c) for n, c in zip(news, torch.randint(0, 50, (b,), generator=g))]
+    nb = sum(-(-n // 64) for n in lens) + 1
+    k, v = _filled(nb, hk, 64, d, 50), _filled(nb, hk, 64, d, 51)
+    q = torch.randn(sum(news), 8, d, generator=g).half()
+    _check(q, k, v, _table(lens, 64, nb, g), lens, news, max_q_len=max(news), max_kv_len=max(lens))
+
+
 @pytest.mark.parametrize("heads", [(8, 2, 64), (8, 2, 128), (4, 1, 256), (64, 16, 128)])
 @pytest.mark.parametrize("n", [1, 2, 4, 8, 40])
 @pytest.mark.parametrize("context", [100, 2500, 17000])
