@@ -895,7 +895,10 @@ struct Kv4Costs {
         if (s > cap || (s > 1 && (s > groups || whole))) break;
         const double turns = ceil(ceil(groups / s) / (kWaves * gangs)), w = tiles * hk * s;
         const auto round = [&](double n) {  // n workgroups at a time
-          const double bytes = n * kWaves * gangs * 32.0 * token_bytes(D) * shared / (gangs == 1 ? 6.5e6 : 7.0e6);
+          // (the CUs share the memory evenly, so those with a workgroup more are the last: 131000
+          // tokens, 12 heads of 64, 24 splits of eight wavefronts 34 us, 64 of four 28)
+          const double as_if = rows <= 8 && n > cus ? ceil(n / cus) * cus : n;
+          const double bytes = as_if * kWaves * gangs * 32.0 * token_bytes(D) * shared / (gangs == 1 ? 6.5e6 : 7.0e6);
           const double beside = turn * (1.0 + 0.3 * (n > cus ? n / cus - 1.0 : 0.0));
           return turns * (beside > bytes ? beside : bytes);
         };
