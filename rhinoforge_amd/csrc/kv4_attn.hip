@@ -38,11 +38,23 @@ struct AttnArgs : PagedArgs {
   const uint16_t* rows;
 };
 
-// Nothing seen yet.  (Finite: differences from scores of -inf are not NaN.)
+// Nothing seen yet.  (Finite: differences from scores of -inf are not NaN.  Scores
+// before their factor are sums of at most 256 products of two fp16 numbers, below 2^41.)
 constexpr float kNothing = -1e30f;
+constexpr float kLeastStep = -24.0f;  // log2 of less than any value step
 // Score factors stay finite and above 0: a masked score is -inf whatever it is
 // multiplied by, and scores beyond these ranges are 0 or infinite to exp2.
 __device__ __forceinline__ float in_range(float factor) { return fminf(fmaxf(factor, 0x1p-126f), 0x1p127f); }
+
+// A row's reference as partial results hold it, in log2 units, -inf where nothing was
+// seen (l = 0), and by how much the rounding moved it, as a factor of the sums.  (At
+// most 2: past 2^24 scores are no more exact than that.  Scores past fp32's range are
+// as its largest number.)
+__device__ __forceinline__ float reference(float m, float factor, float l, float* to) {
+  const float at = __builtin_amdgcn_fmed3f(m * factor, -0x1.fffffep127f, 0x1.fffffep127f);
+  *to = l == 0.0f ? -__builtin_inff() : at;
+  return exp2_fast(__builtin_amdgcn_fmed3f(__builtin_fmaf(m, factor, -at), -1.0f, 1.0f));
+}
 
 // (n - z) of a token pair's numbers: base - (base + z), exact in fp16.
 __device__ __forceinline__ half2v less(uint32_t v, uint32_t z) { return as_half2(v) - as_half2(z); }
@@ -121,6 +133,29 @@ __device__ __forceinline__ uint32_t from_above(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x100 + N, 0xf, 0xf, true);
 }
 
+// op over the lanes that differ by multiples of C (4, 8 or 16), in all of them: turns of
+// a row of 16, then exchanges between rows.  (Through LDS, as __shfl_xor goes, each step
+// is a round trip, up to eight before the first weights: 2000 tokens, 12 heads of 64, 9.1
+// us, so 8.9.)
+template <int C, typename Op>
+__device__ __forceinline__ float over_columns(float v, Op op) {
+  const auto turned = [&](auto ctrl) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl(), 0xf, 0xf, true));
+  };
+  if constexpr (C <= 4) v = op(v, turned([] { return 0x124; }));  // row_ror:4
+  if constexpr (C <= 8) v = op(v, turned([] { return 0x128; }));  // row_ror:8
+  const auto pair = [&](auto both) {
+    const uint32_t x = both[0], y = both[1];
+    return op(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y));
+  };
+  uint32_t u = __builtin_bit_cast(uint32_t, v);
+  v = pair(__builtin_amdgcn_permlane16_swap(u, u, false, false));
+  u = __builtin_bit_cast(uint32_t, v);
+  return pair(__builtin_amdgcn_permlane32_swap(u, u, false, false));
+}
+__device__ __forceinline__ float add(float u, float v) { return u + v; }
+__device__ __forceinline__ float larger(float u, float v) { return fmaxf(u, v); }
+
 // Eight numbers less 8, in the order of their dimensions.
 __device__ __forceinline__ half8 centred8(uint32_t d) {
   constexpr uint32_t k8 = 0x64086408u, k84 = 0x54805480u;  // 1024 + 8, 64 + 8
@@ -134,7 +169,8 @@ __device__ __forceinline__ half8 centred8(uint32_t d) {
 // would take registers there.)
 template <typename T, int D, int RT, int W, int NW>
 __device__ __forceinline__ void finish_tile(const AttnArgs& a, const Tile& t, int h, int rows, int split, int splits,
-                                            bool partial, unsigned id, const float (&m)[RT], float (&l)[RT],
+                                            bool partial, unsigned id, const float (&m)[RT], const float (&d)[RT],
+                                            const float (&factor)[RT], float (&l)[RT],
                                             const floatx4 (&acc)[RT][D / 16], float (&red)[NW][16 / W][D + 4],
                                             float (&red_m)[NW][16 / W * RT], float (&red_l)[NW][16 / W * RT]) {
   constexpr int C = 16 / W, R = C * RT, A = D / 64;
@@ -142,12 +178,15 @@ __device__ __forceinline__ void finish_tile(const AttnArgs& a, const Tile& t, in
   asm volatile("" : "+v"(tid));
   const int lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int lg = lane / 16, col = lane % C, part = lane % 16 / C;
+  float top_w[RT], unit[RT];
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
 #pragma unroll
     for (int n = C; n < kWave; n *= 2) l[r] += __shfl_xor(l[r], n);
+    unit[r] = reference(m[r], factor[r], l[r], &top_w[r]) * exp2_fast(d[r]);
+    l[r] *= unit[r];
     if (lane < C) {
-      red_m[wave][C * r + col] = m[r];
+      red_m[wave][C * r + col] = top_w[r];
       red_l[wave][C * r + col] = l[r];
     }
   }
@@ -158,7 +197,7 @@ __device__ __forceinline__ void finish_tile(const AttnArgs& a, const Tile& t, in
     float top = red_m[0][rr];
 #pragma unroll
     for (int w = 1; w < NW; ++w) top = fmaxf(top, red_m[w][rr]);
-    const float f = exp2_fast(m[r] - top);
+    const float f = exp2_fast(top_w[r] - safe(top)) * unit[r];
     if (part == 0) {
 #pragma unroll
       for (int i = 0; i < A; ++i)
@@ -181,7 +220,7 @@ __device__ __forceinline__ void finish_tile(const AttnArgs& a, const Tile& t, in
       floatx4 o = 0.0f;
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
-        ll += red_l[w][rc] * exp2_fast(red_m[w][rc] - mm);
+        ll += red_l[w][rc] * exp2_fast(red_m[w][rc] - safe(mm));
         o += *reinterpret_cast<const floatx4*>(&red[w][c][d]);
       }
       const int64_t to = out_row(a, t, h, rc);
@@ -279,8 +318,7 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 && RT == 1 ? 3 : 2))) void kv4_decod
       float m = 0.0f;
 #pragma unroll
       for (int i = 0; i < 2 * A; ++i) m = load_amax<T>(raw[r][i], m);
-      m = fmaxf(m, __shfl_xor(m, 16));
-      m = fmaxf(m, __shfl_xor(m, 32));
+      m = over_columns<16>(m, larger);
       const int e = row_exponent(m), e1 = e / 2, e2 = e - e1;
       const float f1 = pow2(-e1), f2 = pow2(-e2);
 #pragma unroll
@@ -297,16 +335,20 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 && RT == 1 ? 3 : 2))) void kv4_decod
     for (int i = 0; i < 2 * A; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j) sum += (float)q[r][i][j];
-    sum += __shfl_xor(sum, 16);
-    sum += __shfl_xor(sum, 32);
-    qsum[r] = -sum;
+    qsum[r] = -over_columns<16>(sum, add);
     pos[r] = t.kv_len - t.queries + (int)((unsigned)(t.row0 + min(C * r + col, rows - 1)) / (unsigned)a.group);
   }
   floatx4 acc[RT][4 * A];
-  float m[RT], l[RT];  // l: each lane's own share of the sum
+  // Weights are relative to 2^(m factor + d): m is the row's largest score, before its
+  // factor, when it was last raised, d what the largest of the scores with log2 of their
+  // value steps had above that (-24 to 13).  Scores count by their difference from m,
+  // which is right for any size of them; m factor, rounded, would be off by more than a
+  // weight's range from 2^28 on.
+  float m[RT], d[RT], l[RT];  // l: each lane's own share of the sum
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     m[r] = kNothing;
+    d[r] = kLeastStep;
     l[r] = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4 * A; ++i) acc[r][i] = floatx4{0, 0, 0, 0};
@@ -364,12 +406,12 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 && RT == 1 ? 3 : 2))) void kv4_decod
     float sum[RT];
     bool raise = false;
     const auto weights = [&](int r) {  // the largest of them
-      const float off = kShift - m[r];
+      const float off = kShift - d[r];
       float most = 0.0f;
       sum[r] = 0.0f;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const float e = exp2_fast(__builtin_fmaf(s[r][i], factor[r], off));
+        const float e = exp2_fast(__builtin_fmaf(minus(s[r][i], m[r]), factor[r], off));
         const float w = __builtin_fmaf((float)vs[i / 2][i % 2], e, 0.0f);
         sum[r] += e;
         most = fmaxf(most, w);
@@ -388,12 +430,18 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 && RT == 1 ? 3 : 2))) void kv4_decod
       for (int r = 0; r < RT; ++r) {
         float top = m[r];
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-          top = fmaxf(top, s[r][i] * factor[r] + log2_fast(fmaxf((float)vs[i / 2][i % 2], 0x1p-24f)));
+        for (int i = 0; i < N; ++i) top = fmaxf(top, s[r][i]);
+        top = over_columns<C>(top, larger);
+        const float fall = (m[r] - top) * factor[r];
+        float above = d[r] + fall;
 #pragma unroll
-        for (int n = C; n < kWave; n *= 2) top = fmaxf(top, __shfl_xor(top, n));
-        const float f = exp2_fast(m[r] - top);
+        for (int i = 0; i < N; ++i)
+          above = fmaxf(above, __builtin_fmaf(minus(s[r][i], top), factor[r],
+                                              log2_fast(fmaxf((float)vs[i / 2][i % 2], 0x1p-24f))));
+        above = over_columns<C>(above, larger);
+        const float f = exp2_fast(fall + (d[r] - above));
         m[r] = top;
+        d[r] = above;
         l[r] *= f;
 #pragma unroll
         for (int i = 0; i < 4 * A; ++i) acc[r][i] *= f;
@@ -455,8 +503,9 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 && RT == 1 ? 3 : 2))) void kv4_decod
     while (turn(0) && turn(1)) {}
   }
 
-  // ---- the four wavefronts' results
-  finish_tile<T, D, RT, W, NW>(a, t, h, rows, split, share.splits, partial, id, m, l, acc, red, red_m, red_l);
+  // ---- the wavefronts' results
+  finish_tile<T, D, RT, W, NW>(a, t, h, rows, split, share.splits, partial, id, m, d, factor, l, acc, red, red_m,
+                               red_l);
 }
 
 // ---------------------------------------------------------------------------

@@ -354,6 +354,13 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 
 __device__ __forceinline__ float log2_fast(float x) { return __builtin_amdgcn_logf(x); }
 
+// A difference of scores, both rounded.  (Taken together with the product that one of
+// them is, in one rounding, it would not be 0 for the largest score.)
+__device__ __forceinline__ float minus(float s, float m) {
+#pragma clang fp contract(off)
+  return s - m;
+}
+
 // ---------------------------------------------------------------------------
 // Splits of one tile.  Each workgroup stores its rows' sums and (m, l), waits
 // for its stores and counts itself; the last one adds all of them in split
