@@ -606,7 +606,7 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv4_prefill_kernel(AttnArgs a) {
   my_hi_min = min(uniform(my_hi_min), end * 32), my_hi_max = min(uniform(my_hi_max), end * 32);
 
   floatx16 acc[D / 32];
-  float m = kNothing, l = 0.0f;
+  float m = kNothing, l = 0.0f;  // weights are relative to 2^(m factor)
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) acc[i] = 0.0f;
 
@@ -728,9 +728,8 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv4_prefill_kernel(AttnArgs a) {
     for (int n = 0; n < NG; ++n)
 #pragma unroll
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[n][i]);
-    mx *= factor;
-    if (__ballot(mx > m + kRaise)) {
-      const float top = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32))), f = exp2_fast(m - top);
+    if (__ballot(minus(mx, m) * factor > kRaise)) {
+      const float top = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32))), f = exp2_fast((m - top) * factor);
       m = top;
       l *= f;
 #pragma unroll
@@ -740,8 +739,19 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv4_prefill_kernel(AttnArgs a) {
     // would keep the sums twice, and spill)
     float off = 0.0f;
     if (opaque(t0) >= 0) {  // (always: a block of its own)
-      off = kShift - m;
+      off = __builtin_fmaf(-m, factor, kShift);
       asm volatile("" : "+v"(off));
+    }
+    // Scores of ordinary size take one instruction for their difference from m.  Of
+    // large ones both terms are rounded, from 2^22 on to more than the fp16 weights have
+    // room for: first the difference, then the factor.
+    if (__ballot(fabsf(off) > kFar)) {
+      keep_branch();
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[n][i] = minus(s[n][i], m);
+      off = kShift;
     }
     half8 p[2];
     const auto weights = [&](int n) {
@@ -815,7 +825,8 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv4_prefill_kernel(AttnArgs a) {
     }
     __syncthreads();
     if (gang == 0) {
-      const float om = stats[0], top = fmaxf(m, om), f = exp2_fast(m - top), of = exp2_fast(om - top);
+      const float om = stats[0], top = fmaxf(m, om);
+      const float f = exp2_fast((m - top) * factor), of = exp2_fast((om - top) * factor);
 #pragma unroll
       for (int i = 0; i < D / 2; ++i) acc[i / 16][i % 16] = acc[i / 16][i % 16] * f + sums[i * kWave] * of;
       m = top;
@@ -832,7 +843,8 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv4_prefill_kernel(AttnArgs a) {
   float* mine = reinterpret_cast<float*>(lds) + wave * 32 * kPitch;
   l += __shfl_xor(l, 32);
   const int left = rows - wrow;  // rows of this wavefront's tile
-  const float f = partial ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+  float top_w;
+  const float unit = reference(m, factor, l, &top_w), f = partial ? unit : l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
   for (int i = 0; i < D / 32; i += 2) {
 #pragma unroll
@@ -863,9 +875,9 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv4_prefill_kernel(AttnArgs a) {
   }
   if (lh == 0 && col < left) {
     const int64_t to = out_row(a, t, h, wrow + col);
-    if (partial) Partials(a).store_stat((int)to * a.splits + split, m, l);
+    if (partial) Partials(a).store_stat((int)to * a.splits + split, top_w, l * unit);
     else if (a.lse)
-      a.lse[to] = l == 0.0f ? -__builtin_inff() : (m - kShift + log2_fast(l)) * kLn2;
+      a.lse[to] = l == 0.0f ? -__builtin_inff() : __builtin_fmaf(m, factor, log2_fast(l) - kShift) * kLn2;
   }
 }
 

@@ -25,9 +25,12 @@ from test_gpu_kv4 import DEV, UNIT, _cache, _filled, _np, _rng, _say, _table
 
 pytestmark = pytest.mark.gpu
 
-# queries, heads, kv_heads, head_dim, cached tokens: tiles of 4, 8 and 16 rows
+# queries, heads, kv_heads, head_dim, cached tokens.  Few rows: tiles of 4, 8, 16 and 32.
 FEW = [(1, 4, 1, 128, 300), (1, 8, 2, 64, 300), (1, 8, 1, 256, 300), (2, 8, 2, 128, 300), (4, 4, 1, 64, 300),
-       (2, 14, 2, 128, 300), (1, 8, 2, 128, 4000)]
+       (2, 14, 2, 128, 300), (3, 8, 1, 256, 300), (5, 4, 1, 128, 300), (7, 8, 2, 64, 300), (1, 8, 2, 128, 4000)]
+# Prompts: one gang and two, and their splits.
+MANY = [(500, 64, 4, 64, 300), (600, 64, 8, 64, 300), (500, 64, 4, 128, 300), (900, 64, 8, 128, 300),
+        (300, 64, 4, 256, 300), (300, 16, 2, 128, 6000), (300, 32, 2, 256, 6000)]
 BS = 32
 
 
@@ -100,7 +103,9 @@ def _near(out, ref, mass, dt, extra=0.0):
 
 CASES = ([(s, dt, ("scale", r)) for r in (0, 24, 29, 45, 110) for s in FEW for dt in UNIT] +
          [(s, torch.bfloat16, ("queries", r)) for r in (29, 100) for s in FEW] +
-         [(s, dt, ("fp16", 0)) for s in FEW for dt in UNIT])
+         [(s, dt, ("fp16", 0)) for s in FEW + MANY for dt in UNIT] +
+         [(s, dt, ("scale", r)) for r in (0, 24, 29, 45, 110) for s in MANY for dt in UNIT] +
+         [(s, torch.bfloat16, ("queries", 60)) for s in MANY])
 
 
 @pytest.mark.parametrize("shape,dt,how", CASES, ids=str)
@@ -138,7 +143,8 @@ def test_the_best_token_takes_all(shape, dt, how):
         assert (np.abs(lse[clear] - x) <= ds[clear] + 2.0 ** -18 + 2.0 ** -22 * np.abs(x)).all()
 
 
-KEYS = ([(s, dt, r, a) for s in FEW for dt in UNIT for r in (0, 26, 30, 90) for a in ("alike", "apart")])
+KEYS = ([(s, dt, r, a) for s in FEW for dt in UNIT for r in (0, 26, 30, 90) for a in ("alike", "apart")] +
+        [(s, torch.bfloat16, r, "apart") for s in MANY for r in (0, 30, 90)])
 
 
 @pytest.mark.parametrize("shape,dt,reach,steps", KEYS, ids=str)
@@ -187,7 +193,7 @@ def test_tokens_of_one_key_over_many_workgroups(heads, reach, n):
     _near(out, want, mass, torch.float16, total * 2.0 ** -32 * np.abs(values).max())
 
 
-@pytest.mark.parametrize("shape", FEW, ids=str)
+@pytest.mark.parametrize("shape", FEW + MANY, ids=str)
 @pytest.mark.parametrize("reach", [0, 32, 100])
 def test_scores_far_below_zero(shape, reach):
     """Every score of a row is about -2^reach; a row that sees tokens is not empty."""
