@@ -188,7 +188,8 @@ int rf_kv8_read(const rf_kv8_cache* cache, const int32_t* slots, int64_t n, int3
  *         lse -inf.  A block id outside the cache gives NaN.
  *   out   contiguous, q's type; lse (may be NULL) fp32 [tokens][heads], natural log
  *   scale > 0 and finite
- *   Scores, sums and softmax statistics are fp32.  A token's weight times its
+ *   Scores, sums and softmax statistics are fp32 (a score past what fp32 holds, in
+ *   units of ln 2, counts as infinite).  A token's weight times its
  *   block's v_scale is rounded to fp16, relative to the largest such product that
  *   the row sees: to 2^-11 of itself, or 2^-32 of that largest one.
  *   tokens * heads < 2^31, (requests + 1) * kv_heads + tokens * heads / 16 < 2^31

@@ -65,14 +65,14 @@ __device__ __forceinline__ float ratio_log2(float log_vs, const Running& r) {
   return fmaxf(log_vs - r.d, -60.0f);
 }
 
-// A row's references after scores of at most x, and of at most xv with log2 vs;
-// by how much l and the sums of p vs v change.
+// A row's references once m is its largest score, and new scores with log2 vs lie at
+// most `above` over that; by how much l and the sums of p vs v change.  (d comes from
+// differences of scores: a score's sum with log2 vs would not hold it from 2^24 on.)
 struct Change {
   float l, o;
 };
-__device__ __forceinline__ Change raise_to(Running& r, float x, float xv) {
-  const float m = fmaxf(r.m, x), top = fmaxf(r.m + r.d, xv);
-  const float d = m == -__builtin_inff() ? 0.0f : top - m, fall = r.m - safe(m);
+__device__ __forceinline__ Change raise_to(Running& r, float m, float above) {
+  const float fall = r.m - safe(m), d = m == -__builtin_inff() ? 0.0f : fmaxf(r.d + fall, above);
   const Change c = {exp2_fast(fall), exp2_fast(fall + (r.d - d))};
   r.m = m;
   r.d = d;
@@ -243,7 +243,7 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_decode_kernel(AttnArgs a) {
       for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[r][tt][i]);
-      raise |= mx + fmaxf(log_vs - run[r].d, 0.0f) > run[r].m + (run[r].m == -__builtin_inff() ? 0.0f : kRaise);
+      raise |= (mx - run[r].m) + fmaxf(log_vs - run[r].d, 0.0f) > kRaise;  // (NaN: nothing seen yet)
     }
     if (__ballot(raise)) {
 #pragma unroll
@@ -255,7 +255,8 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_decode_kernel(AttnArgs a) {
           for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[r][tt][i]);
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const Change f = raise_to(run[r], mx, mx + log_vs);
+        const float m = fmaxf(run[r].m, mx);
+        const Change f = raise_to(run[r], m, (mx - safe(m)) + log_vs);
         run[r].l *= f.l;
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) acc[r][i] *= f.o;
@@ -274,13 +275,13 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_decode_kernel(AttnArgs a) {
     half8 p[RT];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-      const float off = kShift + lr[r] - safe(run[r].m);
+      const float off = kShift + lr[r], m = safe(run[r].m);
       float sum = 0.0f;
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float e = exp2_fast(s[r][tt][i] + off);
+          float e = exp2_fast(minus(s[r][tt][i], m) + off);
           sum += e;
           p[r][tt * 4 + i] = (_Float16)e;
         }
@@ -576,23 +577,25 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_prefill_kernel(AttnArgs a) {
           s[n][i] = (tok < first) | (tok >= past) ? -__builtin_inff() : s[n][i];
         }
     }
-    // the largest score, with log2 vs, and as much of that as is above d
-    float c[NG], mx = -__builtin_inff(), mv = mx, over = mx;
+    // the largest scores, and how far they, or with log2 vs what is above d, are over m
+    float c[NG], most[NG], over = -__builtin_inff();
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
       // (not 0, also where ks is 0 or the product underflows: masked scores are
       // -inf here already, and -inf * 0 is NaN; any score times 2^-126 is 0 to exp2)
       c[n] = fmaxf(as_float(ks[n]) * factor, 0x1p-126f);
-      float most = -__builtin_inff();
+      most[n] = -__builtin_inff();
 #pragma unroll
-      for (int i = 0; i < 16; ++i) most = fmaxf(most, s[n][i]);
-      most *= c[n];
-      mx = fmaxf(mx, most);
-      mv = fmaxf(mv, most + log_vs[n]);
-      over = fmaxf(over, most + fmaxf(log_vs[n] - run.d, 0.0f));
+      for (int i = 0; i < 16; ++i) most[n] = fmaxf(most[n], s[n][i]);
+      most[n] *= c[n];
+      over = fmaxf(over, minus(most[n], run.m) + fmaxf(log_vs[n] - run.d, 0.0f));
     }
-    if (__ballot(over > run.m + (run.m == -__builtin_inff() ? 0.0f : kRaise))) {
-      const Change f = raise_to(run, fmaxf(mx, __shfl_xor(mx, 32)), fmaxf(mv, __shfl_xor(mv, 32)));
+    if (__ballot(over > kRaise)) {
+      float mx = fmaxf(most[0], most[NG - 1]);
+      mx = fmaxf(run.m, fmaxf(mx, __shfl_xor(mx, 32)));
+      float above = fmaxf(minus(most[0], safe(mx)) + log_vs[0], minus(most[NG - 1], safe(mx)) + log_vs[NG - 1]);
+      above = fmaxf(above, __shfl_xor(above, 32));
+      const Change f = raise_to(run, mx, above);
       run.l *= f.l;
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) acc[i] *= f.o;
