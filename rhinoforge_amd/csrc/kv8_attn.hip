@@ -50,6 +50,12 @@ struct Running {
   float d = 0.0f;               // the sums of p vs v are in units of 2^(m + d)
 };
 
+// s c - m, both steps rounded: 0 where m is that product.
+__device__ __forceinline__ float product_minus(float s, float c, float m) {
+#pragma clang fp contract(off)
+  return s * c - m;
+}
+
 // log2 of a value scale; of 0, so low that 2^ it is 0 and differences stay finite.
 __device__ __forceinline__ float scale_log2(uint32_t vs) {
   float log = log2_fast(as_float(vs));
@@ -612,9 +618,23 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_prefill_kernel(AttnArgs a) {
         asm volatile("" : "+v"(lr[n]));
       }
     }
+    // Scores of ordinary size take one instruction for their product with c and the
+    // difference from m.  Of large ones m, rounded, would be off by more than the
+    // weights have room for: the products are rounded as m was.
+    float base = safe(run.m);
+    if (__ballot(fabsf(base) > kFar)) {
+      keep_branch();
+#pragma unroll
+      for (int n = 0; n < NG; ++n) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[n][i] = product_minus(s[n][i], c[n], base);
+        c[n] = 1.0f;
+      }
+      base = 0.0f;
+    }
     half8 p[2];
     const auto weights = [&](int n) {
-      const float off = kShift + lr[n] - safe(run.m);
+      const float off = kShift + lr[n] - base;
       float sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {

@@ -28,6 +28,9 @@ UNIT = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
 # queries, heads, kv_heads, head_dim, cached tokens.  Few rows: tiles of 16 and 32.
 FEW = [(1, 8, 2, 128, 300), (1, 12, 12, 64, 300), (2, 8, 1, 256, 300), (5, 8, 2, 128, 300), (7, 8, 2, 64, 300),
        (1, 32, 8, 128, 9000), (4, 64, 8, 128, 4000), (4, 8, 1, 256, 4000)]
+# Prompts: one gang and two, and their splits.
+MANY = [(500, 64, 4, 64, 300), (600, 64, 8, 64, 300), (500, 64, 4, 128, 300), (900, 64, 8, 128, 300),
+        (300, 64, 4, 256, 300), (200, 64, 4, 256, 1300)]
 BS = 32
 
 
@@ -82,7 +85,9 @@ def _near(out, ref, mass, dt, extra=0.0):
 
 CASES = ([(s, dt, ("scale", r)) for r in (0, 24, 29, 45, 110) for s in FEW for dt in UNIT] +
          [(s, torch.bfloat16, ("queries", r)) for r in (29, 100) for s in FEW] +
-         [(s, dt, ("fp16", 0)) for s in FEW for dt in UNIT])
+         [(s, dt, ("fp16", 0)) for s in FEW + MANY for dt in UNIT] +
+         [(s, dt, ("scale", r)) for r in (0, 24, 29, 45, 110) for s in MANY for dt in UNIT] +
+         [(s, torch.bfloat16, ("queries", 60)) for s in MANY])
 
 
 @pytest.mark.parametrize("shape,dt,how", CASES, ids=str)
@@ -112,7 +117,7 @@ def test_one_token_takes_all(shape, dt, how, window):
         assert (np.abs(lse[clear] - x) <= ds[clear] + 2.0 ** -18 + 2.0 ** -22 * np.abs(x)).all()
 
 
-@pytest.mark.parametrize("shape", FEW, ids=str)
+@pytest.mark.parametrize("shape", FEW + MANY, ids=str)
 @pytest.mark.parametrize("reach", [0, 20, 26, 30, 90])
 @pytest.mark.parametrize("steps", ["alike", "apart"])
 def test_tokens_of_one_key_count_alike(shape, reach, steps):
