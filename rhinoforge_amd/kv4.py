@@ -86,7 +86,7 @@ class KV4Cache:
                                  f"{step.dtype} {list(step.shape)} and {zero.dtype} {list(zero.shape)}")
         words = [(s.contiguous().view(torch.int16), z) for s, z in ((k_step, k_zero), (v_step, v_zero))]
         nan = torch.isnan(k_step)
-        wrong = torch.stack([((w & 15) != 0).logical_and(~nan).any() for w, _ in words] +
+        wrong = torch.stack([((words[0][0] & 15) != 0).logical_and(~nan).any(), ((words[1][0] & 15) != 0).any()] +
                             [~((k_step >= 2.0 ** -20) & (k_step <= MAX_STEP) | nan).all(),
                              ~((v_step >= 2.0 ** -20) & (v_step <= MAX_STEP)).all()] +
                             [(x > 15).any() for x in (k, v, k_zero, v_zero)]).any()
