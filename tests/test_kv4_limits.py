@@ -42,3 +42,23 @@ def test_nan_keys_with_any_payload_are_the_mark():
     q = rf.KV4Cache.from_quantized(**p).to_quantized()
     assert torch.isnan(q[1][0, 0, 7]) and torch.isnan(q[1]).sum() == 1
     assert all(torch.equal(a, b) for a, b in zip(q[3:], (p["v"], p["v_step"], p["v_zero"])))
+
+
+def test_half_a_step_is_within_its_bound():
+    """At most 1/30 of the span and 2^-6 of that more; steps below 2^-14: 2^-21 more."""
+    r = np.random.default_rng(0)
+    worst = dict(large=0.0, small=0.0)
+    for e in np.concatenate((r.uniform(-30, 16, 4000), np.arange(-30, 17))):
+        x = np.sort(r.standard_normal(16)) * 2.0 ** e
+        x = x.astype(np.float32).astype(np.float64)
+        low, high = min(x[0], 0.0), max(x[-1], 0.0)
+        span, step = o.step_of(low, high)
+        if span > 65280:
+            continue
+        small = step < 2.0 ** -14
+        bound = span / 30 + 2.0 ** -21 if small else span / 30 * (1 + 2.0 ** -6)
+        assert span / 30 <= step / 2 <= bound
+        worst["small" if small else "large"] = max(worst["small" if small else "large"], step / 2 / (span / 30))
+        n, s, z = o.quantize(x[None])
+        assert (np.abs(o.values(n, s, z)[0] - x) <= step / 2).all()
+    assert worst["large"] > 1.01 and worst["small"] > 2   # (1/30 of the span alone is no bound)
