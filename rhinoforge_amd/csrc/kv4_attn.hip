@@ -894,12 +894,15 @@ hipError_t launch_sized(AttnArgs a, const PagedPlan& p, hipStream_t stream) {
     if (p.kernel == 1 && p.gangs == 1) kv4_prefill_kernel<T, D, 1><<<grid, kThreads, kLds, stream>>>(a);
     else if (p.kernel == 0 && p.rows == 4 && p.gangs == 2) kv4_decode_kernel<T, D, 1, 4, 8><<<grid, 512, 0, stream>>>(a);
     else if (p.kernel == 0 && p.rows == 8 && p.gangs == 2) kv4_decode_kernel<T, D, 1, 2, 8><<<grid, 512, 0, stream>>>(a);
-    else if (p.kernel == 0 && p.rows == 4) kv4_decode_kernel<T, D, 1, 4, 4><<<grid, kThreads, 0, stream>>>(a);
-    else if (p.kernel == 0 && p.rows == 8) kv4_decode_kernel<T, D, 1, 2, 4><<<grid, kThreads, 0, stream>>>(a);
-    else if (p.kernel == 0 && p.rows == 16) kv4_decode_kernel<T, D, 1, 1, 4><<<grid, kThreads, 0, stream>>>(a);
+    else if (p.kernel == 0 && p.rows == 4 && p.gangs == 1) kv4_decode_kernel<T, D, 1, 4, 4><<<grid, kThreads, 0, stream>>>(a);
+    else if (p.kernel == 0 && p.rows == 8 && p.gangs == 1) kv4_decode_kernel<T, D, 1, 2, 4><<<grid, kThreads, 0, stream>>>(a);
+    else if (p.kernel == 0 && p.rows == 16 && p.gangs == 1) kv4_decode_kernel<T, D, 1, 1, 4><<<grid, kThreads, 0, stream>>>(a);
     else if constexpr (D <= 128) {
-      if (p.kernel == 1) kv4_prefill_kernel<T, D, 2><<<grid, 2 * kThreads, kLds2, stream>>>(a);
-      else kv4_decode_kernel<T, D, 2, 1, 4><<<grid, kThreads, 0, stream>>>(a);
+      if (p.kernel == 1 && p.gangs == 2) kv4_prefill_kernel<T, D, 2><<<grid, 2 * kThreads, kLds2, stream>>>(a);
+      else if (p.kernel == 0 && p.rows == 32 && p.gangs == 1) kv4_decode_kernel<T, D, 2, 1, 4><<<grid, kThreads, 0, stream>>>(a);
+      else return hipErrorInvalidValue;
+    } else {
+      return hipErrorInvalidValue;
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -911,16 +914,10 @@ hipError_t launch_sized(AttnArgs a, const PagedPlan& p, hipStream_t stream) {
 }
 
 struct Kv4Costs {
-  static double base(bool prefill, int rows, int D) {
-    return prefill ? (D == 64 ? 1.1 : D == 128 ? 1.5 : 1.35)
-                   : D == 256 ? 1.1 : (rows <= 16 ? 0.55 : 0.85) * (D == 64 ? 0.75 : 1.0);
-  }
-  static double more(bool prefill, int rows, int D) {
-    return prefill ? (D == 256 ? 0.6 : 0.4) : D == 256 ? 1.2 : (rows <= 16 ? 0.25 : 0.58) * (D == 64 ? 0.6 : 1.0);
-  }
-  static double slots(bool prefill, int gangs, int rows, int D) {
-    return gangs == 2 ? 1.0 : prefill || D == 256 || rows > 16 ? 2.0 : 3.0;
-  }
+  // (of the kernel for many rows alone: the one for few has an estimate of its own)
+  static double base(bool, int, int D) { return D == 64 ? 1.1 : D == 128 ? 1.5 : 1.35; }
+  static double more(bool, int, int D) { return D == 256 ? 0.6 : 0.4; }
+  static double slots(bool, int gangs, int, int) { return gangs == 2 ? 1.0 : 2.0; }
   static double token_bytes(int D) { return D + 4.0; }
   static int few(int64_t rows, int D) { return rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 || D > 128 ? 16 : 32; }
   // Tiles are not cut where they are short, or so many that the CUs have others to go on

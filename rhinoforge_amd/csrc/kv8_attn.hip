@@ -778,10 +778,13 @@ hipError_t launch_sized(AttnArgs a, const PagedPlan& p, hipStream_t stream) {
     a.first = (unsigned)i;
     const unsigned grid = (unsigned)(p.grid - i < most ? p.grid - i : most);
     if (p.kernel == 1 && p.gangs == 1) kv8_prefill_kernel<T, D, 1><<<grid, kThreads, kLds, stream>>>(a);
-    else if (p.kernel == 0 && p.rows == 16) kv8_decode_kernel<T, D, 1><<<grid, kThreads, 0, stream>>>(a);
+    else if (p.kernel == 0 && p.rows == 16 && p.gangs == 1) kv8_decode_kernel<T, D, 1><<<grid, kThreads, 0, stream>>>(a);
     else if constexpr (D <= 128) {
-      if (p.kernel == 1) kv8_prefill_kernel<T, D, 2><<<grid, 2 * kThreads, kLds2, stream>>>(a);
-      else kv8_decode_kernel<T, D, 2><<<grid, kThreads, 0, stream>>>(a);
+      if (p.kernel == 1 && p.gangs == 2) kv8_prefill_kernel<T, D, 2><<<grid, 2 * kThreads, kLds2, stream>>>(a);
+      else if (p.kernel == 0 && p.rows == 32 && p.gangs == 1) kv8_decode_kernel<T, D, 2><<<grid, kThreads, 0, stream>>>(a);
+      else return hipErrorInvalidValue;
+    } else {
+      return hipErrorInvalidValue;
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;

@@ -313,8 +313,8 @@ __device__ __forceinline__ Share share_of(const PagedArgs& a, int g_lo, int g_hi
   return r;
 }
 
-// One 32-token group of a head: where its bytes are and its scales.  A block id
-// outside the cache: block 0 with scales of NaN.
+// One 32-token group of a head: where its bytes are.  A block id outside the cache:
+// block 0, and not ok (the kernels make its scores NaN).
 struct Group {
   int64_t at;  // block * hk + h
   int sub;     // group within the block
@@ -330,7 +330,7 @@ __device__ __forceinline__ Group group_of(const PagedArgs& a, const Tile& t, int
   r.ok = ok;
   return r;
 }
-// Eight query values as fp16 times 2^-e.
+// The largest magnitude of eight query values and m.
 template <typename T>
 __device__ __forceinline__ float load_amax(uint4 v, float m) {
   const floatx8 f = Eight<T>::load(&v);
