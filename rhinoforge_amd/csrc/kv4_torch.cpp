@@ -106,10 +106,10 @@ Two read_hip(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& rows,
   RECORD_FUNCTION("kv4::read", {});
   const char* op = "kv4::read";
   check_read(kc, vc, rows, slots, dtype);
-  const std::vector<int64_t> shape = {slots.size(0), kc.size(1), kc.size(3) * 64};
-  Two out{new_tensor(shape, dtype, kc), new_tensor(shape, dtype, kc)};
   const rf_kv4_cache c = cache_of(kc, vc, rows, op);
   check_same_device(slots, kc, op, "slots");
+  const std::vector<int64_t> shape = {slots.size(0), kc.size(1), kc.size(3) * 64};
+  Two out{new_tensor(shape, dtype, kc), new_tensor(shape, dtype, kc)};
   if (slots.numel() == 0) return out;
   c10::DeviceGuard dev_guard(kc.device());
   check_status(rf_kv4_read(&c, slots.data_ptr<int32_t>(), slots.numel(), dtype_code(dtype),

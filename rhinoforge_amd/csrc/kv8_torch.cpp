@@ -378,10 +378,10 @@ Two read_hip(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks, c
   RECORD_FUNCTION("kv8::read", {});
   const char* op = "kv8::read";
   check_read(kc, vc, ks, vs, slots, dtype);
-  const std::vector<int64_t> shape = {slots.size(0), kc.size(1), kc.size(3) * 32};
-  Two out{new_tensor(shape, dtype, kc), new_tensor(shape, dtype, kc)};
   const rf_kv8_cache c = cache_of(kc, vc, ks, vs, op);
   check_same_device(slots, kc, op, "slots");
+  const std::vector<int64_t> shape = {slots.size(0), kc.size(1), kc.size(3) * 32};
+  Two out{new_tensor(shape, dtype, kc), new_tensor(shape, dtype, kc)};
   if (slots.numel() == 0) return out;
   c10::DeviceGuard dev_guard(kc.device());
   check_status(rf_kv8_read(&c, slots.data_ptr<int32_t>(), slots.numel(), dtype_code(dtype),
