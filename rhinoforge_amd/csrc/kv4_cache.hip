@@ -324,7 +324,10 @@ hipError_t read_sized(ReadArgs a, hipStream_t stream) {
 
 template <typename T>
 hipError_t read_typed(const ReadArgs& a, int D, hipStream_t stream) {
-  // (few entries: in pieces of 8, which leave fewer CUs idle)
+  // Few entries go in pieces of 8, which single tokens need to have enough loads under
+  // way; runs fill one round of workgroups either way (8 heads of 128, pieces of 32 and of
+  // 8: 128 single tokens 4.8 and 3.1 us, 1024 6.7 and 5.5, 4096 13.1 and 13.2; tokens in
+  // runs of 64, 128 of them 3.3 and 4.1, 1024 3.8 and 4.6, 4096 6.9 and 9.7).
   const bool few = a.n * a.heads <= 8192;
   return D == 64    ? few ? read_sized<T, 64, 8>(a, stream) : read_sized<T, 64, 32>(a, stream)
          : D == 128 ? few ? read_sized<T, 128, 8>(a, stream) : read_sized<T, 128, 32>(a, stream)
