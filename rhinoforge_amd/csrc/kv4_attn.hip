@@ -42,10 +42,6 @@ struct AttnArgs : PagedArgs {
 // before their factor are sums of at most 256 products of two fp16 numbers, below 2^41.)
 constexpr float kNothing = -1e30f;
 constexpr float kLeastStep = -24.0f;  // log2 of less than any value step
-// Score factors stay finite and above 0: a masked score is -inf whatever it is
-// multiplied by, and scores beyond these ranges are 0 or infinite to exp2.
-__device__ __forceinline__ float in_range(float factor) { return fminf(fmaxf(factor, 0x1p-126f), 0x1p127f); }
-
 // A row's reference as partial results hold it, in log2 units, -inf where nothing was
 // seen (l = 0), and by how much the rounding moved it, as a factor of the sums.  (At
 // most 2: past 2^24 scores are no more exact than that.  Scores past fp32's range are

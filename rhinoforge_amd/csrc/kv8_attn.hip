@@ -190,6 +190,7 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_decode_kernel(AttnArgs a) {
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) q[r][i] = as_half8(raw[i]);
     }
+    factor[r] = in_range(factor[r]);
     seen(a, t, row, &lo[r], &hi[r]);
   }
   floatx4 acc[RT][D / 16];
@@ -230,7 +231,7 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_decode_kernel(AttnArgs a) {
     bool raise = false;
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-      const float c = as_float(ks) * factor[r];
+      const float c = in_range(as_float(ks) * factor[r]);
       const int first = lo[r] - t0 - 4 * lg, past = hi[r] - t0 - 4 * lg;
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt) s[r][tt] *= c;
@@ -470,6 +471,7 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_prefill_kernel(AttnArgs a) {
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) put_q(i, as_half8(raw[i]));
     }
+    factor = in_range(factor);
     seen(a, t, row, &lo, &hi);
     hi = min(hi, end * 32);
   }
@@ -588,8 +590,8 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_prefill_kernel(AttnArgs a) {
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
       // (not 0, also where ks is 0 or the product underflows: masked scores are
-      // -inf here already, and -inf * 0 is NaN; any score times 2^-126 is 0 to exp2)
-      c[n] = fmaxf(as_float(ks[n]) * factor, 0x1p-126f);
+      // -inf here already, and -inf * 0 is NaN)
+      c[n] = in_range(as_float(ks[n]) * factor);
       most[n] = -__builtin_inff();
 #pragma unroll
       for (int i = 0; i < 16; ++i) most[n] = fmaxf(most[n], s[n][i]);

@@ -357,6 +357,11 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 
 __device__ __forceinline__ float log2_fast(float x) { return __builtin_amdgcn_logf(x); }
 
+// Score factors stay finite and above 0: a masked score is -inf whatever it is
+// multiplied by, a score of 0 is 0, and scores beyond these ranges are 0 or infinite to
+// exp2.
+__device__ __forceinline__ float in_range(float factor) { return fminf(fmaxf(factor, 0x1p-126f), 0x1p127f); }
+
 // A difference of scores, both rounded.  (Taken together with the product that one of
 // them is, in one rounding, it would not be 0 for the largest score.)
 __device__ __forceinline__ float minus(float s, float m) {

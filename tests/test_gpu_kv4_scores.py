@@ -210,3 +210,27 @@ def test_scores_far_below_zero(shape, reach):
         out, lse = _call(q, k, v, table, scale, cached, way)
         assert (np.abs(lse - x) <= ds + 2.0 ** -18 + 2.0 ** -22 * np.abs(x)).all()
         assert (np.abs(out).max(-1) > 0).all()
+
+
+@pytest.mark.parametrize("shape", FEW + MANY, ids=str)
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("form", ["no queries", "no keys"])
+def test_scores_of_zero_under_the_largest_scales(shape, dt, form):
+    """Queries or keys of 0 have scores of 0 whatever the scale: the mean of the values."""
+    _say("zero", shape, dt, form)
+    n, hq, hk, d, cached = shape
+    total = cached + n
+    q, k, v, table, _ = _made(shape, dt, 78, 0, "scale")
+    if form == "no queries":
+        q[:] = 0
+    else:
+        k[0][:], k[2][:] = 8, 8
+        q = q * 2.0 ** (100 if dt == torch.bfloat16 else 0)
+    values = _values(v, table, total, hq)
+    count = np.arange(cached + 1, total + 1)[:, None]
+    want, mass = (np.cumsum(x, 1)[:, cached:] / count for x in (values, np.abs(values)))
+    for scale in (1e37, 3e38):
+        for way in _ways(shape):
+            out, lse = _call(q, k, v, table, scale, cached, way)
+            _near(out, want, mass, dt, total * 2.0 ** -32 * np.abs(values).max(1, keepdims=True))
+            assert (np.abs(lse - np.log(count[:, 0])) <= 2.0 ** -18).all()

@@ -140,3 +140,30 @@ def test_tokens_of_one_key_count_alike(shape, reach, steps):
     for cu in (True, False):
         out, _ = _call(q, (kq, ks, vq, vs), table, total, 2.0 ** reach * d ** -0.5, cu)
         _near(out, want, mass, torch.bfloat16, total * 2.0 ** -32 * 127 * vs.max().item())
+
+
+@pytest.mark.parametrize("shape", FEW + MANY, ids=str)
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("form", ["no queries", "no keys", "no key scale"])
+def test_scores_of_zero_under_the_largest_scales(shape, dt, form):
+    """Queries or keys of 0 have scores of 0 whatever the scale: the mean of the values."""
+    print("zero", shape, dt, form, flush=True)
+    n, hq, hk, d, cached = shape
+    total = cached + n
+    q, (kq, ks, vq, vs), table, _ = _made(shape, dt, 82, 0, "scale")
+    if form == "no queries":
+        q[:] = 0
+    elif form == "no keys":
+        kq[:] = 0
+    else:
+        ks[:] = 0
+    if dt == torch.bfloat16 and form != "no queries":
+        q = q * 2.0 ** 100
+    values = _held(vq, vs, table, total, hq)
+    count = np.arange(cached + 1, total + 1)[:, None]
+    want, mass = (np.cumsum(x, 1)[:, cached:] / count for x in (values, np.abs(values)))
+    for scale in (1e37, 3e38):
+        for cu in (True, False):
+            out, lse = _call(q, (kq, ks, vq, vs), table, total, scale, cu)
+            _near(out, want, mass, dt, total * 2.0 ** -32 * 127 * vs.max().item())
+            assert (np.abs(lse - np.log(count[:, 0])) <= 2.0 ** -18).all()
