@@ -27,7 +27,8 @@
 //     relative, as much as the output's own rounding in fp16.  2^7 times the weight
 //     is what is rounded, the row's largest so far lies in [2^7, 2^15), and what is
 //     below fp16's normal range loses at most 2^-25: 2^-32 of the largest weight.
-//   * m, the sums and o stay in fp32.
+//   * m, the sums and o stay in fp32.  m is a score before its factor, and scores are
+//     taken as differences from it: scores of any size keep their weights.
 #include "kv4_common.h"
 #include "paged_attn.h"
 
