@@ -75,10 +75,10 @@ int rf_kv4_read(const rf_kv4_cache* cache, const int32_t* slots, int64_t n, int3
 /* Attention of a ragged batch's queries over the cache: the fields, the masks, the
  * limits and the workspace of rf_kv8_attention_args.  Scores, sums and softmax
  * statistics are fp32, and scores count by their differences, whatever their size (two
- * of more than fp32 holds in units of ln 2 may count as equal); a token's weight (times its value step, where few rows
- * share a token) is rounded to fp16, to 2^-11 of itself or 2^-32 of the largest one
- * that the row sees.  A query that sees a token which stands for NaN, or one
- * behind a block id outside the cache, gives NaN. */
+ * of more than fp32 holds in units of ln 2 may count as equal); a token's weight
+ * (times its value step, where few rows share a token) is rounded to fp16, to 2^-11 of
+ * itself or 2^-32 of the largest one that the row sees.  A query that sees a token
+ * which stands for NaN, or one behind a block id outside the cache, gives NaN. */
 typedef struct rf_kv4_attention_args {
   rf_kv4_cache cache;
   rf_kv8_heads q;

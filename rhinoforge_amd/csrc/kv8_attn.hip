@@ -250,7 +250,7 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_decode_kernel(AttnArgs a) {
       for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[r][tt][i]);
-      raise |= (mx - run[r].m) + fmaxf(log_vs - run[r].d, 0.0f) > kRaise;  // (NaN: nothing seen yet)
+      raise |= minus(mx, run[r].m) + fmaxf(log_vs - run[r].d, 0.0f) > kRaise;  // (NaN: nothing seen yet)
     }
     if (__ballot(raise)) {
 #pragma unroll
@@ -263,7 +263,7 @@ __attribute__((amdgpu_waves_per_eu(2))) void kv8_decode_kernel(AttnArgs a) {
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
         const float m = fmaxf(run[r].m, mx);
-        const Change f = raise_to(run[r], m, (mx - safe(m)) + log_vs);
+        const Change f = raise_to(run[r], m, minus(mx, safe(m)) + log_vs);
         run[r].l *= f.l;
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) acc[r][i] *= f.o;

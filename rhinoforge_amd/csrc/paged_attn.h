@@ -14,8 +14,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kRaise = 8.0f;  // m follows x from here on: 2^(7 + 8) < 65504
 constexpr float kShift = 7.0f;
-// Scores (log2 units) from which on their differences are taken first: 2^-13 is what
-// rounding one of this size costs.
+// Scores (log2 units) from which on their differences are taken first: rounding one of
+// this size costs 2^-12.
 constexpr float kFar = 4096.0f;
 
 struct PagedArgs {

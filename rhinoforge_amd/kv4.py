@@ -152,8 +152,9 @@ def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.T
     smallest value (or 0) to its largest (or 0): values are off by at most half a
     step, and tokens held before are not touched.  Steps are rounded up to seven
     significant bits, below 2^-14 to multiples of 2^-20: half a step is at most 1/30 of
-    the span and 2^-6 of that more, or 2^-21 more.  A span over 65280 is cut.  A token with an infinity or NaN among the keys or values of a head
-    reads back as NaN there, keys and values.
+    the span and 2^-6 of that more, or 2^-21 more.  A span over 65280 is cut.  A token
+    with an infinity or NaN among the keys or values of a head reads back as NaN there,
+    keys and values.
     """
     _append(*cache.tensors(), k, v, slots)
 
